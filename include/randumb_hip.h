@@ -552,6 +552,40 @@ int rdb_causal_attention_fwd(void *y, void *q, void *k, float *scratch, const vo
 int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const void *q, const void *k, float *scratch, const void *qkv,
                              int64_t batch, int64_t T, int64_t heads, float eps, void *stream);
 
+/* ------------------------------------------------------------------------------------------ ends of a language model
+ * Softmax cross entropy of an output head without its logits: F.cross_entropy(F.linear(x, w), target) of modded-nanogpt/gpt_models.py's head and loss, x [tokens x dim]
+ * and w [classes x dim] both of `dtype` (RDB_F32 or RDB_BF16) with unit inner stride, target int64.  Products, exponentials and sums in fp32 (bf16: on the matrix cores with fp32
+ * sums; fp32: rdb_product_f32's).
+ *   reduction  0: loss[tokens] (0 where target == ignore_index); 1: loss[0], the mean over the other rows (NaN of none); 2: loss[0], their sum
+ *   stats      tokens + 1 floats, for the backward call: log of every row's sum of exponentials, and the number of rows that count
+ * A target outside the classes makes its row's loss and gradients NaN.  Rows with target == ignore_index are not read.
+ * Backward: dloss[tokens] for reduction 0, dloss[0] otherwise; dx [tokens x dim] and dw [classes x dim] contiguous, of `dtype`, overwritten,
+ * 16-byte aligned, NULL where not wanted.  G = (softmax - onehot) is formed from the logits computed again, a piece of the vocabulary at
+ * a time (bf16: rounded to bf16 without the factor that its rows share).  Sums in fixed orders: results are bitwise reproducible.
+ * The workspace's size depends on where w begins.  RDB_E_UNSUPPORTED: x of 2^29 values or more, 2^21 rows or more, ldw of 2^20 or more (size query: 0). */
+int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *w, int64_t ldw, int backward, int want_dx,
+                                                 int want_dw);
+int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
+                                 int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace, int64_t workspace_bytes,
+                                 void *stream);
+int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+                                 const int64_t *target, int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace,
+                                 int64_t workspace_bytes, void *stream);
+
+/* One side's rows: in[b * stride_batch + t * stride_token + h * stride_head + 0 .. head_dim - 1], out contiguous [batch][seq][heads][head_dim]. */
+typedef struct rdb_rotary_rows {
+    void *out;
+    const void *in;
+    int64_t heads, stride_batch, stride_token, stride_head;
+} rdb_rotary_rows;
+/* Rotary positions, Rotary of modded-nanogpt/gpt_models.py:29-49 with other layouts and frequencies: queries, and keys where k is not NULL, of `dtype` (RDB_F32 or
+ * RDB_BF16; fp32 arithmetic, rounded once).  Pair i < pairs of a head at position p, values (i, pairs + i) or, interleaved, (2 i, 2 i + 1):
+ * (a, b) -> (a cos + b sin, b cos - a sin), angle p * inv_freq[i] formed in 64 bits, cosine and sine times scale; inverse: with
+ * -sin, which is the gradient.  The values behind the pairs are copied.  positions: int32 or int64 (pos_bytes) with strides in elements (0 for all
+ * sequences the same), NULL: a token's index.  q and k are descriptions in host memory.  Up to 1024 pairs (RDB_E_UNSUPPORTED otherwise). */
+int rdb_rotary(const rdb_rotary_rows *q, const rdb_rotary_rows *k, int dtype, int64_t batch, int64_t seq, int64_t head_dim, const float *inv_freq, int64_t pairs,
+               const void *positions, int pos_bytes, int64_t pos_stride_batch, int64_t pos_stride_token, int interleaved, float scale, int inverse, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

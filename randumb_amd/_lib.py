@@ -99,6 +99,10 @@ EXPORTS = [
     "rdb_causal_attention_scratch_floats",
     "rdb_causal_attention_fwd",
     "rdb_causal_attention_bwd",
+    "rdb_linear_cross_entropy_workspace_bytes",
+    "rdb_linear_cross_entropy_fwd",
+    "rdb_linear_cross_entropy_bwd",
+    "rdb_rotary",
 ]
 
 ABI_VERSION = 8   # what this binding was written against (rdb_abi_version)
@@ -126,6 +130,13 @@ class LinearDesc(ctypes.Structure):
         ("coef_dtype", ctypes.c_int32),
         ("algo", ctypes.c_int32),
     ]
+
+
+class RotaryRows(ctypes.Structure):
+    """Mirror of ``rdb_rotary_rows``."""
+
+    _fields_ = [("out", ctypes.c_void_p), ("in_", ctypes.c_void_p), ("heads", ctypes.c_int64), ("stride_batch", ctypes.c_int64), ("stride_token", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64)]
 
 
 class RandumbHipError(RuntimeError):
@@ -285,13 +296,19 @@ def load() -> ctypes.CDLL:
     L.rdb_causal_attention_scratch_floats.restype = i64
     L.rdb_causal_attention_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, f32, vp]
     L.rdb_causal_attention_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, vp]
+    L.rdb_linear_cross_entropy_workspace_bytes.argtypes = [i64, i64, i64, ci, vp, i64, ci, ci, ci]
+    L.rdb_linear_cross_entropy_workspace_bytes.restype = i64
+    L.rdb_linear_cross_entropy_fwd.argtypes = [vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
+    L.rdb_linear_cross_entropy_bwd.argtypes = [vp, vp, vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
+    rp = ctypes.POINTER(RotaryRows)
+    L.rdb_rotary.argtypes = [rp, rp, ci, i64, i64, i64, vp, i64, vp, ci, i64, i64, ci, f32, ci, vp]
     for name in ("rdb_sq5_fill_2d", "rdb_sq5_fill_1d", "rdb_materialize_fwd", "rdb_materialize_bwd", "rdb_scale_bias_bwd",
                  "rdb_embed_fwd", "rdb_embed_bwd", "rdb_linear_fwd", "rdb_linear_bwd_dx", "rdb_linear_bwd_dx_dscale", "rdb_linear_rbias_fwd",
                  "rdb_linear_rbias_fwd_ws", "rdb_linear_project_fwd_rbias", "rdb_linear_bwd_projected_rbias", "rdb_linear_rbias_bwd", "rdb_linear_rbias_bwd_to", "rdb_linear_bwd_dcoef",
                  "rdb_linear_project", "rdb_linear_project_fwd", "rdb_linear_fwd_projected", "rdb_linear_bwd_dcoef_projected",
                  "rdb_linear_bwd_projected", "rdb_linear_bwd_projected_to", "rdb_linear_bwd_projected_part",
                  "rdb_rms_norm_fwd", "rdb_rms_norm_bwd", "rdb_relu_square", "rdb_cross_entropy_fwd", "rdb_cross_entropy_bwd",
-                 "rdb_causal_attention_fwd", "rdb_causal_attention_bwd"):
+                 "rdb_causal_attention_fwd", "rdb_causal_attention_bwd", "rdb_linear_cross_entropy_fwd", "rdb_linear_cross_entropy_bwd", "rdb_rotary"):
         getattr(L, name).restype = ci
     _lib = L
     return L

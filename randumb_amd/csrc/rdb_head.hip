@@ -1,0 +1,1018 @@
+// Softmax cross entropy of an output head, x . W^T over a large vocabulary, and its gradient, in pieces of the vocabulary: the logits are
+// never kept, and neither is their gradient.
+//
+//   lse[t] = log sum_v exp <x_t, w_v>,  nll[t] = lse[t] - <x_t, w_target[t]>,  loss = their mean, their sum, or nll itself
+//   G[t][v] = (exp(<x_t, w_v> - lse[t]) - [v == target[t]]) g_t,   dx = G . W,   dW = G^T . x
+//
+// Rows whose target is the ignored label are left out before anything is multiplied (head_gather_kernel): they cost nothing, and what they hold, NaN
+// included, reaches no sum.  A target outside the classes makes its row NaN.
+//
+// bf16 (products on 256-wide tiles, rdb_big.hpp):
+//   head_gather_kernel    the rows that count, one after the other, in rows of a multiple of 8 values
+//   head_stats_kernel     a 256 x 256 tile of logits in the accumulators -> its maximum and its sum of exponentials for each token
+//   head_merge_kernel     those of a token together, the target's logit, nll
+//   head_loss_kernel      the sum over the tokens
+//   head_grad_kernel      the logits of a piece of the vocabulary once more -> G, in bf16, for the next launch
+//   head_products_kernel  dx += G . W and dW = G^T . x of the piece, one list of tiles
+//   head_dx_kernel        dx from its sums, back in the rows' own places
+// G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
+// which are nearly all of the gradient, would all be off by the same rounding.
+// fp32: the same steps with the products of rdb_f32.hip, logits of a piece in fp32 in between.
+#include "rdb_big.hpp"
+#include <algorithm>
+
+namespace rdb {
+
+int num_compute_units();
+
+constexpr int HD_TILE = 256;
+constexpr float HD_LOG2E = 1.44269504088896340736f, HD_LN2 = 0.69314718055994530942f;
+enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
+
+// ----------------------------------------------------------------------------------------------- the rows that count
+struct HeadGather {
+    void *xc;                // [tokens][ldc]: the rows that count, in order; fp32: every row in its place, ignored ones zeros
+    const void *x;
+    int64_t ldx, ldc;
+    const int64_t *target;
+    int *pos;                // [tokens]: where a row went, -1: ignored
+    int *count;              // rows that count
+    // backward, by place: log2 of the row's sum, target (-1: none of the classes), its own factor of G
+    float *lse2, *factor;
+    int *label;
+    const float *stats;      // lse by row
+    const float *dloss;      // [tokens], or NULL: 1
+    int64_t tokens, dim, classes, ignore;
+    int rows;                // per block
+    bool wide;               // x may be read 16 bytes at a time
+};
+// Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.
+template <typename E, bool COMPACT> __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
+{
+    __shared__ int before_[4], place_[64];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const int64_t r0 = (int64_t)blockIdx.x * p.rows;
+    const int mine = p.tokens - r0 < p.rows ? (int)(p.tokens - r0) : p.rows;
+    if (COMPACT) {
+        int n = 0;
+        for (int64_t i = t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
+        if (lane == 0) before_[wave] = n;
+        __syncthreads();
+    }
+    if (wave == 0) {
+        const int64_t c = lane < mine ? p.target[r0 + lane] : p.ignore;
+        const bool counts = c != p.ignore;
+        const unsigned long long all = __ballot(counts);
+        const int first = COMPACT ? before_[0] + before_[1] + before_[2] + before_[3] : 0;
+        const int at = COMPACT ? first + __popcll(all & ((1ull << lane) - 1)) : (int)(r0 + lane);
+        place_[lane] = counts ? at : -1;
+        if (lane < mine) {
+            p.pos[r0 + lane] = counts ? at : -1;
+            if (p.lse2 && (counts || !COMPACT)) {
+                const bool known = c >= 0 && c < p.classes;
+                p.lse2[at] = p.stats[r0 + lane] * HD_LOG2E;
+                p.label[at] = known ? (int)c : -1;
+                p.factor[at] = !counts ? 0.0f : !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
+            }
+        }
+        if (COMPACT && lane == 0 && r0 + mine == p.tokens) *p.count = first + __popcll(all);
+    }
+    __syncthreads();
+    constexpr int PER = 16 / (int)sizeof(E);
+    const int chunks = (int)(p.ldc / PER);
+    const E *x = static_cast<const E *>(p.x);
+    E *xc = static_cast<E *>(p.xc);
+    for (int i = t; i < mine * chunks; i += 256) {
+        const int row = i / chunks, c = (i - row * chunks) * PER;
+        const int at = place_[row];
+        if (at < 0 && COMPACT) continue;
+        const E *src = x + (r0 + row) * p.ldx + c;
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0) {
+            if (p.wide && c + PER <= p.dim) {
+                v = *reinterpret_cast<const f32x4 *>(src);
+            } else {
+                E e[PER];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) e[j] = c + j < p.dim ? src[j] : E(0);
+                __builtin_memcpy(&v, e, 16);
+            }
+        }
+        *reinterpret_cast<f32x4 *>(xc + (COMPACT ? (int64_t)at : r0 + row) * p.ldc + c) = v;
+    }
+}
+
+// rows of `cols` bf16 values from one leading dimension to another; the columns behind them become zeros up to a multiple of 8 where `pad`
+__global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int cols, int out_cols)
+{
+    const int64_t n = rows * out_cols, stride = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const int64_t row = i / out_cols;
+        const int c = (int)(i - row * out_cols);
+        dst[row * ldd + c] = c < cols ? src[row * lds + c] : (bf16_t)0;
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- logits, in the accumulators
+struct HeadLogits {
+    const bf16_t *x;      // the rows that count, [*count][ldx]
+    const bf16_t *w;      // [classes][ldw]
+    int64_t ldx, ldw;
+    const int *count;
+    int dim, classes, v0;     // classes v0 .. v0 + tiles_v * 256 of this launch
+    int tiles_v, tiles_t;
+    float2 *part;         // stats: [2 * tiles_v][tokens]: maximum (times log2 e) and sum
+    int64_t tokens;
+    bf16_t *g;            // gradient: [tokens][ldg], class v0 first
+    int64_t ldg;
+    const float *lse2, *factor;
+    const int *label;
+};
+// as big_y_decode: 32 neighbouring items, which a die runs at a time, share 8 tiles of the weight and 4 of the tokens
+__device__ __forceinline__ void head_decode(int w, int tiles_v, int tiles_t, int &tv, int &tt)
+{
+    const int per_group = 4 * tiles_v, group = w / per_group, in_group = w - group * per_group, first = group * 4;
+    const int size = min(4, tiles_t - first);
+    tv = in_group / size;
+    tt = first + in_group - tv * size;
+}
+__device__ __forceinline__ int head_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
+
+// maximum and sum of exponentials over the tile's classes, for each of the wave's tokens; each wave leaves its 128 classes' own
+template <int NI>
+__device__ __forceinline__ void head_leave_stats(f32x16 (&acc)[4][NI], const HeadLogits &p, int tv, int tok0, int count, int t)
+{
+    const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
+    const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;   // classes of this wave's rows that there are
+    acc_settle<4, NI>(acc);
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+        float v[64], m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = acc_read(acc[i >> 4][ni][i & 15]);
+        if (left < 128) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+                if ((i >> 4) * 32 + head_row(i & 15, g) >= left) v[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) m = fmaxf(m, v[i]);
+        m = fmaxf(m, __shfl_xor(m, 32, 64)) * HD_LOG2E;
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], HD_LOG2E, -ref));
+        s += __shfl_xor(s, 32, 64);
+        const int tok = tok0 + wn * NI * 32 + ni * 32 + r;
+        if (g == 0 && tok < count) p.part[(int64_t)(tv * 2 + wm) * p.tokens + tok] = float2{m, s};
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// G of the tile, through LDS into whole rows; classes past the last one are zeros
+template <int NI>
+__device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[4][NI], bf16_t *__restrict__ lds, const HeadLogits &p, int tv, int tok0, int count, int t)
+{
+    constexpr int BN = NI * 64, LD = HD_TILE + 8;
+    const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
+    const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;
+    acc_settle<4, NI>(acc);
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+        const int b = wn * NI * 32 + ni * 32 + r, tok = min(tok0 + b, count - 1);
+        const float l = p.lse2[tok], f = p.factor[tok];
+        const int rel = p.label[tok] - first;
+        float v[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc_read(acc[i >> 4][ni][i & 15]), HD_LOG2E, -l));
+        if (__any((unsigned)rel < 128u)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+                if ((i >> 4) * 32 + head_row(i & 15, g) == rel) v[i] -= 1.0f;
+        }
+        if (left < 128) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+                if ((i >> 4) * 32 + head_row(i & 15, g) >= left) v[i] = 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            store4<bf16_t>(lds + b * LD + wm * 128 + (q >> 2) * 32 + 8 * (q & 3) + 4 * g, v[q * 4] * f, v[q * 4 + 1] * f, v[q * 4 + 2] * f, v[q * 4 + 3] * f);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    bf16_t *out = p.g + (int64_t)tok0 * p.ldg + (int64_t)tv * HD_TILE;
+    const int a = (t & 31) * 8;
+#pragma unroll 8
+    for (int q = 0; q < BN / 8; ++q) {
+        const int b = q * 8 + (t >> 5);
+        if (tok0 + b < count) *reinterpret_cast<f32x4 *>(out + (int64_t)b * p.ldg + a) = *reinterpret_cast<const f32x4 *>(lds + b * LD + a);
+    }
+    __syncthreads();
+}
+
+template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logits_kernel(HeadLogits p)
+{
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    bf16_t *lds = reinterpret_cast<bf16_t *>(smem_raw);
+    typedef GlobalOperand<HD_TILE, 64, K_CONT> PA;
+    typedef GlobalOperand<BN, 64, K_CONT> PB;
+    const int count = *p.count, tiles_t = (count + BN - 1) / BN, total = p.tiles_v * tiles_t, vtotal = (total + 7) / 8 * 8, nstage = (p.dim + 63) / 64;
+    int v = (int)blockIdx.x;
+    auto next = [&]() {
+        for (; v < vtotal; v += gridDim.x) {
+            const int w = xcd_work_item(v, total);
+            if (w < total) {
+                v += gridDim.x;
+                return w;
+            }
+        }
+        return -1;
+    };
+    PA pa;
+    PB pb;
+    BigRegs<PA, PB> regs;
+    auto request = [&](int w) {
+        int tv, tt;
+        head_decode(w, p.tiles_v, tiles_t, tv, tt);
+        const int row = p.v0 + tv * HD_TILE, rows = min(HD_TILE, p.classes - row), tok = tt * BN, toks = min(BN, count - tok);
+        pa = PA{p.w + (int64_t)row * p.ldw, p.ldw, 0, rows, p.dim, (int64_t)(rows - 1) * p.ldw + p.dim};
+        pb = PB{p.x + (int64_t)tok * p.ldx, p.ldx, 0, toks, p.dim, (int64_t)(toks - 1) * p.ldx + p.dim};
+        big_prefetch(regs, pa, pb, 0);
+    };
+    int w = next();
+    if (w < 0) return;
+    request(w);
+    while (true) {
+        int tv, tt;
+        head_decode(w, p.tiles_v, tiles_t, tv, tt);
+        f32x16 acc[4][BN / 64];
+        big_zero<HD_TILE, BN>(acc);
+        big_mainloop<HD_TILE, BN>(acc, lds, regs, pa, pb, nstage);
+        const int wn = next();
+        if (wn >= 0) request(wn);   // on its way during the epilogue
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (GRAD) head_leave_grad<BN / 64>(acc, lds, p, tv, tt * BN, count, opaque_tid());
+        else head_leave_stats<BN / 64>(acc, p, tv, tt * BN, count, opaque_tid());
+        if (wn < 0) break;
+        w = wn;
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- loss
+struct HeadMerge {
+    float *stats;          // [tokens]: lse, 0 in ignored rows
+    float *nll;            // [tokens]
+    const float2 *part;    // [parts][tokens], by place
+    const int *pos;
+    const bf16_t *x, *w;
+    int64_t ldx, ldw, tokens, classes;
+    const int64_t *target;
+    int parts, dim;        // dim: a multiple of 8, zeros behind the last value
+};
+// Sixteen lanes a token, sixteen tokens a block.
+__global__ __launch_bounds__(256) void head_merge_kernel(HeadMerge p)
+{
+    const int t = threadIdx.x, slot = t >> 4, part = t & 15;
+    __shared__ float ms_[16][17], ss_[16][17];
+    const int64_t r0 = (int64_t)blockIdx.x * 16;
+    {   // neighbouring lanes: neighbouring tokens, as the parts lie; then over to the token's own lanes
+        const int64_t row = r0 + part;
+        const int at = row < p.tokens ? p.pos[row] : -1;
+        float m = -INFINITY, s = 0.0f;
+        if (at >= 0)
+#pragma unroll 4
+            for (int i = slot; i < p.parts; i += 16) {
+                const float2 q = p.part[(int64_t)i * p.tokens + at];
+                const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
+                s = s * __builtin_amdgcn_exp2f(m - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
+                m = top;
+            }
+        ms_[part][slot] = m;
+        ss_[part][slot] = s;
+    }
+    __syncthreads();
+    const int64_t row = r0 + slot;
+    if (row >= p.tokens) return;   // all sixteen lanes of the token
+    const int at = p.pos[row];
+    if (at < 0) {
+        if (part == 0) {
+            p.stats[row] = 0.0f;
+            p.nll[row] = 0.0f;
+        }
+        return;
+    }
+    float m = ms_[slot][part], s = ss_[slot][part];
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+        s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
+        m = top;
+    }
+    const float lse = (m + log2f(s)) * HD_LN2;
+    const int64_t c = p.target[row];
+    const bool known = c >= 0 && c < p.classes;
+    float d = 0.0f;
+    if (known) {
+        const bf16_t *x = p.x + (int64_t)at * p.ldx, *w = p.w + c * p.ldw;
+#pragma unroll 2
+        for (int i = part * 8; i < p.dim; i += 128) {
+            const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) d += __shfl_xor(d, o, 64);
+    if (part == 0) {
+        p.stats[row] = lse;
+        p.nll[row] = known ? lse - d : __uint_as_float(0x7fc00000u);
+    }
+}
+
+// loss[0] = sum of nll (/ rows that count), count beside it.  One block, fixed order.
+__global__ __launch_bounds__(1024) void head_loss_kernel(float *__restrict__ loss, float *__restrict__ count, const float *__restrict__ nll,
+                                                         const int64_t *__restrict__ target, int64_t rows, int64_t ignore, int mean)
+{
+    __shared__ float s[16];
+    __shared__ int n[16];
+    float a = 0.0f;
+    int c = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+        if (loss) a += nll[i];
+        c += target[i] == ignore ? 0 : 1;
+    }
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) {
+        a += __shfl_xor(a, m, 64);
+        c += __shfl_xor(c, m, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        s[threadIdx.x >> 6] = a;
+        n[threadIdx.x >> 6] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a = 0.0f;
+        c = 0;
+        for (int w = 0; w < 16; ++w) {
+            a += s[w];
+            c += n[w];
+        }
+        if (loss) loss[0] = mean ? a / (float)c : a;
+        count[0] = (float)c;
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- dx and dW
+// The factor that all of G's rows share.  No rows: nothing to scale.
+struct HeadScale {
+    const float *dloss;   // NULL: 1 (rows have factors of their own)
+    const float *count;   // NULL: a sum
+    __device__ __forceinline__ float value() const { return !dloss ? 1.0f : !count ? dloss[0] : count[0] > 0.0f ? dloss[0] / count[0] : 0.0f; }
+};
+struct HeadProducts {
+    const bf16_t *g, *x, *w;   // w: the piece's first class
+    int64_t ldg, ldx, ldw;
+    const int *count;
+    int rows_v, dim;           // classes of the piece
+    float *dx;                 // [splits][tokens][lddx] sums, or NULL
+    int64_t lddx, dx_stride, tokens;
+    bool add;                  // to the sums that are there
+    int splits, split_v;       // a split's classes, a multiple of 64
+    bf16_t *dw;                // the piece's first row of [classes][lddw], or NULL
+    int64_t lddw;
+    HeadScale scale;
+    int tiles_t, tiles_d, tiles_v;
+};
+// D[a][b] to out[a * ld + b], as big_store_rows, times a factor (bf16) or added to what is there (fp32)
+template <typename E, bool ADD>
+__device__ __forceinline__ void head_store_rows(f32x16 (&acc)[4][4], bf16_t *__restrict__ lds, E *__restrict__ out, int64_t ld, int na, int b0, int nb, float scale, int t)
+{
+    constexpr int LDP = 128 + 4, PER = 16 / (int)sizeof(E), LPR = 128 / PER, RPP = 64 / LPR;
+    const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
+    float *patch = reinterpret_cast<float *>(lds) + wave * 32 * LDP;
+    acc_settle<4, 4>(acc);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)(((int64_t)(na - 1) * ld + nb) * (int)sizeof(E)), 0x00020000);
+    const int col = (lane % LPR) * PER, b = b0 + wn * 128 + col;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi) {
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) patch[head_row(j, g) * LDP + ni * 32 + r] = acc_read(acc[mi][ni][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 32 / RPP; ++q) {
+            const int row = q * RPP + lane / LPR, a = wm * 128 + mi * 32 + row;
+            const uint32_t off = (a < na && b < nb) ? (uint32_t)(((int64_t)a * ld + b) * (int)sizeof(E)) : BUFFER_OOB_ANY;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(patch + row * LDP + col);
+            if constexpr (sizeof(E) == 2) {
+                const f32x4 u = *reinterpret_cast<const f32x4 *>(patch + row * LDP + col + 4);
+                const i32x4 h = {(int)f32x2_to_bf16x2(v[0] * scale, v[1] * scale), (int)f32x2_to_bf16x2(v[2] * scale, v[3] * scale),
+                                 (int)f32x2_to_bf16x2(u[0] * scale, u[1] * scale), (int)f32x2_to_bf16x2(u[2] * scale, u[3] * scale)};
+                __builtin_amdgcn_raw_buffer_store_b128(h, rs, (int)off, 0, 2);
+            } else {
+                if (ADD) {
+                    const f32x4 o = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += o[e];
+                }
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rs, (int)off, 0, 0);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+}
+
+// A list of tiles: n of them behind `base` others of the launch
+template <class F> __device__ __forceinline__ int head_next(int &r, int base, int n, F)
+{
+    const int nv = (n + 7) / 8 * 8;
+    for (;; ++r) {
+        const int v = big_item((int)blockIdx.x, r, (int)gridDim.x) - base;
+        if (v >= nv) return -1;
+        if (v < 0) continue;
+        const int w = xcd_work_item(v, n);
+        if (w < n) {
+            ++r;
+            return w;
+        }
+    }
+}
+template <bool ADD> __device__ __forceinline__ void head_dx_items(const HeadProducts &p, bf16_t *lds, int count, int tiles_t, int &r, int base, int n)
+{
+    typedef GlobalOperand<HD_TILE, 64, K_CONT> PA;   // G: rows = tokens, contraction = classes
+    typedef GlobalOperand<HD_TILE, 64, M_CONT> PB;   // W: rows = its columns
+    PA pa;
+    PB pb;
+    BigRegs<PA, PB> regs;
+    auto decode = [&](int w, int &s, int &tt, int &td) {   // neighbours share G's rows
+        td = w % p.tiles_d;
+        w /= p.tiles_d;
+        tt = w % tiles_t;
+        s = w / tiles_t;
+    };
+    auto request = [&](int w) {
+        int s, tt, td;
+        decode(w, s, tt, td);
+        const int v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE, toks = min(HD_TILE, count - tok);
+        pa = PA{p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7, (int64_t)(toks - 1) * p.ldg + ((vs + 7) & ~7)};
+        pb = PB{p.w + (int64_t)v0 * p.ldw, p.ldw, td * HD_TILE, p.dim, vs, (int64_t)(vs - 1) * p.ldw + p.dim};
+        big_prefetch(regs, pa, pb, 0);
+    };
+    int w = head_next(r, base, n, 0);
+    if (w < 0) return;
+    request(w);
+    while (true) {
+        int s, tt, td;
+        decode(w, s, tt, td);
+        f32x16 acc[4][4];
+        big_zero<HD_TILE, HD_TILE>(acc);
+        big_mainloop<HD_TILE, HD_TILE>(acc, lds, regs, pa, pb, (min(p.split_v, p.rows_v - s * p.split_v) + 63) / 64);
+        const int wn = head_next(r, base, n, 0);
+        if (wn >= 0) request(wn);
+        __builtin_amdgcn_sched_barrier(0);
+        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tt * HD_TILE * p.lddx, p.lddx, min(HD_TILE, count - tt * HD_TILE), td * HD_TILE, p.dim,
+                                    1.0f, opaque_tid());
+        if (wn < 0) break;
+        w = wn;
+    }
+}
+__device__ __forceinline__ void head_dw_items(const HeadProducts &p, bf16_t *lds, int count, int &r, int base, int n)
+{
+    typedef GlobalOperand<HD_TILE, 64, M_CONT> PA;   // G: rows = classes, contraction = tokens
+    typedef GlobalOperand<HD_TILE, 64, M_CONT> PB;   // x: rows = its columns
+    PA pa;
+    PB pb;
+    BigRegs<PA, PB> regs;
+    auto request = [&](int w) {
+        const int tv = w / p.tiles_d, td = w % p.tiles_d;
+        pa = PA{p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count, (int64_t)count * p.ldg};
+        pb = PB{p.x, p.ldx, td * HD_TILE, p.dim, count, (int64_t)count * p.ldx};   // no rows: nothing is read, dW becomes zeros
+        big_prefetch(regs, pa, pb, 0);
+    };
+    const float scale = p.scale.value();
+    int w = head_next(r, base, n, 0);
+    if (w < 0) return;
+    request(w);
+    while (true) {
+        const int tv = w / p.tiles_d, td = w % p.tiles_d;
+        f32x16 acc[4][4];
+        big_zero<HD_TILE, HD_TILE>(acc);
+        big_mainloop<HD_TILE, HD_TILE>(acc, lds, regs, pa, pb, (count + 63) / 64);
+        const int wn = head_next(r, base, n, 0);
+        if (wn >= 0) request(wn);
+        __builtin_amdgcn_sched_barrier(0);
+        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), td * HD_TILE, p.dim, scale, opaque_tid());
+        if (wn < 0) break;
+        w = wn;
+    }
+}
+__global__ __launch_bounds__(256, 1) void head_products_kernel(HeadProducts p)
+{
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    bf16_t *lds = reinterpret_cast<bf16_t *>(smem_raw);
+    const int count = *p.count, tiles_t = (count + HD_TILE - 1) / HD_TILE;
+    const int n1 = p.dx ? p.splits * tiles_t * p.tiles_d : 0, n1v = (n1 + 7) / 8 * 8, n2 = p.dw ? p.tiles_v * p.tiles_d : 0;
+    int r = 0;
+    if (n1) {
+        if (p.add) head_dx_items<true>(p, lds, count, tiles_t, r, 0, n1);
+        else head_dx_items<false>(p, lds, count, tiles_t, r, 0, n1);
+    }
+    if (n2) head_dw_items(p, lds, count, r, n1v, n2);
+}
+// dx[row] = factor * the sums of its place over the splits, rounded once; zeros in ignored rows
+__global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, const float *__restrict__ sums, const int *__restrict__ pos, int64_t tokens, int dim,
+                                                      int64_t ld, int64_t stride, int splits, HeadScale scale)
+{
+    const float f = scale.value();
+    const int chunks = (int)(ld / 4);
+    const int64_t n = tokens * chunks;
+    const bool whole = dim % 4 == 0;   // rows of dx begin on 8 bytes then
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / chunks;
+        const int c = (int)(i - row * chunks) * 4, at = pos[row];
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0) {
+            for (int s = 0; s < splits; ++s) {
+                const f32x4 u = *reinterpret_cast<const f32x4 *>(sums + s * stride + at * ld + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += u[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= f;
+        }
+        bf16_t *out = dx + row * dim + c;
+        if (whole) {
+            if (c < dim) *reinterpret_cast<uint2 *>(out) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < dim) out[e] = f32_to_bf16(v[e]);
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- fp32: rows of a piece of logits
+struct HeadRows {
+    float *logits;         // [tokens][n], n classes from v0 on; G in their place
+    float2 *state;         // [tokens]: maximum (times log2 e) and sum of the pieces so far
+    float *picked;         // [tokens]: the target's logit
+    const int *pos;
+    const float *lse2, *factor;
+    const int *label;
+    const int64_t *target;
+    float *stats, *nll;
+    HeadScale scale;
+    int64_t tokens, classes, ignore;
+    int n, v0, first, last;
+};
+__device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
+{
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
+    m = top;
+}
+// One block a row.
+__global__ __launch_bounds__(256) void head_rows_stats_kernel(HeadRows p)
+{
+    __shared__ float ms_[4], ss_[4];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x;
+    const int64_t c = p.target[row];
+    if (c == p.ignore) {
+        if (p.last && t == 0) {
+            p.stats[row] = 0.0f;
+            p.nll[row] = 0.0f;
+        }
+        return;
+    }
+    const float *l = p.logits + row * p.n;
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll 4
+    for (int i = t; i < p.n; i += 256) {
+        const float v = l[i], top = fmaxf(m, v), ref = top == -INFINITY ? 0.0f : top;
+        s = s * __expf(m - ref) + __expf(v - ref);
+        m = top;
+    }
+    m *= HD_LOG2E;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    if ((t & 63) == 0) {
+        ms_[t >> 6] = m;
+        ss_[t >> 6] = s;
+    }
+    __syncthreads();
+    if (t) return;
+    for (int w = 1; w < 4; ++w) head_join(m, s, ms_[w], ss_[w]);
+    if (!p.first) head_join(m, s, p.state[row].x, p.state[row].y);
+    const bool known = c >= 0 && c < p.classes;
+    float picked = p.first || !known ? 0.0f : p.picked[row];
+    if (known && c >= p.v0 && c < p.v0 + p.n) picked = l[c - p.v0];
+    if (!p.last) {
+        p.state[row] = float2{m, s};
+        p.picked[row] = picked;
+        return;
+    }
+    const float lse = (m + log2f(s)) * HD_LN2;
+    p.stats[row] = lse;
+    p.nll[row] = known ? lse - picked : __uint_as_float(0x7fc00000u);
+}
+__global__ __launch_bounds__(256) void head_rows_grad_kernel(HeadRows p)
+{
+    const int64_t row = blockIdx.x;
+    float *l = p.logits + row * p.n;
+    const float f = p.pos[row] < 0 ? 0.0f : p.factor[row] * p.scale.value(), lse = p.stats[row];
+    const int label = p.label[row] - p.v0;
+    const bool skip = p.pos[row] < 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.n; i += 256) {
+        float v = expf(l[i] - lse);
+        if (i == label) v -= 1.0f;
+        l[i] = skip ? 0.0f : v * f;
+    }
+}
+__global__ __launch_bounds__(256) void head_add_kernel(float *__restrict__ out, const float *__restrict__ a, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] += a[i];
+}
+
+// ----------------------------------------------------------------------------------------------- plan and calls
+// Bytes of a piece's G (bf16) or logits (fp32): what the next launch finds in the chip's last-level cache, and tiles enough to fill it.
+constexpr int64_t HD_PIECE_BYTES = 256ll << 20;
+
+struct HeadPlan {
+    int64_t tokens, dim, classes;
+    int dtype;
+    bool backward, want_dx, want_dw, pack_w, pad_dw;
+    int64_t dp, vp;            // columns of the copies; classes of a piece
+    int pieces, bn, splits;
+    int64_t split_v;
+    // offsets in the workspace
+    int64_t xc, pos, count, lse2, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
+};
+static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, bool backward, bool want_dx, bool want_dw, bool pack_w)
+{
+    HeadPlan h = {};
+    h.tokens = tokens;
+    h.dim = dim;
+    h.classes = classes;
+    h.dtype = dtype;
+    h.backward = backward;
+    h.want_dx = want_dx;
+    h.want_dw = want_dw;
+    const bool f32 = dtype == RDB_F32;
+    const int64_t es = f32 ? 4 : 2;
+    h.dp = f32 ? (dim + 3) / 4 * 4 : (dim + 7) / 8 * 8;
+    h.pack_w = !f32 && pack_w;
+    h.pad_dw = !f32 && h.dp != dim;
+    int64_t cols = HD_PIECE_BYTES / (es * tokens) / HD_TILE * HD_TILE;
+    if (f32) cols = std::min<int64_t>(cols, ((1ll << 29) - 1) / std::max<int64_t>(tokens, h.dp) / HD_TILE * HD_TILE);
+    else cols = std::min<int64_t>(cols, ((1ll << 28)) / h.dp / HD_TILE * HD_TILE);
+    cols = std::max<int64_t>(cols, HD_TILE);
+    h.pieces = (int)cdiv(classes, cols);
+    h.vp = cdiv(cdiv(classes, h.pieces), HD_TILE) * HD_TILE;
+    if (f32 && h.pieces == 1) h.vp = classes;
+    h.pieces = (int)cdiv(classes, h.vp);
+    h.bn = tokens <= 64 ? 64 : tokens <= 128 ? 128 : 256;
+    const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, HD_TILE);
+    int64_t splits = std::max<int64_t>(1, num_compute_units() / std::max<int64_t>(1, tiles));
+    splits = std::min(splits, std::max<int64_t>(1, h.vp / 1024));
+    splits = std::min<int64_t>(splits, 16);
+    h.split_v = cdiv(cdiv(h.vp, splits), 64) * 64;
+    h.splits = (int)cdiv(std::min(h.vp, classes), h.split_v);   // the first piece's: it writes all the sums that there are
+    int64_t at = 0;
+    auto room = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += (bytes + 255) / 256 * 256;
+        return o;
+    };
+    h.xc = room(tokens * h.dp * es);
+    h.pos = room(tokens * 4);
+    h.count = room(4);
+    if (h.pack_w) h.wc = room(classes * h.dp * 2);
+    if (!backward) {
+        h.nll = room(tokens * 4);
+        if (f32) {
+            h.part = room(tokens * 8);
+            h.picked = room(tokens * 4);
+            h.g = room(tokens * h.vp * 4);
+        } else {
+            h.part = room(2 * cdiv(classes, HD_TILE) * tokens * 8);
+        }
+    } else {
+        h.lse2 = room(tokens * 4);
+        h.factor = room(tokens * 4);
+        h.label = room(tokens * 4);
+        h.g = room(tokens * h.vp * es);
+        if (want_dx && (!f32 || h.pieces > 1)) h.dx = room((f32 ? 1 : h.splits) * tokens * (f32 ? dim : h.dp) * 4);
+        if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2);
+    }
+    if (f32) {
+        h.product_bytes = rdb_product_f32_workspace_bytes(tokens, h.vp, dim);
+        if (h.pieces > 1) h.product_bytes = std::max(h.product_bytes, rdb_product_f32_workspace_bytes(tokens, classes - (h.pieces - 1) * h.vp, dim));
+        if (backward)
+            for (int64_t n : {h.vp, classes - (h.pieces - 1) * h.vp}) {
+                if (want_dx) h.product_bytes = std::max(h.product_bytes, rdb_product_f32_workspace_bytes(tokens, dim, n));
+                if (want_dw) h.product_bytes = std::max(h.product_bytes, rdb_product_f32_workspace_bytes(n, dim, tokens));
+            }
+        h.product = room(h.product_bytes);
+    }
+    h.total = at;
+    return h;
+}
+
+struct HeadCall {
+    const HeadPlan &h;
+    char *ws;
+    const void *x, *w;
+    int64_t ldx, ldw;
+    const int64_t *target;
+    int64_t ignore;
+    hipStream_t s;
+    template <typename T> T *at(int64_t offset) const { return reinterpret_cast<T *>(ws + offset); }
+};
+static bool head_aligned(const void *p, int64_t ld, int es) { return !((uintptr_t)p & 15) && ld * es % 16 == 0; }
+
+static int head_gather(const HeadCall &c, const float *stats, const float *dloss_rows)
+{
+    const HeadPlan &h = c.h;
+    const bool f32 = h.dtype == RDB_F32;
+    HeadGather p = {};
+    p.xc = c.at<void>(h.xc);
+    p.x = c.x;
+    p.ldx = c.ldx;
+    p.ldc = h.dp;
+    p.target = c.target;
+    p.pos = c.at<int>(h.pos);
+    p.count = c.at<int>(h.count);
+    if (h.backward) {
+        p.lse2 = c.at<float>(h.lse2);
+        p.factor = c.at<float>(h.factor);
+        p.label = c.at<int>(h.label);
+        p.stats = stats;
+        p.dloss = dloss_rows;
+    }
+    p.tokens = h.tokens;
+    p.dim = h.dim;
+    p.classes = h.classes;
+    p.ignore = c.ignore;
+    p.rows = h.tokens > 16384 ? 64 : 16;
+    p.wide = head_aligned(c.x, c.ldx, f32 ? 4 : 2);
+    const unsigned grid = (unsigned)cdiv(h.tokens, p.rows);
+    if (f32) head_gather_kernel<float, false><<<grid, 256, 0, c.s>>>(p);
+    else head_gather_kernel<bf16_t, true><<<grid, 256, 0, c.s>>>(p);
+    return check_launch("head_gather_kernel");
+}
+static int head_repack(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, int64_t out_cols, hipStream_t s)
+{
+    const int64_t blocks = std::min<int64_t>(cdiv(rows * out_cols, 2048), 16384);
+    head_repack_kernel<<<(unsigned)blocks, 256, 0, s>>>(dst, ldd, src, lds, rows, (int)cols, (int)out_cols);
+    return check_launch("head_repack_kernel");
+}
+// the weight as the tiles read it: rows from 16-byte boundaries on
+static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
+{
+    *w = static_cast<const bf16_t *>(c.w);
+    *ldw = c.ldw;
+    if (!c.h.pack_w) return RDB_OK;
+    bf16_t *wc = c.at<bf16_t>(c.h.wc);
+    const int rc = head_repack(wc, c.h.dp, *w, c.ldw, c.h.classes, c.h.dim, c.h.dp, c.s);
+    *w = wc;
+    *ldw = c.h.dp;
+    return rc;
+}
+
+template <class K, class P> static int head_launch(K kernel, const P &p, int64_t items, size_t smem, hipStream_t s, const char *name)
+{
+    if (int rl = reserve_lds(reinterpret_cast<const void *>(kernel), smem, name)) return rl;
+    int64_t blocks = std::max<int64_t>(8, num_compute_units() / 8 * 8);   // a multiple of 8: a block's tiles stay on one die's share of the list
+    blocks = std::min<int64_t>(blocks, (items + 7) / 8 * 8);
+    kernel<<<(unsigned)blocks, 256, smem, s>>>(p);
+    return check_launch(name);
+}
+template <int BN, bool GRAD> static int head_logits_on(const HeadLogits &p, hipStream_t s)
+{
+    return head_launch(head_logits_kernel<BN, GRAD>, p, (int64_t)p.tiles_v * p.tiles_t,
+                       big_smem<HD_TILE, BN, OperandTile<HD_TILE, 64, K_CONT>, OperandTile<BN, 64, K_CONT>>(), s, GRAD ? "head_logits_kernel<gradient>" : "head_logits_kernel");
+}
+template <bool GRAD> static int head_logits(HeadLogits &p, int bn, hipStream_t s)
+{
+    p.tiles_t = (int)cdiv(p.tokens, bn);
+    return bn == 64 ? head_logits_on<64, GRAD>(p, s) : bn == 128 ? head_logits_on<128, GRAD>(p, s) : head_logits_on<256, GRAD>(p, s);
+}
+
+static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduction)
+{
+    const HeadPlan &h = c.h;
+    if (int rc = head_gather(c, nullptr, nullptr)) return rc;
+    const bf16_t *w;
+    int64_t ldw;
+    if (int rc = head_weight(c, &w, &ldw)) return rc;
+    HeadLogits p = {};
+    p.x = c.at<bf16_t>(h.xc);
+    p.ldx = h.dp;
+    p.w = w;
+    p.ldw = ldw;
+    p.count = c.at<int>(h.count);
+    p.dim = (int)h.dp;
+    p.classes = (int)h.classes;
+    p.tiles_v = (int)cdiv(h.classes, HD_TILE);
+    p.part = c.at<float2>(h.part);
+    p.tokens = h.tokens;
+    if (int rc = head_logits<false>(p, h.bn, c.s)) return rc;
+    float *nll = reduction == HD_NONE ? loss : c.at<float>(h.nll);
+    const HeadMerge m = {stats, nll, p.part, c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.tokens, h.classes, c.target, 2 * p.tiles_v, (int)h.dp};
+    head_merge_kernel<<<(unsigned)cdiv(h.tokens, 16), 256, 0, c.s>>>(m);
+    return check_launch("head_merge_kernel");
+}
+static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float *dloss, const float *stats, int reduction)
+{
+    const HeadPlan &h = c.h;
+    if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr)) return rc;
+    const bf16_t *w;
+    int64_t ldw;
+    if (int rc = head_weight(c, &w, &ldw)) return rc;
+    const HeadScale scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
+    bf16_t *dwc = h.pad_dw && dw ? c.at<bf16_t>(h.dw) : dw;
+    const int *count = c.at<int>(h.count);
+    for (int i = 0; i < h.pieces; ++i) {
+        const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
+        HeadLogits p = {};
+        p.x = c.at<bf16_t>(h.xc);
+        p.ldx = h.dp;
+        p.w = w;
+        p.ldw = ldw;
+        p.count = count;
+        p.dim = (int)h.dp;
+        p.classes = (int)h.classes;
+        p.v0 = (int)v0;
+        p.tiles_v = (int)cdiv(n, HD_TILE);
+        p.tokens = h.tokens;
+        p.g = c.at<bf16_t>(h.g);
+        p.ldg = h.vp;
+        p.lse2 = c.at<float>(h.lse2);
+        p.factor = c.at<float>(h.factor);
+        p.label = c.at<int>(h.label);
+        if (int rc = head_logits<true>(p, h.bn, c.s)) return rc;
+        HeadProducts q = {};
+        q.g = p.g;
+        q.ldg = h.vp;
+        q.x = p.x;
+        q.ldx = h.dp;
+        q.w = w + v0 * ldw;
+        q.ldw = ldw;
+        q.count = count;
+        q.rows_v = (int)n;
+        q.dim = (int)h.dp;
+        q.tokens = h.tokens;
+        if (dx) {
+            q.dx = c.at<float>(h.dx);
+            q.lddx = h.dp;
+            q.dx_stride = h.tokens * h.dp;
+            q.add = i > 0;
+            q.split_v = (int)h.split_v;
+            q.splits = (int)cdiv(n, h.split_v);
+        }
+        if (dw) {
+            q.dw = dwc + v0 * h.dp;
+            q.lddw = h.dp;
+        }
+        q.scale = scale;
+        q.tiles_t = (int)cdiv(h.tokens, HD_TILE);
+        q.tiles_d = (int)cdiv(h.dp, HD_TILE);
+        q.tiles_v = p.tiles_v;
+        const int64_t items = (dx ? (int64_t)q.splits * q.tiles_t * q.tiles_d + 7 : 0) + (dw ? (int64_t)q.tiles_v * q.tiles_d : 0);
+        if (int rc = head_launch(head_products_kernel, q, items, big_smem<HD_TILE, HD_TILE, OperandTile<HD_TILE, 64, M_CONT>, OperandTile<HD_TILE, 64, M_CONT>>(), c.s,
+                                 "head_products_kernel"))
+            return rc;
+    }
+    if (dx) {
+        const int64_t blocks = std::min<int64_t>(cdiv(h.tokens * h.dp / 4, 256), 8192);
+        head_dx_kernel<<<(unsigned)blocks, 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale);
+        if (int rc = check_launch("head_dx_kernel")) return rc;
+    }
+    if (dw && h.pad_dw) return head_repack(dw, h.dim, dwc, h.dp, h.classes, h.dim, h.dim, c.s);
+    return RDB_OK;
+}
+
+static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduction)
+{
+    const HeadPlan &h = c.h;
+    if (int rc = head_gather(c, nullptr, nullptr)) return rc;
+    HeadRows p = {};
+    p.logits = c.at<float>(h.g);
+    p.state = c.at<float2>(h.part);
+    p.picked = c.at<float>(h.picked);
+    p.target = c.target;
+    p.stats = stats;
+    p.nll = reduction == HD_NONE ? loss : c.at<float>(h.nll);
+    p.tokens = h.tokens;
+    p.classes = h.classes;
+    p.ignore = c.ignore;
+    for (int i = 0; i < h.pieces; ++i) {
+        const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
+        if (int rc = rdb_product_f32(p.logits, c.at<float>(h.xc), h.dp, 0, static_cast<const float *>(c.w) + v0 * c.ldw, c.ldw, 0, nullptr, h.tokens, n, h.dim,
+                                     c.at<void>(h.product), h.product_bytes, c.s))
+            return rc;
+        p.n = (int)n;
+        p.v0 = (int)v0;
+        p.first = i == 0;
+        p.last = i + 1 == h.pieces;
+        head_rows_stats_kernel<<<(unsigned)h.tokens, 256, 0, c.s>>>(p);
+        if (int rc = check_launch("head_rows_stats_kernel")) return rc;
+    }
+    return RDB_OK;
+}
+static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dloss, const float *stats, int reduction)
+{
+    const HeadPlan &h = c.h;
+    if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr)) return rc;
+    HeadRows p = {};
+    p.logits = c.at<float>(h.g);
+    p.pos = c.at<int>(h.pos);
+    p.factor = c.at<float>(h.factor);
+    p.label = c.at<int>(h.label);
+    p.stats = const_cast<float *>(stats);
+    p.scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
+    for (int i = 0; i < h.pieces; ++i) {
+        const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
+        const float *w = static_cast<const float *>(c.w) + v0 * c.ldw, *xc = c.at<float>(h.xc);
+        void *room = c.at<void>(h.product);
+        if (int rc = rdb_product_f32(p.logits, xc, h.dp, 0, w, c.ldw, 0, nullptr, h.tokens, n, h.dim, room, h.product_bytes, c.s)) return rc;
+        p.n = (int)n;
+        p.v0 = (int)v0;
+        head_rows_grad_kernel<<<(unsigned)h.tokens, 256, 0, c.s>>>(p);
+        if (int rc = check_launch("head_rows_grad_kernel")) return rc;
+        if (dx) {
+            float *to = i ? c.at<float>(h.dx) : dx;
+            if (int rc = rdb_product_f32(to, p.logits, n, 0, w, c.ldw, 1, nullptr, h.tokens, h.dim, n, room, h.product_bytes, c.s)) return rc;
+            if (i) {
+                head_add_kernel<<<(unsigned)std::min<int64_t>(cdiv(h.tokens * h.dim, 1024), 4096), 256, 0, c.s>>>(dx, to, h.tokens * h.dim);
+                if (int rc = check_launch("head_add_kernel")) return rc;
+            }
+        }
+        if (dw)
+            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, xc, h.dp, 1, nullptr, n, h.dim, h.tokens, room, h.product_bytes, c.s)) return rc;
+    }
+    return RDB_OK;
+}
+
+static int check_head(const char *who, int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldx, int64_t ldw, int reduction)
+{
+    if (dtype != RDB_BF16 && dtype != RDB_F32) return set_error(RDB_E_DTYPE, "%s: x and w in fp32 or bf16", who);
+    if (tokens <= 0 || dim <= 0 || classes <= 0 || classes >= (1ll << 31) - HD_TILE || ldx < dim || ldw < dim || reduction < 0 || reduction > 2)
+        return set_error(RDB_E_SHAPE, "%s: bad size %lld x %lld x %lld, leading dimensions %lld and %lld, or reduction %d", who, (long long)tokens, (long long)dim,
+                         (long long)classes, (long long)ldx, (long long)ldw, reduction);
+    // 32-bit offsets within an operand: x in rows of a multiple of 8 values, a tile of W's rows, a piece of G
+    if ((dim + 7) / 8 * 8 * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29) || tokens >= (1ll << 21) || ldw >= (1ll << 20))
+        return set_error(RDB_E_UNSUPPORTED, "%s: x of less than 2^29 values and 2^21 rows, rows of w less than 2^20 apart", who);
+    return RDB_OK;
+}
+
+}  // namespace rdb
+
+using namespace rdb;
+
+extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *w, int64_t ldw, int backward, int want_dx,
+                                                            int want_dw)
+{
+    if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, dim, ldw, 0)) return 0;
+    return head_plan(tokens, dim, classes, dtype, backward != 0, want_dx != 0, want_dw != 0, !head_aligned(w, ldw, 2) || dim % 8).total;
+}
+
+extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
+                                            int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace, int64_t workspace_bytes,
+                                            void *stream)
+{
+    constexpr const char *who = "rdb_linear_cross_entropy_fwd";
+    if (int rc = check_head(who, tokens, dim, classes, dtype, ldx, ldw, reduction)) return rc;
+    if (!loss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
+    const HeadPlan h = head_plan(tokens, dim, classes, dtype, false, false, false, !head_aligned(w, ldw, 2) || dim % 8);
+    if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
+    const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
+    if (int rc = dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, reduction) : head_fwd_bf16(c, loss, stats, reduction)) return rc;
+    head_loss_kernel<<<1, 1024, 0, c.s>>>(reduction == HD_NONE ? nullptr : loss, stats + tokens, c.at<float>(h.nll), target, tokens, ignore_index, reduction == HD_MEAN);
+    return check_launch("head_loss_kernel");
+}
+
+extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+                                            const int64_t *target, int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace,
+                                            int64_t workspace_bytes, void *stream)
+{
+    constexpr const char *who = "rdb_linear_cross_entropy_bwd";
+    if (int rc = check_head(who, tokens, dim, classes, dtype, ldx, ldw, reduction)) return rc;
+    if (!dx && !dw) return RDB_OK;
+    if (!dloss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
+    if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return set_error(RDB_E_ALIGN, "%s: dx and dw must be 16-byte aligned", who);
+    const HeadPlan h = head_plan(tokens, dim, classes, dtype, true, dx != nullptr, dw != nullptr, !head_aligned(w, ldw, 2) || dim % 8);
+    if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
+    const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
+    return dtype == RDB_F32 ? head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, reduction)
+                            : head_bwd_bf16(c, static_cast<bf16_t *>(dx), static_cast<bf16_t *>(dw), dloss, stats, reduction);
+}

@@ -1117,6 +1117,117 @@ class CausalAttention : public Function<CausalAttention> {
     }
 };
 
+// ----------------------------------------------------------------------------------------------- ends of a language model
+// loss of x (tokens, dim) against a weight (classes, dim) that never become logits; the argument checks are ops.linear_cross_entropy's
+class LinearCrossEntropy : public Function<LinearCrossEntropy> {
+  public:
+    // unit inner stride, rows less than 2^20 values apart
+    static Tensor rows(const Tensor &t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) < (1 << 20) ? t : t.contiguous(); }
+    static Tensor forward(AutogradContext *ctx, const Tensor &x0, const Tensor &w0, const Tensor &target0, int64_t ignore, int64_t reduction)
+    {
+        const Tensor x = rows(x0), w = rows(w0), target = target0.contiguous();
+        const c10::OptionalDeviceGuard guard(x.device());
+        const int64_t tokens = x.size(0), dim = x.size(1), classes = w.size(0);
+        const auto f32 = x.options().dtype(at::kFloat);
+        Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32);
+        if (tokens) {
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), w.data_ptr(), w.stride(0), 0, 0, 0);
+            const Tensor ws = bytes(need, x);
+            check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), code(x.scalar_type()),
+                                               target.data_ptr<int64_t>(), tokens, dim, classes, ignore, (int)reduction, ptr(ws), need, stream_of(x)),
+                  "rdb_linear_cross_entropy_fwd");
+        } else {
+            loss.fill_(reduction == 1 ? NAN : 0.0f);
+        }
+        ctx->save_for_backward({x0, w0, target, stats});
+        ctx->saved_data["m"] = std::vector<int64_t>{tokens, dim, classes, ignore, reduction};
+        return loss;
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads)
+    {
+        auto d = gradients(ctx, grads[0]);
+        for (Tensor &t : d) t = once_differentiable("linear_cross_entropy", t, grads[0], {0, 1});
+        return {d[0], d[1], Tensor(), Tensor(), Tensor()};
+    }
+    static variable_list gradients(AutogradContext *ctx, const Tensor &grad)
+    {
+        const at::AutoGradMode no_grad(false);
+        const auto saved = ctx->get_saved_variables();
+        const auto m = ctx->saved_data["m"].toIntVector();   // tokens, dim, classes, ignored label, reduction
+        constexpr const char *who = "linear_cross_entropy (backward)";
+        const Tensor dloss = grad.to(at::kFloat).contiguous();
+        const Tensor x = rows(restored(who, saved[0], dloss, {m[0], m[1]})), w = rows(restored(who, saved[1], dloss, {m[2], m[1]}));
+        if (!readable(x.scalar_type()) || x.scalar_type() != w.scalar_type()) fail(PyExc_RuntimeError, std::string(who) + ": a saved tensor came back as something else");
+        restored_values(who, saved[2], dloss, at::kLong, m[0]);
+        restored_values(who, saved[3], dloss, at::kFloat, m[0] + 1);
+        const c10::OptionalDeviceGuard guard(x.device());
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        Tensor dx, dw;
+        if (want_x) dx = at::empty({m[0], m[1]}, x.options());
+        if (want_w) dw = m[0] ? at::empty({m[2], m[1]}, w.options()) : at::zeros({m[2], m[1]}, w.options());
+        if (m[0] && (want_x || want_w)) {
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), w.data_ptr(), w.stride(0), 1, want_x, want_w);
+            const Tensor ws = bytes(need, x);
+            check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                               code(x.scalar_type()), saved[2].data_ptr<int64_t>(), m[0], m[1], m[2], m[3], (int)m[4], ptr(ws), need, stream_of(x)),
+                  "rdb_linear_cross_entropy_bwd");
+        }
+        return {dx, dw};
+    }
+};
+
+// queries and keys (or none) turned by their positions; its own gradient, with the sine's sign turned
+class Rotary : public Function<Rotary> {
+  public:
+    static Tensor inner(const Tensor &t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
+    static variable_list forward(AutogradContext *ctx, const Tensor &q0, const OptTensor &k0, const Tensor &inv_freq0, const OptTensor &positions0, bool interleaved, double scale,
+                                 bool inverse)
+    {
+        const Tensor q = inner(q0), k = k0 ? inner(*k0) : Tensor(), f = inv_freq0.contiguous(), pos = positions0 ? *positions0 : Tensor();
+        const c10::OptionalDeviceGuard guard(q.device());
+        Tensor oq = at::empty(q.sizes(), q.options()), ok = k.defined() ? at::empty(k.sizes(), k.options()) : Tensor();
+        auto rows = [](const Tensor &out, const Tensor &in) { return rdb_rotary_rows{out.data_ptr(), in.data_ptr(), in.size(2), in.stride(0), in.stride(1), in.stride(2)}; };
+        const rdb_rotary_rows rq = rows(oq, q), rk = k.defined() ? rows(ok, k) : rdb_rotary_rows{};
+        const bool each = pos.defined() && pos.dim() == 2 && pos.size(0) != 1;
+        check(rdb_rotary(&rq, k.defined() ? &rk : nullptr, code(q.scalar_type()), q.size(0), q.size(1), q.size(3), f.data_ptr<float>(), f.numel(), ptr(pos),
+                         pos.defined() ? (int)pos.element_size() : 0, each ? pos.stride(0) : 0, pos.defined() ? pos.stride(-1) : 0, interleaved, (float)scale, inverse,
+                         stream_of(q)),
+              "rdb_rotary");
+        ctx->save_for_backward({f, pos});
+        ctx->saved_data["m"] = std::vector<int64_t>{interleaved, inverse, k.defined(), q.size(0), q.size(1), q.size(2), k.defined() ? k.size(2) : 0, q.size(3), (int64_t)q.scalar_type(), f.numel(),
+                                                    pos.defined() ? pos.numel() : 0};
+        ctx->saved_data["scale"] = scale;
+        ctx->set_materialize_grads(false);
+        return k.defined() ? variable_list{oq, ok} : variable_list{oq};
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const auto m = ctx->saved_data["m"].toIntVector();
+        const bool keys = m[2];
+        variable_list g(2);
+        const Tensor &some = grads[0].defined() ? grads[0] : keys ? grads[1] : grads[0];
+        if (!some.defined()) return variable_list(7);
+        constexpr const char *who = "rotary (backward)";
+        restored_values(who, saved[0], some, at::kFloat, m[9]);
+        const Tensor &pos = saved[1];
+        if (m[10]) {
+            same_device(who, some, {&pos});
+            if ((pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) || pos.numel() != m[10] || pos.dim() < 1 || pos.dim() > 2 || pos.size(-1) != m[4])
+                fail(PyExc_RuntimeError, std::string(who) + ": a saved tensor came back as something else");
+        }
+        // a side whose gradient nobody has, or wants, is left out; keys alone take the queries' place
+        const bool want_q = grads[0].defined() && ctx->needs_input_grad(0), want_k = keys && grads[1].defined() && ctx->needs_input_grad(1);
+        if (!want_q && !want_k) return variable_list(7);
+        auto typed = [&](const Tensor &t) { return t.to((at::ScalarType)m[8]); };
+        const variable_list got = Rotary::apply(typed(want_q ? grads[0] : grads[1]), want_q && want_k ? OptTensor(typed(grads[1])) : OptTensor(), saved[0],
+                                                m[10] ? OptTensor(pos) : OptTensor(), (bool)m[0], ctx->saved_data["scale"].toDouble(), !m[1]);
+        if (want_q) g[0] = got[0];
+        if (want_k) g[1] = got[want_q ? 1 : 0];
+        return {g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
 // The sizes the descriptor states are those of the tensors: the library is told in_f and out_f and reads that far.
 void check_sizes(const char *who, const Tensor &x, const Tensor &c, const Layer &l, const OptTensor &scale, const Bias &b)
 {
@@ -1412,6 +1523,47 @@ PyObject *py_causal_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// linear_cross_entropy(x, weight, target, ignore_index, reduction): of ops.linear_cross_entropy, which has checked types and sizes
+PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject * {
+        count_args(n, 5);
+        const Tensor &x = tensor_arg(a[0]), &w = tensor_arg(a[1]), &t = tensor_arg(a[2]);
+        same_device("linear_cross_entropy", x, {&w, &t});
+        if (!past_dispatcher({&x, &w, &t})) Py_RETURN_NONE;
+        const int64_t reduction = int_arg(a[4]);
+        if (x.dim() != 2 || w.dim() != 2 || t.dim() != 1 || x.size(1) != w.size(1) || t.size(0) != x.size(0) || !w.numel() || t.scalar_type() != at::kLong ||
+            !readable(x.scalar_type()) || w.scalar_type() != x.scalar_type() || reduction < 0 || reduction > 2)
+            fail(PyExc_ValueError, "linear_cross_entropy needs x (tokens, dim) and a weight (classes, dim) of one type, int64 targets (tokens) and a reduction 0, 1 or 2");
+        return THPVariable_Wrap(LinearCrossEntropy::apply(x, w, t, int_arg(a[3]), reduction));
+    });
+}
+
+// rotary(q, k or None, inv_freq, positions or None, interleaved, scale): of ops.rotary, which has checked types and sizes
+PyObject *py_rotary(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return guarded([&]() -> PyObject * {
+        count_args(n, 6);
+        const Tensor &q = tensor_arg(a[0]), &f = tensor_arg(a[2]);
+        const OptTensor k = opt_arg(a[1]), pos = opt_arg(a[3]);
+        same_device("rotary", q, {address(k), &f, address(pos)});
+        if (!past_dispatcher({&q, address(k), &f, address(pos)})) Py_RETURN_NONE;
+        const int interleaved = PyObject_IsTrue(a[4]);
+        if (interleaved < 0) throw BadArgument();
+        if (q.dim() != 4 || !readable(q.scalar_type()) || (k && (k->dim() != 4 || k->scalar_type() != q.scalar_type() || k->size(0) != q.size(0) || k->size(1) != q.size(1) ||
+                                                                  k->size(3) != q.size(3))) ||
+            f.dim() != 1 || f.scalar_type() != at::kFloat || 2 * f.numel() > q.size(3) ||
+            (pos && ((pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt) || pos->dim() < 1 || pos->dim() > 2 || pos->size(-1) != q.size(1) ||
+                     (pos->dim() == 2 && pos->size(0) != 1 && pos->size(0) != q.size(0)))))
+            fail(PyExc_ValueError, "rotary needs queries and keys (batch, time, heads, head_dim) of one type, fp32 frequencies and positions (time) or (batch, time)");
+        const variable_list out = Rotary::apply(q, k, f.detach(), pos, interleaved != 0, float_arg(a[5]), false);
+        PyObject *both = PyTuple_New((Py_ssize_t)out.size());
+        if (!both) throw BadArgument();
+        for (size_t i = 0; i < out.size(); ++i) PyTuple_SET_ITEM(both, (Py_ssize_t)i, THPVariable_Wrap(out[i]));
+        return both;
+    });
+}
+
 // once_differentiable(grad, dy, input, input): for the functions in Python, called from their backward passes (negative: no input)
 PyObject *py_once_differentiable(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
@@ -1440,6 +1592,7 @@ PyMethodDef methods[] = {RDB_METHOD(takes_projected),   RDB_METHOD(linear_projec
                          RDB_METHOD(rms_norm),          RDB_METHOD(add_rms_norm),     RDB_METHOD(relu_square),
                          RDB_METHOD(embedding),
                          RDB_METHOD(cross_entropy),     RDB_METHOD(causal_attention), RDB_METHOD(once_differentiable),
+                         RDB_METHOD(linear_cross_entropy), RDB_METHOD(rotary),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rdb_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -1466,5 +1619,7 @@ PyMODINIT_FUNC PyInit__rdb_torch(void)
     name_node<ReluSquare>("ReluSquareBackward");
     name_node<CrossEntropy>("CrossEntropyBackward");
     name_node<CausalAttention>("CausalAttentionBackward");
+    name_node<LinearCrossEntropy>("LinearCrossEntropyBackward");
+    name_node<Rotary>("RotaryBackward");
     return PyModule_Create(&module);
 }

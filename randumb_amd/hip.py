@@ -865,3 +865,67 @@ def set_big_tiles(mode: int) -> int:
     2 = 256-wide tiles whenever k > 256.  y and dx are the same bit for bit either way, dcoef up to the order of fp32 sums over
     token ranges; with the fused random bias mode 0 rounds y and dx once more.  Returns the previous mode."""
     return int(_lib.load().rdb_set_big_tiles(int(mode)))
+
+
+# ------------------------------------------------------------------------------------------------ ends of a language model
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix as the head's kernels read it: unit inner stride, rows less than 2^20 values apart."""
+    return t if t.stride(1) == 1 and t.shape[1] <= t.stride(0) < 1 << 20 else t.contiguous()
+
+
+def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int):
+    """``(loss, stats)`` of the rows ``x`` (tokens, dim) and the weight (classes, dim), both fp32 or both bf16, for int64 targets; reduction 0: a loss
+    for each row, 1: their mean, 2: their sum.  ``stats`` (fp32, tokens + 1) is what the backward call needs."""
+    _need_gpu("linear_cross_entropy", x, weight, target)
+    x, w, t = _rows(x), _rows(weight), target.contiguous()
+    tokens, dim = x.shape
+    dev, L = x.device, _lib.load()
+    loss = torch.empty((tokens,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+    stats = torch.empty((tokens + 1,), dtype=torch.float32, device=dev)
+    if tokens == 0:
+        return loss.fill_(float("nan") if reduction == 1 else 0.0), stats.zero_()
+    with _on(dev):
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(w), w.stride(0), 0, 0, 0))
+        ws = _workspace(n, dev)
+        rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
+                                            _p(ws), n, _stream(dev))
+    _lib.check(rc, "rdb_linear_cross_entropy_fwd")
+    return loss, stats
+
+
+def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int,
+                             want_dx: bool = True, want_dw: bool = True):
+    """``(dx, dweight)`` of :func:`linear_cross_entropy_fwd`, ``None`` where not wanted; ``dloss`` one value, or one for each row with reduction 0."""
+    _need_gpu("linear_cross_entropy", dloss, stats, x, weight, target)
+    x, w, t, d, stats = _rows(x), _rows(weight), target.contiguous(), dloss.to(torch.float32).contiguous(), stats.contiguous()
+    tokens, dim = x.shape
+    if d.numel() != (tokens if reduction == 0 else 1) or stats.dtype != torch.float32 or stats.numel() != tokens + 1:
+        raise ValueError("linear_cross_entropy: a gradient or statistics of another size")
+    dev, L = x.device, _lib.load()
+    dx = torch.empty((tokens, dim), dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty((w.shape[0], dim), dtype=w.dtype, device=dev) if want_dw else None
+    if tokens == 0:
+        return dx, None if dw is None else dw.zero_()
+    with _on(dev):
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(w), w.stride(0), 1, want_dx, want_dw))
+        ws = _workspace(n, dev)
+        rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
+                                            ignore_index, reduction, _p(ws), n, _stream(dev))
+    _lib.check(rc, "rdb_linear_cross_entropy_bwd")
+    return dx, dw
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, positions: Optional[torch.Tensor], interleaved: bool, scale: float, inverse: bool = False):
+    """``(q, k)`` (batch, time, heads, head_dim) turned by their positions; ``inverse``: the other way round, which is the gradient."""
+    _need_gpu("rotary", q, k, inv_freq, positions)
+    q, k = (None if t is None else t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
+    out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    rows = [None if t is None else ctypes.byref(_lib.RotaryRows(o.data_ptr(), t.data_ptr(), t.shape[2], t.stride(0), t.stride(1), t.stride(2)))
+            for t, o in zip((q, k), out)]
+    f = inv_freq.contiguous()
+    pb, pt = (0, 0) if positions is None else (0, positions.stride(0)) if positions.dim() == 1 else (0 if positions.shape[0] == 1 else positions.stride(0), positions.stride(1))
+    with _on(q.device):
+        rc = _lib.load().rdb_rotary(rows[0], rows[1], _DT[q.dtype], q.shape[0], q.shape[1], q.shape[3], _p(f), f.numel(), _p(positions),
+                                    0 if positions is None else positions.element_size(), pb, pt, interleaved, scale, inverse, _stream(q.device))
+    _lib.check(rc, "rdb_rotary")
+    return out[0], out[1]

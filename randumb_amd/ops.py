@@ -8,10 +8,13 @@ Additive to the reference surface:
   (the reference types it ``Tensor`` yet documents ``None`` as the default, RandumbTensor.py:993);
 * ``materialize_bwd`` takes an optional ``coef_rows``;
 * ``rten::linear_fwd`` / ``linear_bwd_dx`` / ``linear_bwd_dcoef``: the fused products that never write the
-  weight (or its gradient) to memory.
+  weight (or its gradient) to memory;
+* :func:`linear_cross_entropy` and :func:`rotary`: the loss of a language model's output head, whose logits are never kept, and rotary
+  positions in the layouts and with the frequencies of such models.
 """
 from __future__ import annotations
 
+import math
 from typing import List, Optional
 
 import torch
@@ -23,7 +26,7 @@ from . import _lib, hip
 __all__ = [
     "materialize_fwd", "materialize_bwd", "scale_bias_bwd", "embed_fwd", "embed_bwd",
     "linear_fwd", "linear_bwd_dx", "linear_bwd_dcoef", "linear", "linear_project", "linear_project_fwd", "linear_fwd_projected",
-    "linear_bwd_dcoef_projected", "linear_bwd_projected", "sq5_gen_2d", "sq5_gen_1d",
+    "linear_bwd_dcoef_projected", "linear_bwd_projected", "linear_cross_entropy", "rotary", "rotary_frequencies", "sq5_gen_2d", "sq5_gen_1d",
 ]
 
 
@@ -488,6 +491,165 @@ def embed_rows(idx: Tensor, coefs: Tensor, rowsize: int, seed: int) -> Tensor:
     if idx.is_cuda and coefs.is_cuda and not _tracing():
         y = (_lib._ext or _lib.extension()).embed_rows(idx, coefs, rowsize, seed)
     return embed_fwd(idx, coefs, rowsize, seed) if y is None else y
+
+
+# ------------------------------------------------------------------------------------------------ rten::linear_cross_entropy_*
+@custom_op("rten::linear_cross_entropy_fwd", mutates_args=())
+def linear_cross_entropy_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> List[Tensor]:
+    """``[loss, stats]``, see :func:`linear_cross_entropy`; the second is what the backward pass needs of the first."""
+    return list(hip.linear_cross_entropy_fwd(x, weight, target, ignore_index, reduction))
+
+
+@linear_cross_entropy_fwd.register_fake
+def _(x, weight, target, ignore_index, reduction):
+    f32 = dict(dtype=torch.float32)
+    return [x.new_empty([x.shape[0]] if reduction == 0 else [], **f32), x.new_empty([x.shape[0] + 1], **f32)]
+
+
+@custom_op("rten::linear_cross_entropy_bwd", mutates_args=())
+def linear_cross_entropy_bwd(dloss: Tensor, stats: Tensor, x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int, want_dx: bool,
+                             want_dweight: bool) -> List[Tensor]:
+    """The wanted ones of ``[dx, dweight]``."""
+    both = hip.linear_cross_entropy_bwd(dloss, stats, x, weight, target, ignore_index, reduction, want_dx, want_dweight)
+    return [g for g in both if g is not None]
+
+
+@linear_cross_entropy_bwd.register_fake
+def _(dloss, stats, x, weight, target, ignore_index, reduction, want_dx, want_dweight):
+    return [t.new_empty(list(t.shape)) for t, wanted in ((x, want_dx), (weight, want_dweight)) if wanted]
+
+
+def _lce_setup_context(ctx, inputs, output):
+    x, weight, target, ctx.ignore_index, ctx.reduction = inputs
+    ctx.save_for_backward(x, weight, target, output[1])
+
+
+def _lce_backward(ctx, grads):
+    x, weight, target, stats = ctx.saved_tensors
+    want = ctx.needs_input_grad[:2]
+    if grads[0] is None or not any(want):
+        return None, None, None, None, None
+    got = iter(linear_cross_entropy_bwd(grads[0], stats, x, weight, target, ctx.ignore_index, ctx.reduction, *want))
+    return next(got) if want[0] else None, next(got) if want[1] else None, None, None, None
+
+
+linear_cross_entropy_fwd.register_autograd(_lce_backward, setup_context=_lce_setup_context)
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """``F.cross_entropy(F.linear(x, weight).float(), target, ignore_index=..., reduction=...)`` for a large vocabulary, with its gradients and without
+    the logits: neither they nor their gradient are ever in memory beyond a piece of the vocabulary.
+
+    ``x`` (..., dim) and ``weight`` (classes, dim): both bf16 or both fp32, on one GPU; ``target`` (...): int64 or int32.  The loss is fp32; logits are
+    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out of the work: what their rows hold does not matter.  The mean over no tokens is
+    NaN, with gradients of zero; a target outside the classes makes its token's loss and gradients NaN.  First derivatives only."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if hasattr(weight, "get_materialized") or hasattr(x, "get_materialized"):
+        raise TypeError("linear_cross_entropy: dense tensors, not pseudorandom ones")
+    if x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
+        raise TypeError(f"linear_cross_entropy: x and weight both bfloat16 or both float32, got {x.dtype} and {weight.dtype}")
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"linear_cross_entropy: target int64 or int32, got {target.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or target.shape != x.shape[:-1] or weight.numel() == 0:
+        raise ValueError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)} do not go together")
+    ignore_index, code = int(ignore_index), _REDUCTIONS[reduction]
+    rows, labels = x.reshape(-1, x.shape[-1]), target.reshape(-1).long()
+    loss = None
+    if not _tracing() and x.is_cuda:
+        loss = (_lib._ext or _lib.extension()).linear_cross_entropy(rows, weight, labels, ignore_index, code)
+    if loss is None:
+        loss = linear_cross_entropy_fwd(rows, weight, labels, ignore_index, code)[0]
+    return loss.reshape(target.shape) if code == 0 else loss
+
+
+# ------------------------------------------------------------------------------------------------ rten::rotary
+@custom_op("rten::rotary", mutates_args=())
+def _rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional[Tensor], interleaved: bool, scale: float, inverse: bool) -> List[Tensor]:
+    return [t for t in hip.rotary(q, k, inv_freq, positions, interleaved, scale, inverse) if t is not None]
+
+
+@_rotary.register_fake
+def _(q, k, inv_freq, positions, interleaved, scale, inverse):
+    return [t.new_empty(list(t.shape)) for t in (q, k) if t is not None]
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    q, k, inv_freq, positions, ctx.interleaved, ctx.scale, ctx.inverse = inputs
+    ctx.save_for_backward(inv_freq, positions)
+    ctx.shapes = [None if t is None else (list(t.shape), t.dtype) for t in (q, k)]
+
+
+def _rotary_backward(ctx, grads):
+    inv_freq, positions = ctx.saved_tensors
+    grads = [g if g is not None else torch.zeros(s[0], dtype=s[1], device=inv_freq.device) for g, s in zip(list(grads) + [None], ctx.shapes) if s is not None]
+    got = _rotary(grads[0], grads[1] if len(grads) > 1 else None, inv_freq, positions, ctx.interleaved, ctx.scale, not ctx.inverse)
+    return got[0], got[1] if len(got) > 1 else None, None, None, None, None, None
+
+
+_rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup_context)
+
+
+def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional[Tensor] = None, *, interleaved: bool = False, scale: float = 1.0):
+    """Queries (batch, time, heads, head_dim) and keys (batch, time, kv_heads, head_dim), or queries alone (``k`` None), turned by their positions, in one
+    launch; returns both.  Of every head the first ``2 * len(inv_freq)`` values are pairs, value i with the one half of them
+    on, or neighbours (``interleaved``): ``(a, b) -> (a cos + b sin, b cos - a sin)``, the direction of :class:`randumb_amd.gpt.Rotary`, with the angle
+    ``position * inv_freq[i]`` formed in 64 bits and cosine and sine times ``scale``; the rest passes through.
+
+    bf16 or fp32, any strides (unit inner ones are read in place), arithmetic in fp32, rounded once.  ``inv_freq``: fp32 (:func:`rotary_frequencies`).  ``positions``:
+    int64 or int32, (time,) or (batch, time), any integers; None: 0, 1, ...  Gradients of any order for q and k, none for the frequencies."""
+    if q.dtype not in (torch.float32, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
+        raise TypeError(f"rotary: queries and keys both bfloat16 or both float32, got {q.dtype}" + ("" if k is None else f" and {k.dtype}"))
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError(f"rotary: queries {tuple(q.shape)}" + ("" if k is None else f" and keys {tuple(k.shape)}") + " are not (batch, time, heads, head_dim)")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= q.shape[3] or inv_freq.numel() > 1024:
+        raise ValueError(f"rotary: float32 frequencies, one for each pair of a head's {q.shape[3]} values (1024 at most), got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if positions is not None and (positions.dtype not in (torch.int64, torch.int32) or positions.shape not in (q.shape[1:2], q.shape[:2], (1, q.shape[1]))):
+        raise ValueError(f"rotary: positions int64 or int32 of shape (time,) or (batch, time), got {positions.dtype} {tuple(positions.shape)}")
+    scale = float(scale)
+    both = None
+    if not _tracing() and q.is_cuda:
+        both = (_lib._ext or _lib.extension()).rotary(q, k, inv_freq, positions, interleaved, scale)
+    if both is None:
+        both = _rotary(q, k, inv_freq.detach(), positions, bool(interleaved), scale, False)
+    return both[0], None if k is None else both[1]
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0, original_context: int = 0,
+                       low: float = 1.0, high: float = 32.0, device=None):
+    """``(inv_freq, scale)`` for :func:`rotary`: ``rotary_dim / 2`` frequencies ``base ** (-2 i / rotary_dim)``, formed in 64 bits, for a context ``factor`` times
+    as long as the one the model was trained with:
+
+    None        as they are
+    "linear"    positions divided by ``factor``
+    "base"      a larger base, ``base * factor ** (rotary_dim / (rotary_dim - 2))``: the lowest frequency divided by ``factor``, the highest kept
+    "parts"     by the number of turns that a pair makes in ``original_context`` positions: divided by ``factor`` up to ``low`` turns, kept from ``high`` turns
+                on, a linear mixture by the pair's index in between, with ``scale = 0.1 ln(factor) + 1``"""
+    if rotary_dim < 2 or rotary_dim % 2 or not base > 0 or not factor > 0:
+        raise ValueError(f"rotary_frequencies: an even number of values, a positive base and factor, got {rotary_dim}, {base}, {factor}")
+    if scaling not in (None, "linear", "base", "parts") or (scaling is None and factor != 1.0):
+        raise ValueError(f"rotary_frequencies: no scaling {scaling!r} with factor {factor}")
+    exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    scale = 1.0
+    if scaling == "base":
+        if rotary_dim < 4:
+            raise ValueError("rotary_frequencies: a larger base changes nothing for one pair")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = float(base) ** -exponent
+    if scaling == "linear":
+        freq = freq / factor
+    if scaling == "parts":
+        if original_context < 1 or not 0 < low < high or base == 1.0:
+            raise ValueError(f"rotary_frequencies: parts of an original context and 0 < low < high, got {original_context}, {low}, {high}")
+        # the pair that makes n turns: original_context * base ** (-2 i / rotary_dim) = 2 pi n
+        first, last = (rotary_dim * math.log(original_context / (2 * math.pi * n)) / (2 * math.log(base)) for n in (high, low))
+        first, last = max(math.floor(first), 0), min(math.ceil(last), rotary_dim - 1)
+        stretched = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - stretched) + freq / factor * stretched
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return freq.to(torch.float32).to(device), scale
 
 
 # ------------------------------------------------------------------------------------------------ rten_cpp::*

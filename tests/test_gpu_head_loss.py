@@ -1,0 +1,273 @@
+"""ops.linear_cross_entropy against its formula in 64 bits, value by value, with bounds that count the roundings: a logit is a sum of ``dim`` products in fp32, a value of the
+softmax is off by its logit's error, and a gradient is a sum of such values (in bf16: rounded once more each) times the other factor."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from randumb_amd import ops
+
+pytestmark = pytest.mark.gpu
+IGNORED = -100
+
+
+def inputs(tokens, dim, classes, dtype, seed, ignored=0.0, scale=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(tokens, dim, device="cuda", generator=g).to(dtype)
+    w = (torch.randn(classes, dim, device="cuda", generator=g) * (scale / math.sqrt(dim))).to(dtype)
+    t = torch.randint(0, classes, (tokens,), device="cuda", generator=g)
+    t = torch.where(torch.rand(tokens, device="cuda", generator=g) < ignored, torch.full_like(t, IGNORED), t)
+    return x, w, t
+
+
+def formula(x, w, t, reduction, dloss):
+    """nll or loss, G, dx and dW in 64 bits."""
+    x, w = x.detach().double(), w.detach().double()
+    keep = t != IGNORED
+    x = torch.where(keep[:, None], x, 0.0)
+    logits = x @ w.T
+    lse = torch.logsumexp(logits, 1)
+    label = torch.where(keep, t, 0).long()
+    nll = torch.where(keep, lse - logits.gather(1, label[:, None])[:, 0], 0.0)
+    share = keep.double() * (dloss.double() if reduction == "none" else dloss.double().reshape(()))
+    loss = nll
+    if reduction == "mean":
+        loss, share = nll.sum() / keep.sum(), share / keep.sum().clamp_min(1)
+    elif reduction == "sum":
+        loss = nll.sum()
+    G = (logits - lse[:, None]).exp()
+    G[torch.arange(len(t)), label] -= 1.0
+    G *= share[:, None]
+    return loss, G, G @ w, G.T @ x
+
+
+def check(x, w, t, reduction, got, dloss, dx=None, dw=None):
+    loss, G, want_dx, want_dw = formula(x, w, t, reduction, dloss)
+    keep, dim, bf16 = t != IGNORED, x.shape[1], x.dtype == torch.bfloat16
+    xa, wa = torch.where(keep[:, None], x.detach().double(), 0.0).abs(), w.detach().double().abs()
+    step = 2.0**-24 if bf16 else 2.0**-23   # bf16 products are exact; fp32 ones leave out what one rounding would
+    # a logit: dim additions; its exponential and logarithm: a few roundings of values of its size
+    logit = (dim + 16) * step * float((xa @ wa.T).max()) + 2.0**-20
+    tokens = max(int(keep.sum()), 1)
+    bound = logit * (1.0 if reduction != "sum" else tokens) + (tokens + 8) * 2.0**-24 * loss.abs().max() if loss.numel() else logit
+    assert got.dtype == torch.float32 and got.shape == loss.shape
+    assert torch.equal(got.isnan(), loss.isnan())
+    if got.numel():
+        assert float((got.double() - loss).nan_to_num().abs().max()) <= float(torch.as_tensor(bound).nan_to_num())
+    half = torch.finfo(x.dtype).eps / 2
+    for d, want, sums, n in ((dx, want_dx, G.abs() @ wa, w.shape[0]), (dw, want_dw, G.abs().T @ xa, len(t))):
+        if d is None:
+            continue
+        assert d.dtype == x.dtype and d.shape == want.shape
+        # G: e^(logit's error), -1 for the target (at most as large again), its factor, in bf16 its rounding; then n additions and the result's rounding.
+        # The exponential's error is relative to p, G of the target is p - 1: of the target's own logit twice p's error at most
+        tol = half * want.abs() + ((half if bf16 else 0.0) + 4 * logit + (n + 16) * step) * sums + 1e-37
+        # the target's G is small where p is near 1, and its error is p's
+        share = dloss.double().abs().max() / (tokens if reduction == "mean" else 1)
+        tol = tol + 4 * logit * share * (wa.max() if d is dx else xa.sum(0).max())
+        bad = (d.double() - want).abs() > tol
+        assert not bool(bad.any()), (float(((d.double() - want).abs() / tol).max()), int(bad.sum()))
+
+
+def both(x, w, t, reduction, dloss=None):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, t, ignore_index=IGNORED, reduction=reduction)
+    if dloss is None:
+        dloss = torch.linspace(0.25, 1.5, len(t), device="cuda") if reduction == "none" else torch.tensor(0.75, device="cuda")
+    return (loss.detach(), dloss, *torch.autograd.grad(loss, [x, w], dloss))
+
+
+SIZES = [(1, 8, 1), (1, 64, 2), (2, 1, 7), (3, 7, 257), (17, 100, 1000), (63, 64, 255), (64, 72, 256), (65, 256, 513), (129, 200, 1025), (257, 768, 999), (300, 33, 4001),
+         (511, 520, 300), (1025, 257, 777)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,dim,classes", SIZES)
+def test_loss_and_gradients(tokens, dim, classes, dtype):
+    print(f"case head loss {tokens} x {dim} -> {classes} {dtype}", flush=True)
+    for i, (reduction, ignored) in enumerate([("mean", 0.0), ("none", 0.3), ("sum", 0.1)]):
+        x, w, t = inputs(tokens, dim, classes, dtype, 17 * tokens + i, ignored)
+        loss, dloss, dx, dw = both(x, w, t, reduction)
+        check(x, w, t, reduction, loss, dloss, dx, dw)
+        # one value more or less of precision: without gradients the same bits
+        with torch.no_grad():
+            assert torch.equal(ops.linear_cross_entropy(x, w, t, IGNORED, reduction).nan_to_num(7), loss.nan_to_num(7))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_several_pieces_of_the_vocabulary(dtype):
+    """More columns than one piece holds (256 MB of them), the last piece a short one."""
+    tokens, dim, classes = (8192, 72, 33003) if dtype == torch.bfloat16 else (4096, 40, 33003)
+    print(f"case head loss in pieces {dtype}", flush=True)
+    x, w, t = inputs(tokens, dim, classes, dtype, 5, 0.2)
+    loss, dloss, dx, dw = both(x, w, t, "mean")
+    check(x, w, t, "mean", loss, dloss, dx, dw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ignored_rows_count_for_nothing(dtype):
+    """Whatever they hold; and rows that are all ignored."""
+    x, w, t = inputs(200, 64, 700, dtype, 3, 0.5)
+    want = both(x, w, t, "mean")
+    dirty = x.clone()
+    dirty[t == IGNORED] = math.nan
+    dirty[(t == IGNORED).nonzero()[0]] = math.inf
+    for a, b in zip(want, both(dirty, w, t, "mean")):
+        assert torch.equal(a, b)
+    assert not bool(want[2][t == IGNORED].any())
+    nothing = torch.full_like(t, IGNORED)
+    for reduction, value in (("mean", math.nan), ("sum", 0.0), ("none", 0.0)):
+        loss, _, dx, dw = both(dirty, w, nothing, reduction)
+        assert torch.equal(loss.nan_to_num(7), torch.full_like(loss, value).nan_to_num(7)) and not bool(dx.any()) and not bool(dw.any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_is_not_a_number(dtype):
+    x, w, t = inputs(70, 64, 300, dtype, 4)
+    # a target outside the classes: its own row, and the weight's gradient
+    for wrong in (-1, 300, 1 << 40):
+        u = t.clone()
+        u[5] = wrong
+        loss, _, dx, dw = both(x, w, u, "none")
+        assert bool(loss[5].isnan()) and int(loss.isnan().sum()) == 1
+        assert bool(dx[5].isnan().all()) and int(dx.isnan().any(1).sum()) == 1 and bool(dw.isnan().any())
+    # an undefined hidden state reaches its own row only, going forward
+    y = x.clone()
+    y[9, 3] = math.nan
+    loss, _, dx, _ = both(y, w, t, "none")
+    assert bool(loss[9].isnan()) and int(loss.isnan().sum()) == 1 and int(dx.isnan().any(1).sum()) == 1
+    # far apart logits: the softmax is a single class
+    big = (x.float() * 100).to(dtype)
+    loss, dloss, dx, dw = both(big, w, t, "mean")
+    assert bool(loss.isfinite()) and bool(dx.isfinite().all()) and bool(dw.isfinite().all())
+    want = formula(big, w, t, "mean", dloss)[0]
+    assert float((loss - want).abs()) <= (64 + 16) * 2.0**-23 * float((big.double().abs() @ w.double().abs().T).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_shapes_and_types_of_the_targets(dtype):
+    tokens, dim, classes = 96, 72, 500
+    x, w, t = inputs(tokens, dim, classes, dtype, 8, 0.1)
+    want = both(x, w, t, "none")
+    wide = torch.full((tokens, dim + 9), math.nan, dtype=dtype, device="cuda")
+    wide[:, 3:3 + dim] = x
+    odd = torch.full((classes, dim + 5), math.nan, dtype=dtype, device="cuda")
+    odd[:, 1:1 + dim] = w
+    dloss = want[1].clone()
+    for a, b in ((wide[:, 3:3 + dim], odd[:, 1:1 + dim]), (x.T.contiguous().T, w.T.contiguous().T), (x, odd[:, 1:1 + dim])):
+        for p, q in zip(want, both(a, b, t, "none", dloss)):
+            assert torch.equal(p, q)
+    for p, q in zip(want, both(x, w, t.int(), "none", dloss)):
+        assert torch.equal(p, q)
+    far = torch.stack([t, t + 1], 1)[:, 0]   # a column of a matrix
+    for p, q in zip(want, both(x, w, far, "none", dloss)):
+        assert torch.equal(p, q)
+    three = x.view(4, 24, dim).requires_grad_()
+    loss = ops.linear_cross_entropy(three, w, t.view(4, 24), IGNORED, "none")
+    assert loss.shape == (4, 24) and torch.equal(loss.detach().view(-1), want[0])
+    assert torch.equal(torch.autograd.grad(loss, three, dloss.view(4, 24))[0].view(-1, dim), want[2])
+    # one of the gradients alone, and a gradient of a sum: a broadcast value
+    for leaf, at in ((0, 2), (1, 3)):
+        leaves = [x.detach(), w.detach()]
+        leaves[leaf].requires_grad_()
+        assert torch.equal(torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, IGNORED, "none"), leaves[leaf], dloss)[0], want[at])
+        leaves[leaf].requires_grad_(False)
+    ones = both(x, w, t, "none", torch.ones(1, device="cuda").expand(tokens))
+    for p, q in zip(ones, both(x, w, t, "none", torch.ones(tokens, device="cuda"))):
+        assert torch.equal(p, q)
+    # no tokens
+    empty = both(x[:0], w, t[:0], "mean")
+    assert bool(empty[0].isnan()) and empty[2].shape == (0, dim) and not bool(empty[3].any())
+    assert both(x[:0], w, t[:0], "none", dloss[:0])[0].shape == (0,) and float(both(x[:0], w, t[:0], "sum")[0]) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_against_differences(dtype):
+    """The step is so long that the loss's own rounding is small against it and so short that its curvature is: with an error d of either loss and a second
+    derivative up to max |w|^2 (of x) the quotient is off by d / h + h max |w|^2 / 2."""
+    x, w, t = inputs(40, 32, 200, torch.bfloat16, 11)
+    x, w = x.to(dtype), w.to(dtype)
+    _, _, dx, _ = both(x, w, t, "none", torch.ones(40, device="cuda"))
+    direction = torch.zeros_like(x)
+    direction[:, 5] = 1.0
+    h = 2.0**-4
+    up, down = x.float(), x.float()
+    up, down = up.clone(), down.clone()
+    base = torch.round(x.float()[:, 5] * 16) / 16   # values that bf16 holds at both ends
+    up[:, 5], down[:, 5] = base + h, base - h
+    x = x.float()
+    x[:, 5] = base
+    x, up, down = x.to(dtype), up.to(dtype), down.to(dtype)
+    _, _, dx, _ = both(x, w, t, "none", torch.ones(40, device="cuda"))
+    step = (up.float() - down.float())[:, 5]
+    a, b = (ops.linear_cross_entropy(v, w, t, IGNORED, "none") for v in (up, down))
+    top = float(w.float().abs().max())
+    tol = 2 * (32 + 16) * 2.0**-23 * 32 * 4 * top / h + (float(step.max()) / 2) ** 2 * top**3 + 2.0**-7 * top * 2
+    assert float(((a - b) / step - dx.float()[:, 5]).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_same_bits_every_time_on_any_stream_and_in_a_graph(dtype):
+    x, w, t = inputs(640, 192, 3001, dtype, 21, 0.2)
+    want = both(x, w, t, "mean")
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, both(x, w, t, "mean")))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = both(x, w, t, "mean")
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    sx, sw, st = x.clone().requires_grad_(), w.clone().requires_grad_(), t.clone()
+    dloss = want[1]
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.linear_cross_entropy(sx, sw, st, IGNORED), [sx, sw], dloss)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):   # two graphs at once: neither uses the other's workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = ops.linear_cross_entropy(sx, sw, st, IGNORED)
+            grads = torch.autograd.grad(loss, [sx, sw], dloss)
+        graphs.append((graph, loss, grads))
+    for seed in (31, 32, 33):
+        nx, nw, nt = inputs(640, 192, 3001, dtype, seed, 0.1 * (seed - 31))
+        with torch.no_grad():
+            sx.copy_(nx), sw.copy_(nw), st.copy_(nt)
+        eager = both(nx, nw, nt, "mean")
+        for graph, loss, grads in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(loss, eager[0]) and torch.equal(grads[0], eager[2]) and torch.equal(grads[1], eager[3])
+
+
+def test_first_derivatives_only():
+    x, w, t = inputs(16, 32, 50, torch.float32, 2)
+    x.requires_grad_()
+    g = torch.autograd.grad(ops.linear_cross_entropy(x, w, t), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_through_the_operators(dtype):
+    """What torch.compile traces: the registered operators and their gradient, the same bits."""
+    x, w, t = inputs(130, 64, 400, dtype, 6, 0.2)
+    want = both(x, w, t, "mean")
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss, _ = torch.ops.rten.linear_cross_entropy_fwd(a, b, t, IGNORED, 1)
+    assert torch.equal(loss.detach(), want[0])
+    for p, q in zip(torch.autograd.grad(loss, [a, b], want[1]), want[2:]):
+        assert torch.equal(p, q)
+
+
+def test_the_stock_operators_say_the_same():
+    """F.cross_entropy of fp32 logits, within fp32's own error of both."""
+    x, w, t = inputs(300, 64, 1000, torch.float32, 12, 0.2)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    want = F.cross_entropy(F.linear(a, b), t, ignore_index=IGNORED)
+    loss, dloss, dx, dw = both(x, w, t, "mean")
+    assert float((loss - want).abs()) < 1e-5
+    for p, q in zip((dx, dw), torch.autograd.grad(want, [a, b], dloss)):
+        assert float((p - q).norm() / q.norm()) < 1e-5
