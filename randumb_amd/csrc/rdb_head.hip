@@ -19,13 +19,14 @@
 // which are nearly all of the gradient, would all be off by the same rounding.
 // fp32: the same steps with the products of rdb_f32.hip, logits of a piece in fp32 in between.
 #include "rdb_big.hpp"
+#include "rdb_duo.hpp"
 #include <algorithm>
 
 namespace rdb {
 
 int num_compute_units();
 
-constexpr int HD_TILE = 256;
+constexpr int HD_TILE = 256, HD_TOK = DUO_B;
 constexpr float HD_LOG2E = 1.44269504088896340736f, HD_LN2 = 0.69314718055994530942f;
 enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
 
@@ -146,12 +147,11 @@ __device__ __forceinline__ void head_leave_stats(f32x16 (&acc)[4][NI], const Hea
 {
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
     const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;   // classes of this wave's rows that there are
-    acc_settle<4, NI>(acc);
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
         float v[64], m = -INFINITY, s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = acc_read(acc[i >> 4][ni][i & 15]);
+        for (int i = 0; i < 64; ++i) v[i] = acc[i >> 4][ni][i & 15];
         if (left < 128) {
 #pragma unroll
             for (int i = 0; i < 64; ++i)
@@ -177,7 +177,6 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[4][NI], bf16_t *__
     constexpr int BN = NI * 64, LD = HD_TILE + 8;
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
     const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;
-    acc_settle<4, NI>(acc);
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
         const int b = wn * NI * 32 + ni * 32 + r, tok = min(tok0 + b, count - 1);
@@ -185,7 +184,7 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[4][NI], bf16_t *__
         const int rel = p.label[tok] - first;
         float v[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc_read(acc[i >> 4][ni][i & 15]), HD_LOG2E, -l));
+        for (int i = 0; i < 64; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc[i >> 4][ni][i & 15], HD_LOG2E, -l));
         if (__any((unsigned)rel < 128u)) {
 #pragma unroll
             for (int i = 0; i < 64; ++i)
@@ -258,6 +257,26 @@ template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logi
         if (wn < 0) break;
         w = wn;
     }
+}
+
+// The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
+template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
+{
+    __shared__ __align__(16) bf16_t lds[DUO_LDS];
+    const int count = *p.count, tiles_t = (count + HD_TOK - 1) / HD_TOK, total = p.tiles_v * tiles_t, per_die = (total + 7) >> 3;
+    const int at = (int)blockIdx.x >> 3, w = ((int)blockIdx.x & 7) * per_die + at;
+    if (at >= per_die || w >= total) return;
+    const int per_group = 8 * p.tiles_v, group = w / per_group, in_group = w - group * per_group, size = min(8, tiles_t - group * 8);
+    const int tv = in_group / size, tok0 = (group * 8 + in_group - tv * size) * HD_TOK, row = p.v0 + tv * HD_TILE;
+    DuoOperand<DUO_A, K_CONT> pa;
+    DuoOperand<DUO_B, K_CONT> pb;
+    pa.set(p.w + (int64_t)row * p.ldw, p.ldw, 0, min(HD_TILE, p.classes - row), p.dim);
+    pb.set(p.x + (int64_t)tok0 * p.ldx, p.ldx, 0, min(HD_TOK, count - tok0), p.dim);
+    f32x16 acc[DUO_MI][DUO_NI];
+    duo_zero(acc);
+    duo_mainloop(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
+    if constexpr (GRAD) head_leave_grad<DUO_NI>(acc, lds, p, tv, tok0, count, opaque_tid());
+    else head_leave_stats<DUO_NI>(acc, p, tv, tok0, count, opaque_tid());
 }
 
 // ----------------------------------------------------------------------------------------------- loss
@@ -387,27 +406,27 @@ struct HeadProducts {
     HeadScale scale;
     int tiles_t, tiles_d, tiles_v;
 };
-// D[a][b] to out[a * ld + b], as big_store_rows, times a factor (bf16) or added to what is there (fp32)
+// D[a][b] to out[a * ld + b], times a factor (bf16) or added to what is there (fp32): each wave passes 32 rows x its 64 columns at a time through LDS, so that a lane
+// stores 16 bytes of a row
 template <typename E, bool ADD>
-__device__ __forceinline__ void head_store_rows(f32x16 (&acc)[4][4], bf16_t *__restrict__ lds, E *__restrict__ out, int64_t ld, int na, int b0, int nb, float scale, int t)
+__device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], bf16_t *__restrict__ lds, E *__restrict__ out, int64_t ld, int na, int b0, int nb, float scale, int t)
 {
-    constexpr int LDP = 128 + 4, PER = 16 / (int)sizeof(E), LPR = 128 / PER, RPP = 64 / LPR;
+    constexpr int COLS = DUO_NI * 32, LDP = COLS + 4, PER = 16 / (int)sizeof(E), LPR = COLS / PER, RPP = 64 / LPR;
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
     float *patch = reinterpret_cast<float *>(lds) + wave * 32 * LDP;
-    acc_settle<4, 4>(acc);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)(((int64_t)(na - 1) * ld + nb) * (int)sizeof(E)), 0x00020000);
-    const int col = (lane % LPR) * PER, b = b0 + wn * 128 + col;
+    const int col = (lane % LPR) * PER, b = b0 + wn * COLS + col;
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi) {
+    for (int mi = 0; mi < DUO_MI; ++mi) {
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni)
+        for (int ni = 0; ni < DUO_NI; ++ni)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) patch[head_row(j, g) * LDP + ni * 32 + r] = acc_read(acc[mi][ni][j]);
+            for (int j = 0; j < 16; ++j) patch[head_row(j, g) * LDP + ni * 32 + r] = acc[mi][ni][j];
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_wave_barrier();   // LDS serves a wave's instructions in order: the reads see these writes
 #pragma unroll
         for (int q = 0; q < 32 / RPP; ++q) {
-            const int row = q * RPP + lane / LPR, a = wm * 128 + mi * 32 + row;
+            const int row = q * RPP + lane / LPR, a = wm * DUO_MI * 32 + mi * 32 + row;
             const uint32_t off = (a < na && b < nb) ? (uint32_t)(((int64_t)a * ld + b) * (int)sizeof(E)) : BUFFER_OOB_ANY;
             f32x4 v = *reinterpret_cast<const f32x4 *>(patch + row * LDP + col);
             if constexpr (sizeof(E) == 2) {
@@ -426,106 +445,40 @@ __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[4][4], bf16_t *__r
         }
         __builtin_amdgcn_wave_barrier();
     }
-    __syncthreads();
 }
 
-// A list of tiles: n of them behind `base` others of the launch
-template <class F> __device__ __forceinline__ int head_next(int &r, int base, int n, F)
+// dx's tiles first (256 tokens x 128 columns, a range of the piece's classes), then dW's (256 classes x 128 columns)
+template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kernel(HeadProducts p)
 {
-    const int nv = (n + 7) / 8 * 8;
-    for (;; ++r) {
-        const int v = big_item((int)blockIdx.x, r, (int)gridDim.x) - base;
-        if (v >= nv) return -1;
-        if (v < 0) continue;
-        const int w = xcd_work_item(v, n);
-        if (w < n) {
-            ++r;
-            return w;
-        }
-    }
-}
-template <bool ADD> __device__ __forceinline__ void head_dx_items(const HeadProducts &p, bf16_t *lds, int count, int tiles_t, int &r, int base, int n)
-{
-    typedef GlobalOperand<HD_TILE, 64, K_CONT> PA;   // G: rows = tokens, contraction = classes
-    typedef GlobalOperand<HD_TILE, 64, M_CONT> PB;   // W: rows = its columns
-    PA pa;
-    PB pb;
-    BigRegs<PA, PB> regs;
-    auto decode = [&](int w, int &s, int &tt, int &td) {   // neighbours share G's rows
-        td = w % p.tiles_d;
-        w /= p.tiles_d;
-        tt = w % tiles_t;
-        s = w / tiles_t;
-    };
-    auto request = [&](int w) {
-        int s, tt, td;
-        decode(w, s, tt, td);
-        const int v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE, toks = min(HD_TILE, count - tok);
-        pa = PA{p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7, (int64_t)(toks - 1) * p.ldg + ((vs + 7) & ~7)};
-        pb = PB{p.w + (int64_t)v0 * p.ldw, p.ldw, td * HD_TILE, p.dim, vs, (int64_t)(vs - 1) * p.ldw + p.dim};
-        big_prefetch(regs, pa, pb, 0);
-    };
-    int w = head_next(r, base, n, 0);
-    if (w < 0) return;
-    request(w);
-    while (true) {
-        int s, tt, td;
-        decode(w, s, tt, td);
-        f32x16 acc[4][4];
-        big_zero<HD_TILE, HD_TILE>(acc);
-        big_mainloop<HD_TILE, HD_TILE>(acc, lds, regs, pa, pb, (min(p.split_v, p.rows_v - s * p.split_v) + 63) / 64);
-        const int wn = head_next(r, base, n, 0);
-        if (wn >= 0) request(wn);
-        __builtin_amdgcn_sched_barrier(0);
-        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tt * HD_TILE * p.lddx, p.lddx, min(HD_TILE, count - tt * HD_TILE), td * HD_TILE, p.dim,
-                                    1.0f, opaque_tid());
-        if (wn < 0) break;
-        w = wn;
-    }
-}
-__device__ __forceinline__ void head_dw_items(const HeadProducts &p, bf16_t *lds, int count, int &r, int base, int n)
-{
-    typedef GlobalOperand<HD_TILE, 64, M_CONT> PA;   // G: rows = classes, contraction = tokens
-    typedef GlobalOperand<HD_TILE, 64, M_CONT> PB;   // x: rows = its columns
-    PA pa;
-    PB pb;
-    BigRegs<PA, PB> regs;
-    auto request = [&](int w) {
-        const int tv = w / p.tiles_d, td = w % p.tiles_d;
-        pa = PA{p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count, (int64_t)count * p.ldg};
-        pb = PB{p.x, p.ldx, td * HD_TILE, p.dim, count, (int64_t)count * p.ldx};   // no rows: nothing is read, dW becomes zeros
-        big_prefetch(regs, pa, pb, 0);
-    };
-    const float scale = p.scale.value();
-    int w = head_next(r, base, n, 0);
-    if (w < 0) return;
-    request(w);
-    while (true) {
-        const int tv = w / p.tiles_d, td = w % p.tiles_d;
-        f32x16 acc[4][4];
-        big_zero<HD_TILE, HD_TILE>(acc);
-        big_mainloop<HD_TILE, HD_TILE>(acc, lds, regs, pa, pb, (count + 63) / 64);
-        const int wn = head_next(r, base, n, 0);
-        if (wn >= 0) request(wn);
-        __builtin_amdgcn_sched_barrier(0);
-        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), td * HD_TILE, p.dim, scale, opaque_tid());
-        if (wn < 0) break;
-        w = wn;
-    }
-}
-__global__ __launch_bounds__(256, 1) void head_products_kernel(HeadProducts p)
-{
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    bf16_t *lds = reinterpret_cast<bf16_t *>(smem_raw);
+    __shared__ __align__(16) bf16_t lds[DUO_LDS];
     const int count = *p.count, tiles_t = (count + HD_TILE - 1) / HD_TILE;
     const int n1 = p.dx ? p.splits * tiles_t * p.tiles_d : 0, n1v = (n1 + 7) / 8 * 8, n2 = p.dw ? p.tiles_v * p.tiles_d : 0;
-    int r = 0;
-    if (n1) {
-        if (p.add) head_dx_items<true>(p, lds, count, tiles_t, r, 0, n1);
-        else head_dx_items<false>(p, lds, count, tiles_t, r, 0, n1);
+    const bool first = (int)blockIdx.x < n1v;
+    const int block = (int)blockIdx.x - (first ? 0 : n1v), n = first ? n1 : n2, per_die = (n + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
+    if ((block >> 3) >= per_die || w >= n) return;
+    f32x16 acc[DUO_MI][DUO_NI];
+    duo_zero(acc);
+    const int td = w % p.tiles_d, b0 = td * DUO_B;
+    if (first) {
+        const int tt = w / p.tiles_d % tiles_t, s = w / p.tiles_d / tiles_t, v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE;
+        const int toks = min(HD_TILE, count - tok);
+        DuoOperand<DUO_A, K_CONT> pa;   // G: rows = tokens, contraction = classes
+        DuoOperand<DUO_B, M_CONT> pb;   // W: rows = its columns
+        pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7);
+        pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
+        duo_mainloop(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
+        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, opaque_tid());
+    } else {
+        const int tv = w / p.tiles_d;
+        DuoOperand<DUO_A, M_CONT> pa;   // G: rows = classes, contraction = tokens
+        DuoOperand<DUO_B, M_CONT> pb;   // x: rows = its columns
+        pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
+        pb.set(p.x, p.ldx, b0, p.dim, count);
+        duo_mainloop(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
+        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), opaque_tid());
     }
-    if (n2) head_dw_items(p, lds, count, r, n1v, n2);
 }
+
 // dx[row] = factor * the sums of its place over the splits, rounded once; zeros in ignored rows
 __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, const float *__restrict__ sums, const int *__restrict__ pos, int64_t tokens, int dim,
                                                       int64_t ld, int64_t stride, int splits, HeadScale scale)
@@ -679,9 +632,9 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.vp = cdiv(cdiv(classes, h.pieces), HD_TILE) * HD_TILE;
     if (f32 && h.pieces == 1) h.vp = classes;
     h.pieces = (int)cdiv(classes, h.vp);
-    h.bn = tokens <= 64 ? 64 : tokens <= 128 ? 128 : 256;
-    const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, HD_TILE);
-    int64_t splits = std::max<int64_t>(1, num_compute_units() / std::max<int64_t>(1, tiles));
+    h.bn = tokens <= 64 ? 64 : HD_TOK;
+    const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, DUO_B);
+    int64_t splits = std::max<int64_t>(1, 2 * num_compute_units() / std::max<int64_t>(1, tiles));
     splits = std::min(splits, std::max<int64_t>(1, h.vp / 1024));
     splits = std::min<int64_t>(splits, 16);
     h.split_v = cdiv(cdiv(h.vp, splits), 64) * 64;
@@ -804,7 +757,9 @@ template <int BN, bool GRAD> static int head_logits_on(const HeadLogits &p, hipS
 template <bool GRAD> static int head_logits(HeadLogits &p, int bn, hipStream_t s)
 {
     p.tiles_t = (int)cdiv(p.tokens, bn);
-    return bn == 64 ? head_logits_on<64, GRAD>(p, s) : bn == 128 ? head_logits_on<128, GRAD>(p, s) : head_logits_on<256, GRAD>(p, s);
+    if (bn == 64) return head_logits_on<64, GRAD>(p, s);
+    head_logits_duo_kernel<GRAD><<<(unsigned)(((int64_t)p.tiles_v * p.tiles_t + 7) / 8 * 8), 256, 0, s>>>(p);
+    return check_launch(GRAD ? "head_logits_duo_kernel<gradient>" : "head_logits_duo_kernel");
 }
 
 static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduction)
@@ -885,12 +840,12 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         }
         q.scale = scale;
         q.tiles_t = (int)cdiv(h.tokens, HD_TILE);
-        q.tiles_d = (int)cdiv(h.dp, HD_TILE);
+        q.tiles_d = (int)cdiv(h.dp, DUO_B);
         q.tiles_v = p.tiles_v;
-        const int64_t items = (dx ? (int64_t)q.splits * q.tiles_t * q.tiles_d + 7 : 0) + (dw ? (int64_t)q.tiles_v * q.tiles_d : 0);
-        if (int rc = head_launch(head_products_kernel, q, items, big_smem<HD_TILE, HD_TILE, OperandTile<HD_TILE, 64, M_CONT>, OperandTile<HD_TILE, 64, M_CONT>>(), c.s,
-                                 "head_products_kernel"))
-            return rc;
+        const int64_t blocks = (dx ? ((int64_t)q.splits * q.tiles_t * q.tiles_d + 7) / 8 * 8 : 0) + (dw ? ((int64_t)q.tiles_v * q.tiles_d + 7) / 8 * 8 : 0);
+        if (q.add) head_products_kernel<true><<<(unsigned)blocks, 256, 0, c.s>>>(q);
+        else head_products_kernel<false><<<(unsigned)blocks, 256, 0, c.s>>>(q);
+        if (int rc = check_launch("head_products_kernel")) return rc;
     }
     if (dx) {
         const int64_t blocks = std::min<int64_t>(cdiv(h.tokens * h.dp / 4, 256), 8192);
