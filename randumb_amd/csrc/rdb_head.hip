@@ -56,6 +56,7 @@ template <typename E, bool COMPACT> __global__ __launch_bounds__(256) void head_
     const int mine = p.tokens - r0 < p.rows ? (int)(p.tokens - r0) : p.rows;
     if (COMPACT) {
         int n = 0;
+#pragma unroll 8
         for (int64_t i = t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
@@ -105,14 +106,29 @@ template <typename E, bool COMPACT> __global__ __launch_bounds__(256) void head_
     }
 }
 
-// rows of `cols` bf16 values from one leading dimension to another; the columns behind them become zeros up to a multiple of 8 where `pad`
-__global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int cols, int out_cols)
+// rows of `cols` bf16 values from one leading dimension to another, 8 a lane at any address; PAD: zeros behind them up to a multiple of 8 (ldd)
+template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *__restrict__ dst, int64_t ldd, const bf16_t *__restrict__ src, int64_t lds, int64_t rows, int cols,
+                                                                              int per_block)
 {
-    const int64_t n = rows * out_cols, stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-        const int64_t row = i / out_cols;
-        const int c = (int)(i - row * out_cols);
-        dst[row * ldd + c] = c < cols ? src[row * lds + c] : (bf16_t)0;
+    const int64_t r0 = (int64_t)blockIdx.x * per_block;
+    const int chunks = (cols + 7) / 8, n = (int)min((int64_t)per_block, rows - r0) * chunks;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int row = i / chunks, c = (i - row * chunks) * 8;
+        const bf16_t *from = src + (r0 + row) * lds + c;
+        bf16_t *to = dst + (r0 + row) * ldd + c;
+        bf16_t v[8];
+        if (c + 8 <= cols) {
+            __builtin_memcpy(v, from, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? from[e] : (bf16_t)0;
+        }
+        if (PAD || c + 8 <= cols) {
+            __builtin_memcpy(to, v, 16);
+        } else {
+            for (int e = 0; c + e < cols; ++e) to[e] = v[e];
+        }
     }
 }
 
@@ -260,12 +276,10 @@ template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logi
 }
 
 // The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
-template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
+template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
 {
-    __shared__ __align__(16) bf16_t lds[DUO_LDS];
-    const int count = *p.count, tiles_t = (count + HD_TOK - 1) / HD_TOK, total = p.tiles_v * tiles_t, per_die = (total + 7) >> 3;
-    const int at = (int)blockIdx.x >> 3, w = ((int)blockIdx.x & 7) * per_die + at;
-    if (at >= per_die || w >= total) return;
+    const int tiles_t = (count + HD_TOK - 1) / HD_TOK, total = p.tiles_v * tiles_t, per_die = (total + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
+    if ((block >> 3) >= per_die || w >= total) return;
     const int per_group = 8 * p.tiles_v, group = w / per_group, in_group = w - group * per_group, size = min(8, tiles_t - group * 8);
     const int tv = in_group / size, tok0 = (group * 8 + in_group - tv * size) * HD_TOK, row = p.v0 + tv * HD_TILE;
     DuoOperand<DUO_A, K_CONT> pa;
@@ -277,6 +291,11 @@ template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_k
     duo_mainloop(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
     if constexpr (GRAD) head_leave_grad<DUO_NI>(acc, lds, p, tv, tok0, count, opaque_tid());
     else head_leave_stats<DUO_NI>(acc, p, tv, tok0, count, opaque_tid());
+}
+template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
+{
+    __shared__ __align__(16) bf16_t lds[DUO_LDS];
+    head_logits_tile<GRAD>(p, lds, *p.count, (int)blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------- loss
@@ -404,7 +423,8 @@ struct HeadProducts {
     bf16_t *dw;                // the piece's first row of [classes][lddw], or NULL
     int64_t lddw;
     HeadScale scale;
-    int tiles_t, tiles_d, tiles_v;
+    int tiles_d, tiles_v;
+    int blocks_dw, blocks_dx;   // of the launch, multiples of 8; the others are the next piece's logits
 };
 // D[a][b] to out[a * ld + b], times a factor (bf16) or added to what is there (fp32): each wave passes 32 rows x its 64 columns at a time through LDS, so that a lane
 // stores 16 bytes of a row
@@ -447,19 +467,30 @@ __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], b
     }
 }
 
-// dx's tiles first (256 tokens x 128 columns, a range of the piece's classes), then dW's (256 classes x 128 columns)
-template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kernel(HeadProducts p)
+// dW's tiles (256 classes x 128 columns), dx's (256 tokens x 128 columns, a range of the piece's classes), and the next piece's logits: short tiles that fill the
+// compute units that have no more of the long ones.
+template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kernel(HeadProducts p, HeadLogits next)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
-    const int count = *p.count, tiles_t = (count + HD_TILE - 1) / HD_TILE;
-    const int n1 = p.dx ? p.splits * tiles_t * p.tiles_d : 0, n1v = (n1 + 7) / 8 * 8, n2 = p.dw ? p.tiles_v * p.tiles_d : 0;
-    const bool first = (int)blockIdx.x < n1v;
-    const int block = (int)blockIdx.x - (first ? 0 : n1v), n = first ? n1 : n2, per_die = (n + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
+    const int count = *p.count;
+    int block = (int)blockIdx.x;
+    if (block >= p.blocks_dw + p.blocks_dx) return head_logits_tile<true>(next, lds, count, block - p.blocks_dw - p.blocks_dx);
+    const bool dw = block < p.blocks_dw;
+    if (!dw) block -= p.blocks_dw;
+    const int tiles_t = (count + HD_TILE - 1) / HD_TILE, n = (dw ? p.tiles_v : p.splits * tiles_t) * p.tiles_d, per_die = (n + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
     if ((block >> 3) >= per_die || w >= n) return;
     f32x16 acc[DUO_MI][DUO_NI];
     duo_zero(acc);
     const int td = w % p.tiles_d, b0 = td * DUO_B;
-    if (first) {
+    if (dw) {
+        const int tv = w / p.tiles_d;
+        DuoOperand<DUO_A, M_CONT> pa;   // G: rows = classes, contraction = tokens
+        DuoOperand<DUO_B, M_CONT> pb;   // x: rows = its columns
+        pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
+        pb.set(p.x, p.ldx, b0, p.dim, count);
+        duo_mainloop(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
+        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), opaque_tid());
+    } else {
         const int tt = w / p.tiles_d % tiles_t, s = w / p.tiles_d / tiles_t, v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE;
         const int toks = min(HD_TILE, count - tok);
         DuoOperand<DUO_A, K_CONT> pa;   // G: rows = tokens, contraction = classes
@@ -468,14 +499,6 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
         pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
         duo_mainloop(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
         head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, opaque_tid());
-    } else {
-        const int tv = w / p.tiles_d;
-        DuoOperand<DUO_A, M_CONT> pa;   // G: rows = classes, contraction = tokens
-        DuoOperand<DUO_B, M_CONT> pb;   // x: rows = its columns
-        pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
-        pb.set(p.x, p.ldx, b0, p.dim, count);
-        duo_mainloop(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
-        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), opaque_tid());
     }
 }
 
@@ -662,7 +685,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         h.lse2 = room(tokens * 4);
         h.factor = room(tokens * 4);
         h.label = room(tokens * 4);
-        h.g = room(tokens * h.vp * es);
+        h.g = room(tokens * h.vp * es * (!f32 && h.pieces > 1 ? 2 : 1));   // bf16: a piece's, and the next one's beside it
         if (want_dx && (!f32 || h.pieces > 1)) h.dx = room((f32 ? 1 : h.splits) * tokens * (f32 ? dim : h.dp) * 4);
         if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2);
     }
@@ -722,10 +745,10 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
     else head_gather_kernel<bf16_t, true><<<grid, 256, 0, c.s>>>(p);
     return check_launch("head_gather_kernel");
 }
-static int head_repack(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, int64_t out_cols, hipStream_t s)
+template <bool PAD> static int head_repack(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, hipStream_t s)
 {
-    const int64_t blocks = std::min<int64_t>(cdiv(rows * out_cols, 2048), 16384);
-    head_repack_kernel<<<(unsigned)blocks, 256, 0, s>>>(dst, ldd, src, lds, rows, (int)cols, (int)out_cols);
+    const int64_t per_block = std::max<int64_t>(1, 8192 / cols);   // four pieces a lane
+    head_repack_kernel<PAD><<<(unsigned)cdiv(rows, per_block), 256, 0, s>>>(dst, ldd, src, lds, rows, (int)cols, (int)per_block);
     return check_launch("head_repack_kernel");
 }
 // the weight as the tiles read it: rows from 16-byte boundaries on
@@ -735,7 +758,7 @@ static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
     *ldw = c.ldw;
     if (!c.h.pack_w) return RDB_OK;
     bf16_t *wc = c.at<bf16_t>(c.h.wc);
-    const int rc = head_repack(wc, c.h.dp, *w, c.ldw, c.h.classes, c.h.dim, c.h.dp, c.s);
+    const int rc = head_repack<true>(wc, c.h.dp, *w, c.ldw, c.h.classes, c.h.dim, c.s);
     *w = wc;
     *ldw = c.h.dp;
     return rc;
@@ -796,9 +819,9 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
     const HeadScale scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
     bf16_t *dwc = h.pad_dw && dw ? c.at<bf16_t>(h.dw) : dw;
     const int *count = c.at<int>(h.count);
-    for (int i = 0; i < h.pieces; ++i) {
-        const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
+    auto piece = [&](int i) {
         HeadLogits p = {};
+        const int64_t v0 = i * h.vp;
         p.x = c.at<bf16_t>(h.xc);
         p.ldx = h.dp;
         p.w = w;
@@ -807,18 +830,24 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         p.dim = (int)h.dp;
         p.classes = (int)h.classes;
         p.v0 = (int)v0;
-        p.tiles_v = (int)cdiv(n, HD_TILE);
+        p.tiles_v = (int)cdiv(std::min(h.vp, h.classes - v0), HD_TILE);
         p.tokens = h.tokens;
-        p.g = c.at<bf16_t>(h.g);
+        p.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp;
         p.ldg = h.vp;
         p.lse2 = c.at<float>(h.lse2);
         p.factor = c.at<float>(h.factor);
         p.label = c.at<int>(h.label);
-        if (int rc = head_logits<true>(p, h.bn, c.s)) return rc;
+        return p;
+    };
+    HeadLogits p = piece(0);
+    if (int rc = head_logits<true>(p, h.bn, c.s)) return rc;
+    auto blocks_of = [](int64_t tiles) { return (int)((tiles + 7) / 8 * 8); };
+    for (int i = 0; i < h.pieces; ++i) {
+        const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
         HeadProducts q = {};
-        q.g = p.g;
+        q.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp;
         q.ldg = h.vp;
-        q.x = p.x;
+        q.x = c.at<bf16_t>(h.xc);
         q.ldx = h.dp;
         q.w = w + v0 * ldw;
         q.ldw = ldw;
@@ -826,25 +855,30 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         q.rows_v = (int)n;
         q.dim = (int)h.dp;
         q.tokens = h.tokens;
+        q.tiles_d = (int)cdiv(h.dp, DUO_B);
+        q.tiles_v = (int)cdiv(n, HD_TILE);
+        q.scale = scale;
         if (dx) {
             q.dx = c.at<float>(h.dx);
             q.lddx = h.dp;
             q.dx_stride = h.tokens * h.dp;
-            q.add = i > 0;
             q.split_v = (int)h.split_v;
             q.splits = (int)cdiv(n, h.split_v);
+            q.blocks_dx = blocks_of(q.splits * cdiv(h.tokens, HD_TILE) * q.tiles_d);
         }
         if (dw) {
             q.dw = dwc + v0 * h.dp;
             q.lddw = h.dp;
+            q.blocks_dw = blocks_of((int64_t)q.tiles_v * q.tiles_d);
         }
-        q.scale = scale;
-        q.tiles_t = (int)cdiv(h.tokens, HD_TILE);
-        q.tiles_d = (int)cdiv(h.dp, DUO_B);
-        q.tiles_v = p.tiles_v;
-        const int64_t blocks = (dx ? ((int64_t)q.splits * q.tiles_t * q.tiles_d + 7) / 8 * 8 : 0) + (dw ? ((int64_t)q.tiles_v * q.tiles_d + 7) / 8 * 8 : 0);
-        if (q.add) head_products_kernel<true><<<(unsigned)blocks, 256, 0, c.s>>>(q);
-        else head_products_kernel<false><<<(unsigned)blocks, 256, 0, c.s>>>(q);
+        HeadLogits next = {};
+        int64_t blocks = (int64_t)q.blocks_dw + q.blocks_dx;
+        if (i + 1 < h.pieces) {
+            next = piece(i + 1);
+            blocks += blocks_of(next.tiles_v * cdiv(h.tokens, HD_TOK));
+        }
+        if (i > 0) head_products_kernel<true><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
+        else head_products_kernel<false><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
         if (int rc = check_launch("head_products_kernel")) return rc;
     }
     if (dx) {
@@ -852,7 +886,7 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         head_dx_kernel<<<(unsigned)blocks, 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale);
         if (int rc = check_launch("head_dx_kernel")) return rc;
     }
-    if (dw && h.pad_dw) return head_repack(dw, h.dim, dwc, h.dp, h.classes, h.dim, h.dim, c.s);
+    if (dw && h.pad_dw) return head_repack<false>(dw, h.dim, dwc, h.dp, h.classes, h.dim, c.s);
     return RDB_OK;
 }
 
