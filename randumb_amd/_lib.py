@@ -296,7 +296,7 @@ def load() -> ctypes.CDLL:
     L.rdb_causal_attention_scratch_floats.restype = i64
     L.rdb_causal_attention_fwd.argtypes = [vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, f32, vp]
     L.rdb_causal_attention_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, vp]
-    L.rdb_linear_cross_entropy_workspace_bytes.argtypes = [i64, i64, i64, ci, vp, i64, ci, ci, ci]
+    L.rdb_linear_cross_entropy_workspace_bytes.argtypes = [i64, i64, i64, ci, vp, i64, vp, i64, ci, ci, ci]
     L.rdb_linear_cross_entropy_workspace_bytes.restype = i64
     L.rdb_linear_cross_entropy_fwd.argtypes = [vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
     L.rdb_linear_cross_entropy_bwd.argtypes = [vp, vp, vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]

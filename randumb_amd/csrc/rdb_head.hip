@@ -32,12 +32,12 @@ enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
 
 // ----------------------------------------------------------------------------------------------- the rows that count
 struct HeadGather {
-    void *xc;                // [tokens][ldc]: the rows that count, in order; fp32: every row in its place, ignored ones zeros
-    const void *x;
+    bf16_t *xc;              // [tokens][ldc]: the rows that count, in order, zeros behind their last values
+    const bf16_t *x;
     int64_t ldx, ldc;
     const int64_t *target;
     int *pos;                // [tokens]: where a row went, -1: ignored
-    int *count;              // rows that count
+    int *count;              // rows that count; behind it the counter of head_merge_kernel's blocks, cleared
     // backward, by place: log2 of the row's sum, target (-1: none of the classes), its own factor of G
     float *lse2, *factor;
     int *label;
@@ -45,89 +45,92 @@ struct HeadGather {
     const float *dloss;      // [tokens], or NULL: 1
     int64_t tokens, dim, classes, ignore;
     int rows;                // per block
-    bool wide;               // x may be read 16 bytes at a time
 };
 // Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.
-template <typename E, bool COMPACT> __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
+__global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
 {
     __shared__ int before_[4], place_[64];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t r0 = (int64_t)blockIdx.x * p.rows;
     const int mine = p.tokens - r0 < p.rows ? (int)(p.tokens - r0) : p.rows;
-    if (COMPACT) {
-        int n = 0;
-#pragma unroll 8
-        for (int64_t i = t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
+    const int64_t c = wave == 0 && lane < mine ? p.target[r0 + lane] : p.ignore;
+    int n = 0;
+#pragma unroll 16
+    for (int64_t i = t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
-        if (lane == 0) before_[wave] = n;
-        __syncthreads();
-    }
+    for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
+    if (lane == 0) before_[wave] = n;
+    __syncthreads();
     if (wave == 0) {
-        const int64_t c = lane < mine ? p.target[r0 + lane] : p.ignore;
         const bool counts = c != p.ignore;
         const unsigned long long all = __ballot(counts);
-        const int first = COMPACT ? before_[0] + before_[1] + before_[2] + before_[3] : 0;
-        const int at = COMPACT ? first + __popcll(all & ((1ull << lane) - 1)) : (int)(r0 + lane);
+        const int first = before_[0] + before_[1] + before_[2] + before_[3], at = first + __popcll(all & ((1ull << lane) - 1));
         place_[lane] = counts ? at : -1;
         if (lane < mine) {
             p.pos[r0 + lane] = counts ? at : -1;
-            if (p.lse2 && (counts || !COMPACT)) {
+            if (p.lse2 && counts) {
                 const bool known = c >= 0 && c < p.classes;
                 p.lse2[at] = p.stats[r0 + lane] * HD_LOG2E;
                 p.label[at] = known ? (int)c : -1;
-                p.factor[at] = !counts ? 0.0f : !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
+                p.factor[at] = !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
             }
         }
-        if (COMPACT && lane == 0 && r0 + mine == p.tokens) *p.count = first + __popcll(all);
+        if (lane == 0 && r0 + mine == p.tokens) {
+            p.count[0] = first + __popcll(all);
+            p.count[1] = 0;
+        }
     }
     __syncthreads();
-    constexpr int PER = 16 / (int)sizeof(E);
-    const int chunks = (int)(p.ldc / PER);
-    const E *x = static_cast<const E *>(p.x);
-    E *xc = static_cast<E *>(p.xc);
+    const int chunks = (int)(p.ldc / 8);
+#pragma unroll 4
     for (int i = t; i < mine * chunks; i += 256) {
-        const int row = i / chunks, c = (i - row * chunks) * PER;
-        const int at = place_[row];
-        if (at < 0 && COMPACT) continue;
-        const E *src = x + (r0 + row) * p.ldx + c;
-        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (at >= 0) {
-            if (p.wide && c + PER <= p.dim) {
-                v = *reinterpret_cast<const f32x4 *>(src);
-            } else {
-                E e[PER];
+        const int row = i / chunks, col = (i - row * chunks) * 8, at = place_[row];
+        if (at < 0) continue;
+        const bf16_t *src = p.x + (r0 + row) * p.ldx + col;
+        bf16_t v[8];
+        if (col + 8 <= p.dim) {
+            __builtin_memcpy(v, src, 16);
+        } else {
 #pragma unroll
-                for (int j = 0; j < PER; ++j) e[j] = c + j < p.dim ? src[j] : E(0);
-                __builtin_memcpy(&v, e, 16);
-            }
+            for (int j = 0; j < 8; ++j) v[j] = col + j < p.dim ? src[j] : (bf16_t)0;
         }
-        *reinterpret_cast<f32x4 *>(xc + (COMPACT ? (int64_t)at : r0 + row) * p.ldc + c) = v;
+        __builtin_memcpy(__builtin_assume_aligned(p.xc + (int64_t)at * p.ldc + col, 16), v, 16);
     }
 }
 
-// rows of `cols` bf16 values from one leading dimension to another, 8 a lane at any address; PAD: zeros behind them up to a multiple of 8 (ldd)
-template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *__restrict__ dst, int64_t ldd, const bf16_t *__restrict__ src, int64_t lds, int64_t rows, int cols,
-                                                                              int per_block)
+// Rows of `cols` bf16 values into rows of a multiple of 8 of them (PAD, zeros behind the last ones) or out of them into rows without gaps; a lane reads 8 values at any address
+// and writes them to a multiple of 16 bytes.  per_block: a multiple of 8.
+template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *__restrict__ dst, const bf16_t *__restrict__ src, int64_t lds, int64_t rows, int cols, int per_block)
 {
     const int64_t r0 = (int64_t)blockIdx.x * per_block;
-    const int chunks = (cols + 7) / 8, n = (int)min((int64_t)per_block, rows - r0) * chunks;
+    const int mine = rows - r0 < per_block ? (int)(rows - r0) : per_block, out_cols = PAD ? (cols + 7) & ~7 : cols, total = mine * out_cols;
+    src += r0 * lds;
+    dst += r0 * out_cols;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int row = i / chunks, c = (i - row * chunks) * 8;
-        const bf16_t *from = src + (r0 + row) * lds + c;
-        bf16_t *to = dst + (r0 + row) * ldd + c;
+    for (int i = threadIdx.x * 8; i < total; i += 2048) {
+        const int row = i / out_cols, c = i - row * out_cols;
+        const bf16_t *from = src + (int64_t)row * lds + c;
         bf16_t v[8];
         if (c + 8 <= cols) {
             __builtin_memcpy(v, from, 16);
-        } else {
+        } else if (PAD) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? from[e] : (bf16_t)0;
+        } else {   // on into the next row (rows of fewer than 8 values: rows)
+            int r = row, k = c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = r < mine ? src[(int64_t)r * lds + k] : (bf16_t)0;
+                if (++k == cols) {
+                    k = 0;
+                    ++r;
+                }
+            }
         }
-        if (PAD || c + 8 <= cols) {
-            __builtin_memcpy(to, v, 16);
+        if (i + 8 <= total) {
+            __builtin_memcpy(__builtin_assume_aligned(dst + i, 16), v, 16);
         } else {
-            for (int e = 0; c + e < cols; ++e) to[e] = v[e];
+            for (int e = 0; i + e < total; ++e) dst[i + e] = v[e];
         }
     }
 }
@@ -137,7 +140,8 @@ struct HeadLogits {
     const bf16_t *x;      // the rows that count, [*count][ldx]
     const bf16_t *w;      // [classes][ldw]
     int64_t ldx, ldw;
-    const int *count;
+    const int *count;     // NULL: all tokens
+    unsigned int *cleared;   // NULL, or a word that block 0 sets to zero for a later launch
     int dim, classes, v0;     // classes v0 .. v0 + tiles_v * 256 of this launch
     int tiles_v, tiles_t;
     float2 *part;         // stats: [2 * tiles_v][tokens]: maximum (times log2 e) and sum
@@ -233,7 +237,7 @@ template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logi
     bf16_t *lds = reinterpret_cast<bf16_t *>(smem_raw);
     typedef GlobalOperand<HD_TILE, 64, K_CONT> PA;
     typedef GlobalOperand<BN, 64, K_CONT> PB;
-    const int count = *p.count, tiles_t = (count + BN - 1) / BN, total = p.tiles_v * tiles_t, vtotal = (total + 7) / 8 * 8, nstage = (p.dim + 63) / 64;
+    const int count = p.count ? *p.count : (int)p.tokens, tiles_t = (count + BN - 1) / BN, total = p.tiles_v * tiles_t, vtotal = (total + 7) / 8 * 8, nstage = (p.dim + 63) / 64;
     int v = (int)blockIdx.x;
     auto next = [&]() {
         for (; v < vtotal; v += gridDim.x) {
@@ -245,6 +249,7 @@ template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logi
         }
         return -1;
     };
+    if (p.cleared && blockIdx.x == 0 && threadIdx.x == 0) *p.cleared = 0u;
     PA pa;
     PB pb;
     BigRegs<PA, PB> regs;
@@ -295,113 +300,133 @@ template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const Head
 template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
-    head_logits_tile<GRAD>(p, lds, *p.count, (int)blockIdx.x);
+    head_logits_tile<GRAD>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------- loss
-struct HeadMerge {
-    float *stats;          // [tokens]: lse, 0 in ignored rows
-    float *nll;            // [tokens]
-    const float2 *part;    // [parts][tokens], by place
-    const int *pos;
-    const bf16_t *x, *w;
-    int64_t ldx, ldw, tokens, classes;
+// What is left of the loss when every row's nll is there: the sum over the rows, in a fixed order, by the block that comes last.  Values pass between blocks on
+// different dies, so they are stored and loaded around the dies' caches.
+struct HeadSum {
+    float *loss;                // one value, or NULL: the rows' own are the loss
+    float *count;               // rows that count, as fp32
+    float *nll;                 // [tokens]
+    unsigned int *arrived;      // 0 when the launch begins
     const int64_t *target;
-    int parts, dim;        // dim: a multiple of 8, zeros behind the last value
+    int64_t tokens, ignore;
+    int mean;
 };
-// Sixteen lanes a token, sixteen tokens a block.
-__global__ __launch_bounds__(256) void head_merge_kernel(HeadMerge p)
+__device__ __forceinline__ void head_leave_nll(const HeadSum &p, int64_t row, float v)
 {
-    const int t = threadIdx.x, slot = t >> 4, part = t & 15;
-    __shared__ float ms_[16][17], ss_[16][17];
-    const int64_t r0 = (int64_t)blockIdx.x * 16;
-    {   // neighbouring lanes: neighbouring tokens, as the parts lie; then over to the token's own lanes
-        const int64_t row = r0 + part;
-        const int at = row < p.tokens ? p.pos[row] : -1;
-        float m = -INFINITY, s = 0.0f;
-        if (at >= 0)
-#pragma unroll 4
-            for (int i = slot; i < p.parts; i += 16) {
-                const float2 q = p.part[(int64_t)i * p.tokens + at];
-                const float top = fmaxf(m, q.x), ref = top == -INFINITY ? 0.0f : top;
-                s = s * __builtin_amdgcn_exp2f(m - ref) + q.y * __builtin_amdgcn_exp2f(q.x - ref);
-                m = top;
-            }
-        ms_[part][slot] = m;
-        ss_[part][slot] = s;
-    }
-    __syncthreads();
-    const int64_t row = r0 + slot;
-    if (row >= p.tokens) return;   // all sixteen lanes of the token
-    const int at = p.pos[row];
-    if (at < 0) {
-        if (part == 0) {
-            p.stats[row] = 0.0f;
-            p.nll[row] = 0.0f;
-        }
-        return;
-    }
-    float m = ms_[slot][part], s = ss_[slot][part];
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-        s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
-        m = top;
-    }
-    const float lse = (m + log2f(s)) * HD_LN2;
-    const int64_t c = p.target[row];
-    const bool known = c >= 0 && c < p.classes;
-    float d = 0.0f;
-    if (known) {
-        const bf16_t *x = p.x + (int64_t)at * p.ldx, *w = p.w + c * p.ldw;
-#pragma unroll 2
-        for (int i = part * 8; i < p.dim; i += 128) {
-            const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
-        }
-    }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) d += __shfl_xor(d, o, 64);
-    if (part == 0) {
-        p.stats[row] = lse;
-        p.nll[row] = known ? lse - d : __uint_as_float(0x7fc00000u);
-    }
+    if (p.loss) __hip_atomic_store(p.nll + row, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else p.nll[row] = v;
 }
-
-// loss[0] = sum of nll (/ rows that count), count beside it.  One block, fixed order.
-__global__ __launch_bounds__(1024) void head_loss_kernel(float *__restrict__ loss, float *__restrict__ count, const float *__restrict__ nll,
-                                                         const int64_t *__restrict__ target, int64_t rows, int64_t ignore, int mean)
+// One block of THREADS.
+template <int THREADS> __device__ __forceinline__ void head_add_up(const HeadSum &p)
 {
-    __shared__ float s[16];
-    __shared__ int n[16];
+    __shared__ float s_[THREADS / 64];
+    __shared__ int n_[THREADS / 64];
+    const int t = threadIdx.x;
     float a = 0.0f;
     int c = 0;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) {
-        if (loss) a += nll[i];
-        c += target[i] == ignore ? 0 : 1;
+    for (int64_t i = t; i < p.tokens; i += THREADS) {
+        a += __hip_atomic_load(p.nll + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        c += p.target[i] == p.ignore ? 0 : 1;
     }
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) {
         a += __shfl_xor(a, m, 64);
         c += __shfl_xor(c, m, 64);
     }
-    if ((threadIdx.x & 63) == 0) {
-        s[threadIdx.x >> 6] = a;
-        n[threadIdx.x >> 6] = c;
+    if ((t & 63) == 0) {
+        s_[t >> 6] = a;
+        n_[t >> 6] = c;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        a = 0.0f;
-        c = 0;
-        for (int w = 0; w < 16; ++w) {
-            a += s[w];
-            c += n[w];
-        }
-        if (loss) loss[0] = mean ? a / (float)c : a;
-        count[0] = (float)c;
+    if (t) return;
+    a = 0.0f;
+    c = 0;
+    for (int w = 0; w < THREADS / 64; ++w) {
+        a += s_[w];
+        c += n_[w];
     }
+    p.loss[0] = p.mean ? a / (float)c : a;
+    p.count[0] = (float)c;
+}
+__global__ __launch_bounds__(1024) void head_loss_kernel(HeadSum p) { head_add_up<1024>(p); }
+// The same by the last block of a launch; all THREADS threads of all blocks, after their last head_leave_nll.  Counting one word costs 10 ns a block.
+template <int THREADS> __device__ __forceinline__ void head_sum(const HeadSum &p)
+{
+    __shared__ int last_;
+    if (!p.loss) return;
+    __builtin_amdgcn_s_waitcnt(0);   // this wave's values are in memory
+    __syncthreads();                 // ... and every other wave's
+    if (threadIdx.x == 0) last_ = __hip_atomic_fetch_add(p.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    __syncthreads();
+    if (last_) head_add_up<THREADS>(p);
+}
+
+__device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
+{
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
+    m = top;
+}
+struct HeadMerge {
+    float *stats;          // [tokens]: lse, 0 in ignored rows
+    const float2 *part;    // [parts][tokens], by place
+    const int *pos;        // NULL: every row in its place
+    const bf16_t *x, *w;
+    int64_t ldx, ldw, classes;
+    int parts, dim;        // dim: a multiple of 8, zeros behind the last value
+    HeadSum sum;
+};
+// LANES lanes a token: many where the tokens are few and their parts a chain of loads.
+template <int LANES> __global__ __launch_bounds__(1024) void head_merge_kernel(HeadMerge p)
+{
+    constexpr int TOK = 1024 / LANES;
+    __shared__ float ms_[TOK][LANES + 1], ss_[TOK][LANES + 1];
+    const int t = threadIdx.x;
+    const int64_t r0 = (int64_t)blockIdx.x * TOK, tokens = p.sum.tokens;
+    auto place = [&](int64_t row) { return row >= tokens ? -1 : p.pos ? p.pos[row] : p.sum.target[row] == p.sum.ignore ? -1 : (int)row; };
+    {   // neighbouring lanes: neighbouring tokens, as the parts lie; then over to the token's own lanes
+        const int tok = t % TOK, slot = t / TOK, at = place(r0 + tok);
+        float m = -INFINITY, s = 0.0f;
+        if (at >= 0)
+#pragma unroll 8
+            for (int i = slot; i < p.parts; i += LANES) {
+                const float2 q = p.part[(int64_t)i * tokens + at];
+                head_join(m, s, q.x, q.y);
+            }
+        ms_[tok][slot] = m;
+        ss_[tok][slot] = s;
+    }
+    __syncthreads();
+    const int tok = t / LANES, lane = t % LANES, at = place(r0 + tok);
+    const int64_t row = r0 + tok;
+    float m = ms_[tok][lane], s = ss_[tok][lane], d = 0.0f;
+    const int64_t c = at < 0 ? 0 : p.sum.target[row];
+    const bool known = c >= 0 && c < p.classes;
+    if (at >= 0 && known) {
+        const bf16_t *x = p.x + (int64_t)at * p.ldx, *w = p.w + c * p.ldw;
+#pragma unroll 2
+        for (int i = lane * 8; i < p.dim; i += LANES * 8) {
+            const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+        head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+        d += __shfl_xor(d, o, 64);
+    }
+    if (lane == 0 && row < tokens) {
+        const float lse = (m + log2f(s)) * HD_LN2;
+        p.stats[row] = at < 0 ? 0.0f : lse;
+        head_leave_nll(p.sum, row, at < 0 ? 0.0f : known ? lse - d : __uint_as_float(0x7fc00000u));
+    }
+    head_sum<1024>(p.sum);
 }
 
 // ----------------------------------------------------------------------------------------------- dx and dW
@@ -539,43 +564,35 @@ struct HeadRows {
     float *logits;         // [tokens][n], n classes from v0 on; G in their place
     float2 *state;         // [tokens]: maximum (times log2 e) and sum of the pieces so far
     float *picked;         // [tokens]: the target's logit
-    const int *pos;
-    const float *lse2, *factor;
-    const int *label;
-    const int64_t *target;
-    float *stats, *nll;
-    HeadScale scale;
-    int64_t tokens, classes, ignore;
+    float *stats;
+    int64_t classes;
     int n, v0, first, last;
+    HeadSum sum;           // tokens and targets; the last piece: nll
+    // gradient
+    HeadScale scale;
+    const float *dloss;    // [tokens], or NULL
+    float *xc;             // NULL, or where a row of x goes, zeros for an ignored one
+    const float *x;
+    int64_t ldx;
+    int dim;
 };
-__device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
-{
-    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
-    m = top;
-}
 // One block a row.
 __global__ __launch_bounds__(256) void head_rows_stats_kernel(HeadRows p)
 {
     __shared__ float ms_[4], ss_[4];
     const int64_t row = blockIdx.x;
     const int t = threadIdx.x;
-    const int64_t c = p.target[row];
-    if (c == p.ignore) {
-        if (p.last && t == 0) {
-            p.stats[row] = 0.0f;
-            p.nll[row] = 0.0f;
-        }
-        return;
-    }
+    const int64_t c = p.sum.target[row];
+    const bool counts = c != p.sum.ignore, known = c >= 0 && c < p.classes;
     const float *l = p.logits + row * p.n;
     float m = -INFINITY, s = 0.0f;
+    if (counts)
 #pragma unroll 4
-    for (int i = t; i < p.n; i += 256) {
-        const float v = l[i], top = fmaxf(m, v), ref = top == -INFINITY ? 0.0f : top;
-        s = s * __expf(m - ref) + __expf(v - ref);
-        m = top;
-    }
+        for (int i = t; i < p.n; i += 256) {
+            const float v = l[i], top = fmaxf(m, v), ref = top == -INFINITY ? 0.0f : top;
+            s = s * __expf(m - ref) + __expf(v - ref);
+            m = top;
+        }
     m *= HD_LOG2E;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
@@ -584,34 +601,39 @@ __global__ __launch_bounds__(256) void head_rows_stats_kernel(HeadRows p)
         ss_[t >> 6] = s;
     }
     __syncthreads();
-    if (t) return;
-    for (int w = 1; w < 4; ++w) head_join(m, s, ms_[w], ss_[w]);
-    if (!p.first) head_join(m, s, p.state[row].x, p.state[row].y);
-    const bool known = c >= 0 && c < p.classes;
-    float picked = p.first || !known ? 0.0f : p.picked[row];
-    if (known && c >= p.v0 && c < p.v0 + p.n) picked = l[c - p.v0];
-    if (!p.last) {
-        p.state[row] = float2{m, s};
-        p.picked[row] = picked;
-        return;
+    if (t == 0) {
+        for (int w = 1; w < 4; ++w) head_join(m, s, ms_[w], ss_[w]);
+        if (!p.first && counts) head_join(m, s, p.state[row].x, p.state[row].y);
+        float picked = p.first || !known || !counts ? 0.0f : p.picked[row];
+        if (counts && known && c >= p.v0 && c < p.v0 + p.n) picked = l[c - p.v0];
+        if (p.last) {
+            const float lse = (m + log2f(s)) * HD_LN2;
+            p.stats[row] = counts ? lse : 0.0f;
+            head_leave_nll(p.sum, row, !counts ? 0.0f : known ? lse - picked : __uint_as_float(0x7fc00000u));
+        } else {
+            p.state[row] = float2{m, s};
+            p.picked[row] = picked;
+        }
     }
-    const float lse = (m + log2f(s)) * HD_LN2;
-    p.stats[row] = lse;
-    p.nll[row] = known ? lse - picked : __uint_as_float(0x7fc00000u);
 }
 __global__ __launch_bounds__(256) void head_rows_grad_kernel(HeadRows p)
 {
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x, c = p.sum.target[row];
+    const bool counts = c != p.sum.ignore, known = c >= 0 && c < p.classes;
     float *l = p.logits + row * p.n;
-    const float f = p.pos[row] < 0 ? 0.0f : p.factor[row] * p.scale.value(), lse = p.stats[row];
-    const int label = p.label[row] - p.v0;
-    const bool skip = p.pos[row] < 0;
+    const float lse = p.stats[row], f = !counts ? 0.0f : !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[row] : p.scale.value();
+    const int label = known ? (int)(c - p.v0) : -1;
+    if (counts)
 #pragma unroll 4
-    for (int i = threadIdx.x; i < p.n; i += 256) {
-        float v = expf(l[i] - lse);
-        if (i == label) v -= 1.0f;
-        l[i] = skip ? 0.0f : v * f;
-    }
+        for (int i = threadIdx.x; i < p.n; i += 256) {
+            float v = expf(l[i] - lse);
+            if (i == label) v -= 1.0f;
+            l[i] = v * f;
+        }
+    else
+        for (int i = threadIdx.x; i < p.n; i += 256) l[i] = 0.0f;
+    if (p.xc)
+        for (int i = threadIdx.x; i < p.dim; i += 256) p.xc[row * p.dim + i] = counts ? p.x[row * p.ldx + i] : 0.0f;
 }
 __global__ __launch_bounds__(256) void head_add_kernel(float *__restrict__ out, const float *__restrict__ a, int64_t n)
 {
@@ -619,20 +641,36 @@ __global__ __launch_bounds__(256) void head_add_kernel(float *__restrict__ out, 
 }
 
 // ----------------------------------------------------------------------------------------------- plan and calls
-// Bytes of a piece's G (bf16) or logits (fp32): what the next launch finds in the chip's last-level cache, and tiles enough to fill it.
-constexpr int64_t HD_PIECE_BYTES = 256ll << 20;
+// Bytes of a piece's G (bf16) or logits (fp32).  Such an amount the next launch finds in the chip's last-level cache.  A piece of G is twice or four times as large where
+// its launch (dW, dx and the next piece's logits) would otherwise end with dW's tiles, which contract all tokens: in units of a stage of 64, as long as a block
+// has, on average, less than twice the length of one.  8192 tokens -> 50304, us a step with pieces of 128, 256, 384, 512, 1024 MB: 256 columns 1472, 1222, 1118, 1034, 1097;
+// 768 columns 2319, 2319, 2329, 2322, 2449; 4096 tokens x 4096 -> 65536 7076, 7082, 7090, 7138, 7134.
+constexpr int64_t HD_PIECE_BYTES = 128ll << 20, HD_PIECE_MOST = 512ll << 20;
+constexpr int HD_TILE_COST = 8;   // of a tile's first operands and its stores
+static int64_t head_piece_bytes(int64_t tokens, int64_t dim)
+{
+    const int64_t td = cdiv(dim, DUO_B), longest = cdiv(tokens, DUO_K) + HD_TILE_COST;
+    const int64_t of_256 = td * longest + cdiv(tokens, HD_TILE) * td * (HD_TILE / DUO_K) + cdiv(tokens, HD_TOK) * (cdiv(dim, DUO_K) + HD_TILE_COST);   // work of 256 classes
+    int64_t bytes = HD_PIECE_BYTES;
+    while (bytes < HD_PIECE_MOST && bytes / (2 * HD_TILE * tokens) * of_256 < 2 * longest * 2 * num_compute_units()) bytes *= 2;
+    return bytes;
+}
 
 struct HeadPlan {
     int64_t tokens, dim, classes;
     int dtype;
     bool backward, want_dx, want_dw, pack_w, pad_dw;
+    bool direct;               // few tokens, forward: x as it is, ignored rows and all
     int64_t dp, vp;            // columns of the copies; classes of a piece
     int pieces, bn, splits;
     int64_t split_v;
     // offsets in the workspace
     int64_t xc, pos, count, lse2, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
 };
-static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, bool backward, bool want_dx, bool want_dw, bool pack_w)
+// Tokens up to which a copy of the rows that count costs more than leaving some out gains: one tile of tokens either way.
+constexpr int64_t HD_FEW = 64;
+
+static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, bool backward, bool want_dx, bool want_dw, bool wide_x, bool pack_w)
 {
     HeadPlan h = {};
     h.tokens = tokens;
@@ -644,10 +682,10 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.want_dw = want_dw;
     const bool f32 = dtype == RDB_F32;
     const int64_t es = f32 ? 4 : 2;
-    h.dp = f32 ? (dim + 3) / 4 * 4 : (dim + 7) / 8 * 8;
+    h.dp = f32 ? dim : (dim + 7) / 8 * 8;
     h.pack_w = !f32 && pack_w;
     h.pad_dw = !f32 && h.dp != dim;
-    int64_t cols = HD_PIECE_BYTES / (es * tokens) / HD_TILE * HD_TILE;
+    int64_t cols = (f32 ? 2 * HD_PIECE_BYTES : head_piece_bytes(tokens, dim)) / (es * tokens) / HD_TILE * HD_TILE;
     if (f32) cols = std::min<int64_t>(cols, ((1ll << 29) - 1) / std::max<int64_t>(tokens, h.dp) / HD_TILE * HD_TILE);
     else cols = std::min<int64_t>(cols, ((1ll << 28)) / h.dp / HD_TILE * HD_TILE);
     cols = std::max<int64_t>(cols, HD_TILE);
@@ -655,7 +693,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.vp = cdiv(cdiv(classes, h.pieces), HD_TILE) * HD_TILE;
     if (f32 && h.pieces == 1) h.vp = classes;
     h.pieces = (int)cdiv(classes, h.vp);
-    h.bn = tokens <= 64 ? 64 : HD_TOK;
+    h.bn = tokens <= HD_FEW ? 64 : HD_TOK;
     const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, DUO_B);
     int64_t splits = std::max<int64_t>(1, 2 * num_compute_units() / std::max<int64_t>(1, tiles));
     splits = std::min(splits, std::max<int64_t>(1, h.vp / 1024));
@@ -668,9 +706,10 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         at += (bytes + 255) / 256 * 256;
         return o;
     };
-    h.xc = room(tokens * h.dp * es);
-    h.pos = room(tokens * 4);
-    h.count = room(4);
+    h.direct = !f32 && !backward && tokens <= HD_FEW && wide_x;
+    if (f32 ? want_dw : !h.direct) h.xc = room(tokens * h.dp * es);
+    if (!f32 && !h.direct) h.pos = room(tokens * 4);
+    h.count = room(8);
     if (h.pack_w) h.wc = room(classes * h.dp * 2);
     if (!backward) {
         h.nll = room(tokens * 4);
@@ -682,9 +721,11 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
             h.part = room(2 * cdiv(classes, HD_TILE) * tokens * 8);
         }
     } else {
-        h.lse2 = room(tokens * 4);
-        h.factor = room(tokens * 4);
-        h.label = room(tokens * 4);
+        if (!f32) {
+            h.lse2 = room(tokens * 4);
+            h.factor = room(tokens * 4);
+            h.label = room(tokens * 4);
+        }
         h.g = room(tokens * h.vp * es * (!f32 && h.pieces > 1 ? 2 : 1));   // bf16: a piece's, and the next one's beside it
         if (want_dx && (!f32 || h.pieces > 1)) h.dx = room((f32 ? 1 : h.splits) * tokens * (f32 ? dim : h.dp) * 4);
         if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2);
@@ -718,10 +759,9 @@ static bool head_aligned(const void *p, int64_t ld, int es) { return !((uintptr_
 static int head_gather(const HeadCall &c, const float *stats, const float *dloss_rows)
 {
     const HeadPlan &h = c.h;
-    const bool f32 = h.dtype == RDB_F32;
     HeadGather p = {};
-    p.xc = c.at<void>(h.xc);
-    p.x = c.x;
+    p.xc = c.at<bf16_t>(h.xc);
+    p.x = static_cast<const bf16_t *>(c.x);
     p.ldx = c.ldx;
     p.ldc = h.dp;
     p.target = c.target;
@@ -738,17 +778,14 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
     p.dim = h.dim;
     p.classes = h.classes;
     p.ignore = c.ignore;
-    p.rows = h.tokens > 16384 ? 64 : 16;
-    p.wide = head_aligned(c.x, c.ldx, f32 ? 4 : 2);
-    const unsigned grid = (unsigned)cdiv(h.tokens, p.rows);
-    if (f32) head_gather_kernel<float, false><<<grid, 256, 0, c.s>>>(p);
-    else head_gather_kernel<bf16_t, true><<<grid, 256, 0, c.s>>>(p);
+    p.rows = h.tokens > 16384 ? 64 : h.tokens > 4096 ? 8 : 4;
+    head_gather_kernel<<<(unsigned)cdiv(h.tokens, p.rows), 256, 0, c.s>>>(p);
     return check_launch("head_gather_kernel");
 }
-template <bool PAD> static int head_repack(bf16_t *dst, int64_t ldd, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, hipStream_t s)
+template <bool PAD> static int head_repack(bf16_t *dst, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, hipStream_t s)
 {
-    const int64_t per_block = std::max<int64_t>(1, 8192 / cols);   // four pieces a lane
-    head_repack_kernel<PAD><<<(unsigned)cdiv(rows, per_block), 256, 0, s>>>(dst, ldd, src, lds, rows, (int)cols, (int)per_block);
+    const int64_t per_block = std::max<int64_t>(1, 1024 / cols) * 8;   // four pieces a lane
+    head_repack_kernel<PAD><<<(unsigned)cdiv(rows, per_block), 256, 0, s>>>(dst, src, lds, rows, (int)cols, (int)per_block);
     return check_launch("head_repack_kernel");
 }
 // the weight as the tiles read it: rows from 16-byte boundaries on
@@ -758,7 +795,7 @@ static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
     *ldw = c.ldw;
     if (!c.h.pack_w) return RDB_OK;
     bf16_t *wc = c.at<bf16_t>(c.h.wc);
-    const int rc = head_repack<true>(wc, c.h.dp, *w, c.ldw, c.h.classes, c.h.dim, c.s);
+    const int rc = head_repack<true>(wc, *w, c.ldw, c.h.classes, c.h.dim, c.s);
     *w = wc;
     *ldw = c.h.dp;
     return rc;
@@ -785,28 +822,37 @@ template <bool GRAD> static int head_logits(HeadLogits &p, int bn, hipStream_t s
     return check_launch(GRAD ? "head_logits_duo_kernel<gradient>" : "head_logits_duo_kernel");
 }
 
+static HeadSum head_sum_of(const HeadCall &c, float *loss, float *stats, int reduction)
+{
+    const HeadPlan &h = c.h;
+    return {reduction == HD_NONE ? nullptr : loss, stats + h.tokens, reduction == HD_NONE ? loss : c.at<float>(h.nll), c.at<unsigned int>(h.count) + 1, c.target, h.tokens, c.ignore,
+            reduction == HD_MEAN};
+}
 static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
-    if (int rc = head_gather(c, nullptr, nullptr)) return rc;
+    if (!h.direct)
+        if (int rc = head_gather(c, nullptr, nullptr)) return rc;
     const bf16_t *w;
     int64_t ldw;
     if (int rc = head_weight(c, &w, &ldw)) return rc;
     HeadLogits p = {};
-    p.x = c.at<bf16_t>(h.xc);
-    p.ldx = h.dp;
+    p.x = h.direct ? static_cast<const bf16_t *>(c.x) : c.at<bf16_t>(h.xc);
+    p.ldx = h.direct ? c.ldx : h.dp;
     p.w = w;
     p.ldw = ldw;
-    p.count = c.at<int>(h.count);
+    p.count = h.direct ? nullptr : c.at<int>(h.count);
+    p.cleared = h.direct ? c.at<unsigned int>(h.count) + 1 : nullptr;
     p.dim = (int)h.dp;
     p.classes = (int)h.classes;
     p.tiles_v = (int)cdiv(h.classes, HD_TILE);
     p.part = c.at<float2>(h.part);
     p.tokens = h.tokens;
     if (int rc = head_logits<false>(p, h.bn, c.s)) return rc;
-    float *nll = reduction == HD_NONE ? loss : c.at<float>(h.nll);
-    const HeadMerge m = {stats, nll, p.part, c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.tokens, h.classes, c.target, 2 * p.tiles_v, (int)h.dp};
-    head_merge_kernel<<<(unsigned)cdiv(h.tokens, 16), 256, 0, c.s>>>(m);
+    const HeadMerge m = {stats, p.part, h.direct ? nullptr : c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.classes, 2 * p.tiles_v, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
+    // 16 lanes a token from as many tokens on as give every other compute unit a block of 64
+    if (h.tokens >= 8192) head_merge_kernel<16><<<(unsigned)cdiv(h.tokens, 64), 1024, 0, c.s>>>(m);
+    else head_merge_kernel<64><<<(unsigned)cdiv(h.tokens, 16), 1024, 0, c.s>>>(m);
     return check_launch("head_merge_kernel");
 }
 static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float *dloss, const float *stats, int reduction)
@@ -886,27 +932,30 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         head_dx_kernel<<<(unsigned)blocks, 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale);
         if (int rc = check_launch("head_dx_kernel")) return rc;
     }
-    if (dw && h.pad_dw) return head_repack<false>(dw, h.dim, dwc, h.dp, h.classes, h.dim, c.s);
+    if (dw && h.pad_dw) return head_repack<false>(dw, dwc, h.dp, h.classes, h.dim, c.s);
     return RDB_OK;
 }
 
+static HeadRows head_rows(const HeadCall &c)
+{
+    HeadRows p = {};
+    p.logits = c.at<float>(c.h.g);
+    p.classes = c.h.classes;
+    p.sum.target = c.target;
+    p.sum.ignore = c.ignore;
+    return p;
+}
 static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
-    if (int rc = head_gather(c, nullptr, nullptr)) return rc;
-    HeadRows p = {};
-    p.logits = c.at<float>(h.g);
+    HeadRows p = head_rows(c);
     p.state = c.at<float2>(h.part);
     p.picked = c.at<float>(h.picked);
-    p.target = c.target;
     p.stats = stats;
-    p.nll = reduction == HD_NONE ? loss : c.at<float>(h.nll);
-    p.tokens = h.tokens;
-    p.classes = h.classes;
-    p.ignore = c.ignore;
+    p.sum = head_sum_of(c, loss, stats, reduction);
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
-        if (int rc = rdb_product_f32(p.logits, c.at<float>(h.xc), h.dp, 0, static_cast<const float *>(c.w) + v0 * c.ldw, c.ldw, 0, nullptr, h.tokens, n, h.dim,
+        if (int rc = rdb_product_f32(p.logits, static_cast<const float *>(c.x), c.ldx, 0, static_cast<const float *>(c.w) + v0 * c.ldw, c.ldw, 0, nullptr, h.tokens, n, h.dim,
                                      c.at<void>(h.product), h.product_bytes, c.s))
             return rc;
         p.n = (int)n;
@@ -916,26 +965,28 @@ static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduct
         head_rows_stats_kernel<<<(unsigned)h.tokens, 256, 0, c.s>>>(p);
         if (int rc = check_launch("head_rows_stats_kernel")) return rc;
     }
-    return RDB_OK;
+    if (!p.sum.loss) return RDB_OK;
+    head_loss_kernel<<<1, 1024, 0, c.s>>>(p.sum);
+    return check_launch("head_loss_kernel");
 }
 static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dloss, const float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
-    if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr)) return rc;
-    HeadRows p = {};
-    p.logits = c.at<float>(h.g);
-    p.pos = c.at<int>(h.pos);
-    p.factor = c.at<float>(h.factor);
-    p.label = c.at<int>(h.label);
+    HeadRows p = head_rows(c);
     p.stats = const_cast<float *>(stats);
-    p.scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
+    p.scale = {dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
+    p.dloss = reduction == HD_NONE ? dloss : nullptr;
+    p.x = static_cast<const float *>(c.x);
+    p.ldx = c.ldx;
+    p.dim = (int)h.dim;
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
-        const float *w = static_cast<const float *>(c.w) + v0 * c.ldw, *xc = c.at<float>(h.xc);
+        const float *w = static_cast<const float *>(c.w) + v0 * c.ldw;
         void *room = c.at<void>(h.product);
-        if (int rc = rdb_product_f32(p.logits, xc, h.dp, 0, w, c.ldw, 0, nullptr, h.tokens, n, h.dim, room, h.product_bytes, c.s)) return rc;
+        if (int rc = rdb_product_f32(p.logits, p.x, c.ldx, 0, w, c.ldw, 0, nullptr, h.tokens, n, h.dim, room, h.product_bytes, c.s)) return rc;
         p.n = (int)n;
         p.v0 = (int)v0;
+        p.xc = dw && i == 0 ? c.at<float>(h.xc) : nullptr;
         head_rows_grad_kernel<<<(unsigned)h.tokens, 256, 0, c.s>>>(p);
         if (int rc = check_launch("head_rows_grad_kernel")) return rc;
         if (dx) {
@@ -947,7 +998,7 @@ static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dl
             }
         }
         if (dw)
-            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, xc, h.dp, 1, nullptr, n, h.dim, h.tokens, room, h.product_bytes, c.s)) return rc;
+            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, c.at<float>(h.xc), h.dim, 1, nullptr, n, h.dim, h.tokens, room, h.product_bytes, c.s)) return rc;
     }
     return RDB_OK;
 }
@@ -968,11 +1019,17 @@ static int check_head(const char *who, int64_t tokens, int64_t dim, int64_t clas
 
 using namespace rdb;
 
-extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *w, int64_t ldw, int backward, int want_dx,
-                                                            int want_dw)
+static HeadPlan head_plan_of(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, bool backward, bool want_dx, bool want_dw)
 {
-    if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, dim, ldw, 0)) return 0;
-    return head_plan(tokens, dim, classes, dtype, backward != 0, want_dx != 0, want_dw != 0, !head_aligned(w, ldw, 2) || dim % 8).total;
+    const bool whole = dim % 8 == 0;
+    return head_plan(tokens, dim, classes, dtype, backward, want_dx, want_dw, whole && head_aligned(x, ldx, 2), !whole || !head_aligned(w, ldw, 2));
+}
+
+extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                                                            int backward, int want_dx, int want_dw)
+{
+    if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, ldx, ldw, 0)) return 0;
+    return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward != 0, want_dx != 0, want_dw != 0).total;
 }
 
 extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
@@ -982,12 +1039,10 @@ extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const voi
     constexpr const char *who = "rdb_linear_cross_entropy_fwd";
     if (int rc = check_head(who, tokens, dim, classes, dtype, ldx, ldw, reduction)) return rc;
     if (!loss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
-    const HeadPlan h = head_plan(tokens, dim, classes, dtype, false, false, false, !head_aligned(w, ldw, 2) || dim % 8);
+    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, false, false, false);
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
-    if (int rc = dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, reduction) : head_fwd_bf16(c, loss, stats, reduction)) return rc;
-    head_loss_kernel<<<1, 1024, 0, c.s>>>(reduction == HD_NONE ? nullptr : loss, stats + tokens, c.at<float>(h.nll), target, tokens, ignore_index, reduction == HD_MEAN);
-    return check_launch("head_loss_kernel");
+    return dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, reduction) : head_fwd_bf16(c, loss, stats, reduction);
 }
 
 extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
@@ -999,7 +1054,7 @@ extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dlo
     if (!dx && !dw) return RDB_OK;
     if (!dloss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
     if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return set_error(RDB_E_ALIGN, "%s: dx and dw must be 16-byte aligned", who);
-    const HeadPlan h = head_plan(tokens, dim, classes, dtype, true, dx != nullptr, dw != nullptr, !head_aligned(w, ldw, 2) || dim % 8);
+    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, true, dx != nullptr, dw != nullptr);
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
     return dtype == RDB_F32 ? head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, reduction)

@@ -1131,7 +1131,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const auto f32 = x.options().dtype(at::kFloat);
         Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32);
         if (tokens) {
-            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), w.data_ptr(), w.stride(0), 0, 0, 0);
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), 0, 0, 0);
             const Tensor ws = bytes(need, x);
             check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), code(x.scalar_type()),
                                                target.data_ptr<int64_t>(), tokens, dim, classes, ignore, (int)reduction, ptr(ws), need, stream_of(x)),
@@ -1166,7 +1166,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         if (want_x) dx = at::empty({m[0], m[1]}, x.options());
         if (want_w) dw = m[0] ? at::empty({m[2], m[1]}, w.options()) : at::zeros({m[2], m[1]}, w.options());
         if (m[0] && (want_x || want_w)) {
-            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), w.data_ptr(), w.stride(0), 1, want_x, want_w);
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), 1, want_x, want_w);
             const Tensor ws = bytes(need, x);
             check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
                                                code(x.scalar_type()), saved[2].data_ptr<int64_t>(), m[0], m[1], m[2], m[3], (int)m[4], ptr(ws), need, stream_of(x)),

@@ -885,7 +885,7 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
     if tokens == 0:
         return loss.fill_(float("nan") if reduction == 1 else 0.0), stats.zero_()
     with _on(dev):
-        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(w), w.stride(0), 0, 0, 0))
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), x.stride(0), _p(w), w.stride(0), 0, 0, 0))
         ws = _workspace(n, dev)
         rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
                                             _p(ws), n, _stream(dev))
@@ -907,7 +907,7 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
     if tokens == 0:
         return dx, None if dw is None else dw.zero_()
     with _on(dev):
-        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(w), w.stride(0), 1, want_dx, want_dw))
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), x.stride(0), _p(w), w.stride(0), 1, want_dx, want_dw))
         ws = _workspace(n, dev)
         rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
                                             ignore_index, reduction, _p(ws), n, _stream(dev))

@@ -105,8 +105,9 @@ def test_the_library_refuses():
     L = _lib.load()
     one = 4096   # an address that nothing reads
     size = L.rdb_linear_cross_entropy_workspace_bytes
-    assert size(8, 64, 100, _lib.RDB_BF16, one, 64, 0, 0, 0) > 0
-    assert size(8, 64, 100, 7, one, 64, 0, 0, 0) == 0 and size(0, 64, 100, 1, one, 64, 0, 0, 0) == 0 and size(1 << 20, 1 << 10, 100, 1, one, 1 << 10, 0, 0, 0) == 0
+    assert size(8, 64, 100, _lib.RDB_BF16, one, 64, one, 64, 0, 0, 0) > 0
+    assert size(8, 64, 100, 7, one, 64, one, 64, 0, 0, 0) == 0 and size(0, 64, 100, 1, one, 64, one, 64, 0, 0, 0) == 0
+    assert size(1 << 20, 1 << 10, 100, 1, one, 1 << 10, one, 1 << 10, 0, 0, 0) == 0
     fwd = lambda **k: L.rdb_linear_cross_entropy_fwd(*{**dict(loss=one, stats=one, x=one, ldx=64, w=one, ldw=64, dtype=1, target=one, tokens=8, dim=64, classes=100,  # noqa: E731
                                                              ignore=-100, reduction=1, ws=one, n=0, stream=None), **k}.values())
     assert fwd() == -6 and fwd(dtype=2) == -3 and fwd(tokens=0) == -2 and fwd(dim=0) == -2 and fwd(classes=0) == -2 and fwd(ldx=63) == -2 and fwd(ldw=63) == -2
