@@ -99,39 +99,41 @@ __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
 }
 
 // Rows of `cols` bf16 values into rows of a multiple of 8 of them (PAD, zeros behind the last ones) or out of them into rows without gaps; a lane reads 8 values at any address
-// and writes them to a multiple of 16 bytes.  per_block: a multiple of 8.
+// and writes them to a multiple of 16 bytes.  per_block: a multiple of 8, at most 8192 values; out of padded rows it reads up to 14 bytes behind the last of them.
 template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *__restrict__ dst, const bf16_t *__restrict__ src, int64_t lds, int64_t rows, int cols, int per_block)
 {
     const int64_t r0 = (int64_t)blockIdx.x * per_block;
     const int mine = rows - r0 < per_block ? (int)(rows - r0) : per_block, out_cols = PAD ? (cols + 7) & ~7 : cols, total = mine * out_cols;
     src += r0 * lds;
     dst += r0 * out_cols;
-#pragma unroll 4
-    for (int i = threadIdx.x * 8; i < total; i += 2048) {
-        const int row = i / out_cols, c = i - row * out_cols;
-        const bf16_t *from = src + (int64_t)row * lds + c;
-        bf16_t v[8];
-        if (c + 8 <= cols) {
-            __builtin_memcpy(v, from, 16);
-        } else if (PAD) {
+    // whole pieces, but for those that would read behind the last row that there is
+    const int whole = cols < 8 ? 0 : PAD && r0 + mine == rows ? total - out_cols : total & ~7;
+    for (int i0 = threadIdx.x * 8; i0 < whole; i0 += 4 * 2048) {
+        u32x4 v[4], u[4];
+        int left[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? from[e] : (bf16_t)0;
-        } else {   // on into the next row (rows of fewer than 8 values: rows)
-            int r = row, k = c;
+        for (int q = 0; q < 4; ++q) {
+            const int i = min(i0 + q * 2048, whole - 8), row = i / out_cols, c = i - row * out_cols;
+            const bf16_t *from = src + (int64_t)row * lds + c;
+            left[q] = cols - c;   // values of this row; the others are zeros, or the next row's first
+            __builtin_memcpy(&v[q], from, 16);
+            u[q] = u32x4{0u, 0u, 0u, 0u};
+            if (!PAD) __builtin_memcpy(&u[q], left[q] < 8 ? from + lds - cols : from, 16);
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = r < mine ? src[(int64_t)r * lds + k] : (bf16_t)0;
-                if (++k == cols) {
-                    k = 0;
-                    ++r;
-                }
+        for (int q = 0; q < 4; ++q) {
+            const int i = i0 + q * 2048;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t m = (2 * e < left[q] ? 0xffffu : 0u) | (2 * e + 1 < left[q] ? 0xffff0000u : 0u);
+                v[q][e] = (v[q][e] & m) | (u[q][e] & ~m);
             }
+            if (i < whole) *reinterpret_cast<u32x4 *>(dst + i) = v[q];
         }
-        if (i + 8 <= total) {
-            __builtin_memcpy(__builtin_assume_aligned(dst + i, 16), v, 16);
-        } else {
-            for (int e = 0; i + e < total; ++e) dst[i + e] = v[e];
-        }
+    }
+    for (int i = whole + (int)threadIdx.x; i < total; i += 256) {
+        const int row = i / out_cols, c = i - row * out_cols;
+        dst[i] = c < cols ? src[(int64_t)row * lds + c] : (bf16_t)0;
     }
 }
 
@@ -728,7 +730,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         }
         h.g = room(tokens * h.vp * es * (!f32 && h.pieces > 1 ? 2 : 1));   // bf16: a piece's, and the next one's beside it
         if (want_dx && (!f32 || h.pieces > 1)) h.dx = room((f32 ? 1 : h.splits) * tokens * (f32 ? dim : h.dp) * 4);
-        if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2);
+        if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2 + 16);
     }
     if (f32) {
         h.product_bytes = rdb_product_f32_workspace_bytes(tokens, h.vp, dim);

@@ -15,14 +15,28 @@ int num_compute_units();
 constexpr int RT_TOKENS = 8;       // at most, of a block
 constexpr int RT_PAIRS = 1024;     // pairs of cosine and sine of a block at most
 
+// n / d for n < 2^31: (n + (n m >> 32)) >> l with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1
+struct RtDivide {
+    uint32_t d, m;
+    int l;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (n + __umulhi(n, m)) >> l; }
+};
+static RtDivide rt_divide(int64_t d)
+{
+    RtDivide r = {(uint32_t)d, 0, 0};
+    while ((1ll << r.l) < d) ++r.l;
+    r.m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << r.l) - (uint64_t)d)) / (uint64_t)d + 1);
+    return r;
+}
 struct RotaryRows {
     void *out;
     const void *in;
     int64_t sb, st, sh;   // elements
-    int heads;
+    RtDivide heads;
 };
 struct RotaryParams {
-    RotaryRows q, k;      // k.heads 0: none
+    RotaryRows q, k;      // k.heads.d 0: none
+    RtDivide units;       // pieces of a head
     const float *inv_freq;
     const void *positions;
     int64_t pb, pt;       // strides of positions
@@ -31,34 +45,34 @@ struct RotaryParams {
     float scale, sign;
 };
 
-template <typename E> struct RtPiece;   // 16 bytes as fp32 values
-template <> struct RtPiece<float> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void open(float (&v)[4], const u32x4 &w)
-    {
+// N values at once
+template <int N> __device__ __forceinline__ void rt_load(float (&v)[N], const float *p) { __builtin_memcpy(v, __builtin_assume_aligned(p, N * 4), N * 4); }
+template <int N> __device__ __forceinline__ void rt_store(float *p, const float (&v)[N]) { __builtin_memcpy(__builtin_assume_aligned(p, N * 4), v, N * 4); }
+template <int N> __device__ __forceinline__ void rt_load(float (&v)[N], const bf16_t *p)
+{
+    if constexpr (N == 1) {
+        v[0] = bf16_to_f32(*p);
+    } else {
+        uint32_t w[N / 2];
+        __builtin_memcpy(w, __builtin_assume_aligned(p, N * 2), N * 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
-    }
-    static __device__ __forceinline__ u32x4 close(const float (&v)[4]) { return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}; }
-};
-template <> struct RtPiece<bf16_t> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void open(float (&v)[8], const u32x4 &w)
-    {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < N / 2; ++e) {
             v[2 * e] = lo_f32(w[e]);
             v[2 * e + 1] = hi_f32(w[e]);
         }
     }
-    static __device__ __forceinline__ u32x4 close(const float (&v)[8])
-    {
-        u32x4 w;
+}
+template <int N> __device__ __forceinline__ void rt_store(bf16_t *p, const float (&v)[N])
+{
+    if constexpr (N == 1) {
+        *p = f32_to_bf16(v[0]);
+    } else {
+        uint32_t w[N / 2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = f32x2_to_bf16x2(v[2 * e], v[2 * e + 1]);
-        return w;
+        for (int e = 0; e < N / 2; ++e) w[e] = f32x2_to_bf16x2(v[2 * e], v[2 * e + 1]);
+        __builtin_memcpy(__builtin_assume_aligned(p, N * 2), w, N * 2);
     }
-};
+}
 
 __device__ __forceinline__ float2 rt_turn(const RotaryParams &p, int64_t b, int t, int i)
 {
@@ -74,70 +88,54 @@ __device__ __forceinline__ float2 rt_turn(const RotaryParams &p, int64_t b, int 
     return float2{(n & 2 ? -c : c) * p.scale, (n & 2 ? -s : s) * p.scale * p.sign};
 }
 
-// Whole pieces of 16 bytes: rows, strides, half the rotary part and the rest are multiples of them.
-template <typename E, bool INTERLEAVED> __device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows &x, const float2 *cs, int64_t b, int t0, int nt)
+// All heads of a block's tokens, N values (or N of either side of N pairs) a lane and step: rows, strides, the pairs' number and what is behind them are multiples of N.
+template <typename E, bool INTERLEAVED, int N>
+__device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows &x, const float2 *cs, int64_t b, int t0, int nt)
 {
-    constexpr int N = RtPiece<E>::N;
-    const int paired = INTERLEAVED ? 2 * p.pairs / N : p.pairs / N, units = paired + (p.dim - 2 * p.pairs) / N, per_token = x.heads * units, total = nt * per_token;
+    constexpr int P = INTERLEAVED ? (N > 1 ? N / 2 : 1) : N;   // pairs of a piece
+    const uint32_t paired = (uint32_t)p.pairs / P, total = (uint32_t)nt * x.heads.d * p.units.d;
     const E *in = static_cast<const E *>(x.in) + b * x.sb + (int64_t)t0 * x.st;
-    E *out = static_cast<E *>(x.out) + (b * p.seq + t0) * x.heads * p.dim;
+    E *out = static_cast<E *>(x.out) + (b * p.seq + t0) * x.heads.d * p.dim;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < total; i += 256) {
-        const int row = i / units, u = i - row * units, t = row / x.heads, h = row - t * x.heads;
+    for (uint32_t i = threadIdx.x; i < total; i += 256) {
+        const uint32_t row = p.units(i), u = i - row * p.units.d, t = x.heads(row), h = row - t * x.heads.d;
         const E *src = in + (int64_t)t * x.st + (int64_t)h * x.sh;
         E *dst = out + (int64_t)row * p.dim;
         if (u >= paired) {
-            const int c = 2 * p.pairs + (u - paired) * N;
-            *reinterpret_cast<u32x4 *>(dst + c) = *reinterpret_cast<const u32x4 *>(src + c);
+            const int c = 2 * p.pairs + (int)(u - paired) * N;
+            float a[N];
+            rt_load(a, src + c);
+            rt_store(dst + c, a);
             continue;
         }
-        const float2 *w = cs + t * p.pairs + u * (INTERLEAVED ? N / 2 : N);
-        float a[N];
-        RtPiece<E>::open(a, *reinterpret_cast<const u32x4 *>(src + u * N));
-        if (INTERLEAVED) {
+        const float2 *w = cs + t * p.pairs + u * P;
+        if constexpr (INTERLEAVED && N > 1) {
+            float a[N];
+            rt_load(a, src + u * N);
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
+            for (int e = 0; e < P; ++e) {
                 const float v = a[2 * e];
                 a[2 * e] = v * w[e].x + a[2 * e + 1] * w[e].y;
                 a[2 * e + 1] = a[2 * e + 1] * w[e].x - v * w[e].y;
             }
+            rt_store(dst + u * N, a);
         } else {
-            float c[N];
-            RtPiece<E>::open(c, *reinterpret_cast<const u32x4 *>(src + p.pairs + u * N));
+            const int ia = INTERLEAVED ? 2 * (int)u : (int)u * N, ib = INTERLEAVED ? ia + 1 : p.pairs + ia;
+            float a[N], c[N];
+            rt_load(a, src + ia);
+            rt_load(c, src + ib);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const float v = a[e];
                 a[e] = v * w[e].x + c[e] * w[e].y;
                 c[e] = c[e] * w[e].x - v * w[e].y;
             }
-            *reinterpret_cast<u32x4 *>(dst + p.pairs + u * N) = RtPiece<E>::close(c);
+            rt_store(dst + ia, a);
+            rt_store(dst + ib, c);
         }
-        *reinterpret_cast<u32x4 *>(dst + u * N) = RtPiece<E>::close(a);
     }
 }
-// Any sizes and strides: a pair, or a value of the rest, a lane and step.
-template <typename E, bool INTERLEAVED> __device__ __forceinline__ void rt_rows_any(const RotaryParams &p, const RotaryRows &x, const float2 *cs, int64_t b, int t0, int nt)
-{
-    const int units = p.dim - p.pairs, per_token = x.heads * units, total = nt * per_token;
-    const E *in = static_cast<const E *>(x.in) + b * x.sb + (int64_t)t0 * x.st;
-    E *out = static_cast<E *>(x.out) + (b * p.seq + t0) * x.heads * p.dim;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < total; i += 256) {
-        const int row = i / units, u = i - row * units, t = row / x.heads, h = row - t * x.heads;
-        const E *src = in + (int64_t)t * x.st + (int64_t)h * x.sh;
-        E *dst = out + (int64_t)row * p.dim;
-        if (u >= p.pairs) {
-            dst[p.pairs + u] = src[p.pairs + u];
-            continue;
-        }
-        const int ia = INTERLEAVED ? 2 * u : u, ib = INTERLEAVED ? 2 * u + 1 : p.pairs + u;
-        const float2 w = cs[t * p.pairs + u];
-        const float a = elem<E>::load(src + ia), c = elem<E>::load(src + ib);
-        elem<E>::store(dst + ia, a * w.x + c * w.y);
-        elem<E>::store(dst + ib, c * w.x - a * w.y);
-    }
-}
-template <typename E, bool INTERLEAVED, bool PIECES> __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p)
+template <typename E, bool INTERLEAVED, int N> __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p)
 {
     __shared__ float2 cs[RT_PAIRS];
     const int64_t b = blockIdx.x / p.blocks_per_seq;
@@ -147,28 +145,27 @@ template <typename E, bool INTERLEAVED, bool PIECES> __global__ __launch_bounds_
         cs[i] = rt_turn(p, b, t0 + t, i - t * p.pairs);
     }
     __syncthreads();
-    if (PIECES) {
-        rt_rows<E, INTERLEAVED>(p, p.q, cs, b, t0, nt);
-        if (p.k.heads) rt_rows<E, INTERLEAVED>(p, p.k, cs, b, t0, nt);
-    } else {
-        rt_rows_any<E, INTERLEAVED>(p, p.q, cs, b, t0, nt);
-        if (p.k.heads) rt_rows_any<E, INTERLEAVED>(p, p.k, cs, b, t0, nt);
-    }
+    rt_rows<E, INTERLEAVED, N>(p, p.q, cs, b, t0, nt);
+    if (p.k.heads.d) rt_rows<E, INTERLEAVED, N>(p, p.k, cs, b, t0, nt);
 }
 
-static bool rt_pieces(const rdb_rotary_rows *x, int es)
+// Whether rows may be taken n values at a time.
+static bool rt_pieces(const rdb_rotary_rows *x, int es, int n)
 {
-    const int n = 16 / es;
-    return !(((uintptr_t)x->in | (uintptr_t)x->out) & 15) && x->stride_batch % n == 0 && x->stride_token % n == 0 && x->stride_head % n == 0;
+    return !(((uintptr_t)x->in | (uintptr_t)x->out) & (n * es - 1)) && x->stride_batch % n == 0 && x->stride_token % n == 0 && x->stride_head % n == 0;
 }
-template <typename E> static int launch_rotary(const RotaryParams &p, int64_t blocks, bool pieces, bool interleaved, hipStream_t s)
+template <typename E, bool INTERLEAVED, int N> static int launch_rotary(const RotaryParams &p, int64_t blocks, hipStream_t s)
 {
-    const dim3 grid((unsigned)blocks);
-    if (pieces && interleaved) rotary_kernel<E, true, true><<<grid, 256, 0, s>>>(p);
-    else if (pieces) rotary_kernel<E, false, true><<<grid, 256, 0, s>>>(p);
-    else if (interleaved) rotary_kernel<E, true, false><<<grid, 256, 0, s>>>(p);
-    else rotary_kernel<E, false, false><<<grid, 256, 0, s>>>(p);
+    rotary_kernel<E, INTERLEAVED, N><<<(unsigned)blocks, 256, 0, s>>>(p);
     return check_launch("rotary_kernel");
+}
+template <typename E, bool INTERLEAVED> static int launch_rotary(const RotaryParams &p, int64_t blocks, int n, hipStream_t s)
+{
+    if constexpr (sizeof(E) == 2)
+        if (n == 8) return launch_rotary<E, INTERLEAVED, 8>(p, blocks, s);
+    if (n == 4) return launch_rotary<E, INTERLEAVED, 4>(p, blocks, s);
+    if (n == 2) return launch_rotary<E, INTERLEAVED, 2>(p, blocks, s);
+    return launch_rotary<E, INTERLEAVED, 1>(p, blocks, s);
 }
 
 }  // namespace rdb
@@ -192,10 +189,10 @@ extern "C" int rdb_rotary(const rdb_rotary_rows *q, const rdb_rotary_rows *k, in
     if (!batch || !seq || !q->heads) return RDB_OK;
     if (k && !k->heads) k = nullptr;
     if (!q->in || !q->out || (k && (!k->in || !k->out))) return set_error(RDB_E_NULL, "rdb_rotary: an input or output is NULL");
-    const int es = dtype == RDB_BF16 ? 2 : 4, n = 16 / es;
+    const int es = dtype == RDB_BF16 ? 2 : 4;
     RotaryParams p = {};
-    p.q = {q->out, q->in, q->stride_batch, q->stride_token, q->stride_head, (int)q->heads};
-    if (k) p.k = {k->out, k->in, k->stride_batch, k->stride_token, k->stride_head, (int)k->heads};
+    p.q = {q->out, q->in, q->stride_batch, q->stride_token, q->stride_head, rt_divide(q->heads)};
+    if (k) p.k = {k->out, k->in, k->stride_batch, k->stride_token, k->stride_head, rt_divide(k->heads)};
     p.inv_freq = inv_freq;
     p.positions = positions;
     p.pb = pos_stride_batch;
@@ -213,7 +210,11 @@ extern "C" int rdb_rotary(const rdb_rotary_rows *q, const rdb_rotary_rows *k, in
     p.blocks_per_seq = (int)cdiv(seq, p.tokens);
     const int64_t blocks = batch * p.blocks_per_seq;
     if (blocks >= (1ll << 31)) return set_error(RDB_E_UNSUPPORTED, "rdb_rotary: too many sequences");
-    const bool pieces = rt_pieces(q, es) && (!k || rt_pieces(k, es)) && head_dim % n == 0 && (interleaved ? 2 * pairs : pairs) % n == 0;
-    return dtype == RDB_BF16 ? launch_rotary<bf16_t>(p, blocks, pieces, interleaved != 0, (hipStream_t)stream)
-                             : launch_rotary<float>(p, blocks, pieces, interleaved != 0, (hipStream_t)stream);
+    int n = 16 / es;   // values a lane takes at once
+    while (n > 1 && !(rt_pieces(q, es, n) && (!k || rt_pieces(k, es, n)) && head_dim % n == 0 && (interleaved ? 2 * pairs : pairs) % n == 0)) n /= 2;
+    const int64_t paired = interleaved && n > 1 ? 2 * pairs / n : pairs / n;
+    p.units = rt_divide(paired + (head_dim - 2 * pairs) / n);
+    const auto stream_ = (hipStream_t)stream;
+    if (dtype == RDB_BF16) return interleaved ? launch_rotary<bf16_t, true>(p, blocks, n, stream_) : launch_rotary<bf16_t, false>(p, blocks, n, stream_);
+    return interleaved ? launch_rotary<float, true>(p, blocks, n, stream_) : launch_rotary<float, false>(p, blocks, n, stream_);
 }
