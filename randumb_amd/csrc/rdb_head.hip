@@ -81,20 +81,26 @@ __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
         }
     }
     __syncthreads();
-    const int chunks = (int)(p.ldc / 8);
-#pragma unroll 4
-    for (int i = t; i < mine * chunks; i += 256) {
-        const int row = i / chunks, col = (i - row * chunks) * 8, at = place_[row];
-        if (at < 0) continue;
-        const bf16_t *src = p.x + (r0 + row) * p.ldx + col;
-        bf16_t v[8];
-        if (col + 8 <= p.dim) {
-            __builtin_memcpy(v, src, 16);
-        } else {
+    // 8 values a lane, at any address; a ragged piece of the last row that there is one by one: 16 bytes would reach behind it
+    const int chunks = (int)(p.ldc / 8), dim = (int)p.dim, total = mine * chunks, whole = dim % 8 && r0 + mine == p.tokens ? total - 1 : total;
+    for (int i0 = t; i0 < whole; i0 += 1024) {
+        u32x4 v[4];
+        bf16_t *to[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = col + j < p.dim ? src[j] : (bf16_t)0;
+        for (int q = 0; q < 4; ++q) {
+            const int i = min(i0 + q * 256, whole - 1), row = i / chunks, col = (i - row * chunks) * 8, at = place_[row], left = dim - col;
+            __builtin_memcpy(&v[q], p.x + (r0 + row) * p.ldx + col, 16);
+            to[q] = at < 0 || i0 + q * 256 >= whole ? nullptr : p.xc + (int64_t)at * p.ldc + col;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
         }
-        __builtin_memcpy(__builtin_assume_aligned(p.xc + (int64_t)at * p.ldc + col, 16), v, 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (to[q]) *reinterpret_cast<u32x4 *>(to[q]) = v[q];
+    }
+    if (whole < total && t < 8 && place_[mine - 1] >= 0) {
+        const int col = (chunks - 1) * 8 + t;
+        p.xc[(int64_t)place_[mine - 1] * p.ldc + col] = col < dim ? p.x[(p.tokens - 1) * p.ldx + col] : (bf16_t)0;
     }
 }
 

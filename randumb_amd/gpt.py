@@ -10,10 +10,11 @@ and the language-model head are ordinary dense layers unless the configuration a
 plain layers, whose squared ReLU is formed and differentiated in the kernels that store their rows (RT_MLP).  The rest of a
 block (normalisation, rotary attention with a head dimension of 64, squared ReLU, the loss) is stock PyTorch, except in bf16 on the
 GPU, run eagerly: chains of stock operators took 6 times what the linears' kernels take there, most of it in passes over memory
-that the fused ones do not make.
+that the fused ones do not make.  Where the configuration asks for it, the loss is formed without the logits (ops.linear_cross_entropy) and positions
+turn other pairs, parts of the heads or by other frequencies (ops.rotary).
 """
 from dataclasses import dataclass
-from typing import Generator
+from typing import Generator, Optional
 
 import torch
 import torch.nn.functional as F
@@ -57,13 +58,29 @@ def _add_norm(x: torch.Tensor, delta: torch.Tensor):
 
 
 class Rotary(nn.Module):
-    """Rotary position embedding over (batch, time, head, head_dim), as gpt_models.py:29-49."""
+    """Rotary position embedding over (batch, time, head, head_dim), as gpt_models.py:29-49.  With any of the further arguments its layout and
+    frequencies are those of :func:`ops.rotary` and :func:`ops.rotary_frequencies`, on the GPU, the frequencies fp32 whatever the module's type:
+    neighbouring pairs (``interleaved``), the first ``rotary_dim`` values of a head, ``scaling`` for longer contexts."""
 
-    def __init__(self, dim: int, base: float = 10000.0):
+    def __init__(self, dim: int, base: float = 10000.0, *, interleaved: bool = False, rotary_dim: Optional[int] = None, **scaling):
         super().__init__()
-        self.register_buffer("inv_freq", (1.0 / base) ** (torch.arange(0, dim, 2) / dim), persistent=False)
+        self.stock = not interleaved and rotary_dim is None and not scaling
+        self.interleaved, self.scale = interleaved, 1.0
+        if self.stock:
+            self.register_buffer("inv_freq", (1.0 / base) ** (torch.arange(0, dim, 2) / dim), persistent=False)
+        else:
+            if rotary_dim is not None and not 2 <= rotary_dim <= dim:
+                raise ValueError(f"Rotary: between 2 and {dim} values of a head, got {rotary_dim}")
+            freq, self.scale = ops.rotary_frequencies(dim if rotary_dim is None else rotary_dim, base, **scaling)
+            self.register_buffer("freq_bits", freq.view(torch.int32), persistent=False)   # as whole numbers: a module's change of type leaves them alone
+
+    def both(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None):
+        """Queries and keys (or None) in one launch."""
+        return ops.rotary(q, k, self.freq_bits.to(q.device).view(torch.float32), positions, interleaved=self.interleaved, scale=self.scale)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not self.stock:
+            return self.both(x, None)[0]
         t = torch.arange(x.shape[1], device=x.device)
         freqs = torch.outer(t, self.inv_freq.to(x.device))
         cos, sin = freqs.cos()[None, :, None, :], freqs.sin()[None, :, None, :]
@@ -82,6 +99,11 @@ class RT_GPTConfig:
     # True: the token embedding and the output head are random-backed too, as in the reference's model
     # (modded-nanogpt/gpt_models.py:303, 310); they then draw the first and the last (k, seed) of the generators
     random_embedding_and_head: bool = False
+    # True: the loss comes from the head's input and weight (or coefficients), on the GPU, without the logits ever being in memory, and without
+    # their rounding to bf16
+    loss_without_logits: bool = False
+    # further arguments of Rotary (interleaved, rotary_dim, base, scaling, factor, ...)
+    rotary: Optional[dict] = None
 
 
 class RT_CastedLinear(SillyLinear):
@@ -102,20 +124,20 @@ class RT_CausalSelfAttention(nn.Module):
         assert dim % n_head == 0
         self.n_head = n_head
         self.c_qkv = RT_CastedLinear(dim, 3 * dim, config)
-        self.rotary = Rotary(dim // n_head)
+        self.rotary = Rotary(dim // n_head, **(config.rotary or {}))
         self.c_proj = RT_CastedLinear(dim, dim, config)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, T, D = x.shape
         qkv = self.c_qkv(x)
         ext = _fused(qkv)
-        if ext is not None and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
+        if ext is not None and self.rotary.stock and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
             y = ext.causal_attention(qkv, self.rotary.inv_freq, self.n_head, _EPS)
             if y is not None:
                 return self.c_proj(y)
         q, k, v = qkv.view(B, T, 3, self.n_head, D // self.n_head).unbind(2)
         q, k = RT_norm(q), RT_norm(k)
-        q, k = self.rotary(q), self.rotary(k)
+        q, k = (self.rotary(q), self.rotary(k)) if self.rotary.stock else self.rotary.both(q, k)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
         return self.c_proj(y.transpose(1, 2).reshape(B, T, D))
 
@@ -213,7 +235,7 @@ class RT_Block(nn.Module):
 
 
 # as they stand here: replaced ones are called
-_BLOCK_FORWARD, _LINEAR_FORWARD, _EMBEDDING_FORWARD, _MODULE_CALL = RT_Block.forward, RT_CastedLinear.forward, nn.Embedding.forward, nn.Module.__call__
+_BLOCK_FORWARD, _LINEAR_FORWARD, _EMBEDDING_FORWARD, _DENSE_FORWARD, _MODULE_CALL = RT_Block.forward, RT_CastedLinear.forward, nn.Embedding.forward, nn.Linear.forward, nn.Module.__call__
 
 
 def _embed(wte: nn.Module, idx: torch.Tensor) -> torch.Tensor:
@@ -242,6 +264,29 @@ class RT_GPT(nn.Module):
             self.lm_head = RT_CastedLinear(config.n_embd, config.vocab_size, config)
         else:
             self.lm_head = nn.Linear(config.n_embd, config.vocab_size, bias=False)
+        self.loss_without_logits = config.loss_without_logits
+        if config.loss_without_logits and config.random_embedding_and_head:
+            self.register_buffer("unit_coefs", torch.eye(self.lm_head.weight_coef.shape[1]), persistent=False)
+
+    def _loss_without_logits(self, x: torch.Tensor, target: torch.Tensor) -> Optional[torch.Tensor]:
+        """The loss of the head's input; None where the head is more than its product, or not on the GPU."""
+        head = self.lm_head
+        if not x.is_cuda or torch.is_autocast_enabled():
+            return None
+        if type(head) is nn.Linear and nn.Linear.forward is _DENSE_FORWARD:
+            w = head._parameters.get("weight")
+            if not _unhooked(head) or head.bias is not None or w is None or w.dtype != x.dtype:
+                return None
+            return ops.linear_cross_entropy(x, w, target)
+        if type(head) is not RT_CastedLinear or RT_CastedLinear.forward is not _LINEAR_FORWARD or not _unhooked(head):
+            return None
+        w, coef = head.weight, head.weight_coef
+        if w.fused_bias or head.bias is not None or coef.dtype != x.dtype:
+            return None
+        # logits = z . C^T with z = x . N^T, which is what a layer with the identity's coefficients gives: the vocabulary meets k values a token
+        k, d = coef.shape[1], head.in_features
+        z = ops.linear(x.reshape(-1, d), self.unit_coefs, d, k, d, 1, w.seed, None, None)
+        return ops.linear_cross_entropy(z, coef, target.reshape(-1))
 
     def forward(self, idx: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
         x = _embed(self.wte, idx)
@@ -252,7 +297,11 @@ class RT_GPT(nn.Module):
                 x, normed = block._with_norm(x, RT_norm(x) if normed is None else normed)
             else:
                 x, normed = block(x), None
-        logits = self.lm_head(RT_norm(x) if normed is None else normed)
+        normed = RT_norm(x) if normed is None else normed
+        loss = self._loss_without_logits(normed, target) if self.loss_without_logits else None
+        if loss is not None:
+            return loss
+        logits = self.lm_head(normed)
         ext = _fused(logits)
         if ext is not None and logits.size(-1) % 8 == 0 and logits.numel() and target.dtype is torch.int64:
             loss = ext.cross_entropy(logits.view(-1, logits.size(-1)), target.view(-1), -100)
