@@ -548,6 +548,7 @@ __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, c
         const int c = (int)(i - row * chunks) * 4, at = pos[row];
         f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (at >= 0) {
+#pragma unroll 8
             for (int s = 0; s < splits; ++s) {
                 const f32x4 u = *reinterpret_cast<const f32x4 *>(sums + s * stride + at * ld + c);
 #pragma unroll
@@ -703,9 +704,11 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.pieces = (int)cdiv(classes, h.vp);
     h.bn = tokens <= HD_FEW ? 64 : HD_TOK;
     const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, DUO_B);
+    // Ranges of the classes, each with sums of dx of its own, until every block slot has a tile: at least 4 stages each, and 16 ranges or 16 MB of sums (24 tokens x 960 ->
+    // 39040: 16 ranges of 38 stages 60 us, 64 of 10 35; 5 x 64 -> 1792: one of 28 24 us, 7 of 4 7).
     int64_t splits = std::max<int64_t>(1, 2 * num_compute_units() / std::max<int64_t>(1, tiles));
-    splits = std::min(splits, std::max<int64_t>(1, h.vp / 1024));
-    splits = std::min<int64_t>(splits, 16);
+    splits = std::min(splits, cdiv(std::min(h.vp, classes), 4 * DUO_K));
+    splits = std::min(splits, std::max<int64_t>(16, std::min<int64_t>(64, (16ll << 20) / (tokens * h.dp * 4))));
     h.split_v = cdiv(cdiv(h.vp, splits), 64) * 64;
     h.splits = (int)cdiv(std::min(h.vp, classes), h.split_v);   // the first piece's: it writes all the sums that there are
     int64_t at = 0;
