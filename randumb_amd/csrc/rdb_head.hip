@@ -7,7 +7,7 @@
 // Rows whose target is the ignored label are left out before anything is multiplied (head_gather_kernel): they cost nothing, and what they hold, NaN
 // included, reaches no sum.  A target outside the classes makes its row NaN.
 //
-// bf16 (products on 256-wide tiles, rdb_big.hpp):
+// bf16 (products on the tiles of rdb_duo.hpp, of few tokens on those of rdb_gemm.hpp):
 //   head_gather_kernel    the rows that count, one after the other, in rows of a multiple of 8 values
 //   head_stats_kernel     a 256 x 256 tile of logits in the accumulators -> its maximum and its sum of exponentials for each token
 //   head_merge_kernel     those of a token together, the target's logit, nll
@@ -18,7 +18,6 @@
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
 // which are nearly all of the gradient, would all be off by the same rounding.
 // fp32: the same steps with the products of rdb_f32.hip, logits of a piece in fp32 in between.
-#include "rdb_big.hpp"
 #include "rdb_duo.hpp"
 #include <algorithm>
 
@@ -27,6 +26,7 @@ namespace rdb {
 int num_compute_units();
 
 constexpr int HD_TILE = 256, HD_TOK = DUO_B;
+constexpr uint32_t HD_OOB = 0xfffffff0u;   // outside a buffer of any size up to 2^32 - 16 bytes
 constexpr float HD_LOG2E = 1.44269504088896340736f, HD_LN2 = 0.69314718055994530942f;
 enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
 
@@ -151,7 +151,7 @@ struct HeadLogits {
     const int *count;     // NULL: all tokens
     unsigned int *cleared;   // NULL, or a word that block 0 sets to zero for a later launch
     int dim, classes, v0;     // classes v0 .. v0 + tiles_v * 256 of this launch
-    int tiles_v, tiles_t;
+    int tiles_v;
     float2 *part;         // stats: [2 * tiles_v][tokens]: maximum (times log2 e) and sum
     int64_t tokens;
     bf16_t *g;            // gradient: [tokens][ldg], class v0 first
@@ -159,39 +159,46 @@ struct HeadLogits {
     const float *lse2, *factor;
     const int *label;
 };
-// as big_y_decode: 32 neighbouring items, which a die runs at a time, share 8 tiles of the weight and 4 of the tokens
-__device__ __forceinline__ void head_decode(int w, int tiles_v, int tiles_t, int &tv, int &tt)
-{
-    const int per_group = 4 * tiles_v, group = w / per_group, in_group = w - group * per_group, first = group * 4;
-    const int size = min(4, tiles_t - first);
-    tv = in_group / size;
-    tt = first + in_group - tv * size;
-}
 __device__ __forceinline__ int head_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
 
-// maximum and sum of exponentials over the tile's classes, for each of the wave's tokens; each wave leaves its 128 classes' own
-template <int NI>
-__device__ __forceinline__ void head_leave_stats(f32x16 (&acc)[4][NI], const HeadLogits &p, int tv, int tok0, int count, int t)
+// Tiles of MI * 64 classes x NI * 64 tokens, waves 2 x 2.
+// Maximum (times log2 e) and sum of exponentials over a wave's `left` classes, of its ni-th 32 tokens.
+template <int MI, int NI> __device__ __forceinline__ void head_stats(const f32x16 (&acc)[MI][NI], int ni, int left, int g, float &m, float &s)
+{
+    constexpr int N = MI * 16;
+    float v[N];
+    m = -INFINITY;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = acc[i >> 4][ni][i & 15];
+    if (left < MI * 32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((i >> 4) * 32 + head_row(i & 15, g) >= left) v[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
+    m = fmaxf(m, __shfl_xor(m, 32, 64)) * HD_LOG2E;
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], HD_LOG2E, -ref));
+    s += __shfl_xor(s, 32, 64);
+}
+__device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
+{
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
+    m = top;
+}
+// ... for each of the wave's tokens; each wave leaves its half of the classes' own
+template <int MI, int NI>
+__device__ __forceinline__ void head_leave_stats(const f32x16 (&acc)[MI][NI], const HeadLogits &p, int tv, int tok0, int count, int t)
 {
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
-    const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;   // classes of this wave's rows that there are
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
-        float v[64], m = -INFINITY, s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = acc[i >> 4][ni][i & 15];
-        if (left < 128) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-                if ((i >> 4) * 32 + head_row(i & 15, g) >= left) v[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 64; ++i) m = fmaxf(m, v[i]);
-        m = fmaxf(m, __shfl_xor(m, 32, 64)) * HD_LOG2E;
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], HD_LOG2E, -ref));
-        s += __shfl_xor(s, 32, 64);
+        float m, s;
+        head_stats(acc, ni, p.classes - (p.v0 + (tv * 2 + wm) * MI * 32), g, m, s);
         const int tok = tok0 + wn * NI * 32 + ni * 32 + r;
         if (g == 0 && tok < count) p.part[(int64_t)(tv * 2 + wm) * p.tokens + tok] = float2{m, s};
         __builtin_amdgcn_sched_barrier(0);
@@ -199,94 +206,90 @@ __device__ __forceinline__ void head_leave_stats(f32x16 (&acc)[4][NI], const Hea
 }
 
 // G of the tile, through LDS into whole rows; classes past the last one are zeros
-template <int NI>
-__device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[4][NI], bf16_t *__restrict__ lds, const HeadLogits &p, int tv, int tok0, int count, int t)
+template <int MI, int NI>
+__device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *__restrict__ lds, const HeadLogits &p, int tv, int tok0, int count, int t)
 {
-    constexpr int BN = NI * 64, LD = HD_TILE + 8;
+    constexpr int HALF = MI * 32, N = MI * 16, BM = MI * 64, BN = NI * 64, LD = BM + 8;
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
-    const int first = p.v0 + tv * HD_TILE + wm * 128, left = p.classes - first;
+    const int first = p.v0 + tv * BM + wm * HALF, left = p.classes - first;
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
         const int b = wn * NI * 32 + ni * 32 + r, tok = min(tok0 + b, count - 1);
         const float l = p.lse2[tok], f = p.factor[tok];
         const int rel = p.label[tok] - first;
-        float v[64];
+        float v[N];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc[i >> 4][ni][i & 15], HD_LOG2E, -l));
-        if (__any((unsigned)rel < 128u)) {
+        for (int i = 0; i < N; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc[i >> 4][ni][i & 15], HD_LOG2E, -l));
+        if (__any((unsigned)rel < (unsigned)HALF)) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
+            for (int i = 0; i < N; ++i)
                 if ((i >> 4) * 32 + head_row(i & 15, g) == rel) v[i] -= 1.0f;
         }
-        if (left < 128) {
+        if (left < HALF) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
+            for (int i = 0; i < N; ++i)
                 if ((i >> 4) * 32 + head_row(i & 15, g) >= left) v[i] = 0.0f;
         }
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-            store4<bf16_t>(lds + b * LD + wm * 128 + (q >> 2) * 32 + 8 * (q & 3) + 4 * g, v[q * 4] * f, v[q * 4 + 1] * f, v[q * 4 + 2] * f, v[q * 4 + 3] * f);
+        for (int q = 0; q < MI * 4; ++q)
+            store4<bf16_t>(lds + b * LD + wm * HALF + (q >> 2) * 32 + 8 * (q & 3) + 4 * g, v[q * 4] * f, v[q * 4 + 1] * f, v[q * 4 + 2] * f, v[q * 4 + 3] * f);
         __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    bf16_t *out = p.g + (int64_t)tok0 * p.ldg + (int64_t)tv * HD_TILE;
-    const int a = (t & 31) * 8;
+    constexpr int LPR = BM / 8, RPP = 256 / LPR;   // lanes a row, rows at once
+    bf16_t *out = p.g + (int64_t)tok0 * p.ldg + (int64_t)tv * BM;
+    const int a = (t % LPR) * 8;
 #pragma unroll 8
-    for (int q = 0; q < BN / 8; ++q) {
-        const int b = q * 8 + (t >> 5);
+    for (int q = 0; q < BN / RPP; ++q) {
+        const int b = q * RPP + t / LPR;
         if (tok0 + b < count) *reinterpret_cast<f32x4 *>(out + (int64_t)b * p.ldg + a) = *reinterpret_cast<const f32x4 *>(lds + b * LD + a);
     }
-    __syncthreads();
 }
 
-template <int BN, bool GRAD> __global__ __launch_bounds__(256, 1) void head_logits_kernel(HeadLogits p)
+// Few tokens, one tile of them: bound by the weight, which is read once.  Tiles of 64 classes, so that many blocks have loads on their way, four stages of 64 x 64 each
+// ahead; statistics by up to two blocks a compute unit, each with several tiles in turn and one part for all of them: parts are what the merging kernel's time goes by.
+// us a forward call, 256 x 64 tiles of rdb_big.hpp -> so: 64 tokens x 4096 -> 16384 57 -> 32, 32 x 1000 -> 100000 58.6 -> 56.9, 16 x 768 -> 50304 22.7 -> 23.8
+// (77 MB of weight: 15 at the rate of a large copy); 256 x 128 on two blocks a compute unit 75, 60.5, 26.1.
+constexpr int HF_V = 64, HF_T = 64, HF_AHEAD = 4;
+template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_few_kernel(HeadLogits p)
 {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    bf16_t *lds = reinterpret_cast<bf16_t *>(smem_raw);
-    typedef GlobalOperand<HD_TILE, 64, K_CONT> PA;
-    typedef GlobalOperand<BN, 64, K_CONT> PB;
-    const int count = p.count ? *p.count : (int)p.tokens, tiles_t = (count + BN - 1) / BN, total = p.tiles_v * tiles_t, vtotal = (total + 7) / 8 * 8, nstage = (p.dim + 63) / 64;
-    int v = (int)blockIdx.x;
-    auto next = [&]() {
-        for (; v < vtotal; v += gridDim.x) {
-            const int w = xcd_work_item(v, total);
-            if (w < total) {
-                v += gridDim.x;
-                return w;
-            }
-        }
-        return -1;
-    };
+    typedef GlobalOperand<HF_V, 64, K_CONT> PA;
+    typedef GlobalOperand<HF_T, 64, K_CONT> PB;
+    __shared__ __align__(16) bf16_t lds[2 * (PA::Tile::LDS_ELEMS + PB::Tile::LDS_ELEMS)];
+    __shared__ float ms_[2][2][32];
     if (p.cleared && blockIdx.x == 0 && threadIdx.x == 0) *p.cleared = 0u;
-    PA pa;
-    PB pb;
-    BigRegs<PA, PB> regs;
-    auto request = [&](int w) {
-        int tv, tt;
-        head_decode(w, p.tiles_v, tiles_t, tv, tt);
-        const int row = p.v0 + tv * HD_TILE, rows = min(HD_TILE, p.classes - row), tok = tt * BN, toks = min(BN, count - tok);
-        pa = PA{p.w + (int64_t)row * p.ldw, p.ldw, 0, rows, p.dim, (int64_t)(rows - 1) * p.ldw + p.dim};
-        pb = PB{p.x + (int64_t)tok * p.ldx, p.ldx, 0, toks, p.dim, (int64_t)(toks - 1) * p.ldx + p.dim};
-        big_prefetch(regs, pa, pb, 0);
-    };
-    int w = next();
-    if (w < 0) return;
-    request(w);
-    while (true) {
-        int tv, tt;
-        head_decode(w, p.tiles_v, tiles_t, tv, tt);
-        f32x16 acc[4][BN / 64];
-        big_zero<HD_TILE, BN>(acc);
-        big_mainloop<HD_TILE, BN>(acc, lds, regs, pa, pb, nstage);
-        const int wn = next();
-        if (wn >= 0) request(wn);   // on its way during the epilogue
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (GRAD) head_leave_grad<BN / 64>(acc, lds, p, tv, tt * BN, count, opaque_tid());
-        else head_leave_stats<BN / 64>(acc, p, tv, tt * BN, count, opaque_tid());
-        if (wn < 0) break;
-        w = wn;
+    const int count = p.count ? *p.count : (int)p.tokens;
+    if (count <= 0) return;
+    const int t = threadIdx.x, lane = t & 63, r = lane & 31, g = lane >> 5, wm = t >> 7, wn = (t >> 6) & 1;
+    float m = -INFINITY, s = 0.0f;
+    for (int tv = (int)blockIdx.x; tv < p.tiles_v; tv += (int)gridDim.x) {
+        const int row = p.v0 + tv * HF_V, rows = min(HF_V, p.classes - row);
+        PA pa = {p.w + (int64_t)row * p.ldw, p.ldw, 0, rows, p.dim, (int64_t)(rows - 1) * p.ldw + p.dim};
+        PB pb = {p.x, p.ldx, 0, count, p.dim, (int64_t)(count - 1) * p.ldx + p.dim};
+        f32x16 acc[1][1] = {{zero16()}};
+        gemm_mainloop<HF_V, HF_T, 64, HF_AHEAD, HF_AHEAD>(acc, lds, pa, pb, 0, (p.dim + 63) / 64);
+        if constexpr (GRAD) {
+            head_leave_grad<1, 1>(acc, lds, p, tv, 0, count, t);
+            __syncthreads();
+        } else {
+            float m2, s2;
+            head_stats(acc, 0, p.classes - (row + wm * 32), g, m2, s2);
+            head_join(m, s, m2, s2);
+        }
+    }
+    if constexpr (!GRAD) {
+        if (wm == 1 && g == 0) {
+            ms_[0][wn][r] = m;
+            ms_[1][wn][r] = s;
+        }
+        __syncthreads();
+        if (wm == 0 && g == 0) {
+            head_join(m, s, ms_[0][wn][r], ms_[1][wn][r]);
+            if (wn * 32 + r < count) p.part[(int64_t)blockIdx.x * p.tokens + wn * 32 + r] = float2{m, s};
+        }
     }
 }
+static int head_few_blocks(int64_t classes) { return (int)std::min<int64_t>(cdiv(classes, HF_V), 2 * num_compute_units()); }
 
 // The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
 template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
@@ -302,8 +305,8 @@ template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const Head
     f32x16 acc[DUO_MI][DUO_NI];
     duo_zero(acc);
     duo_mainloop(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
-    if constexpr (GRAD) head_leave_grad<DUO_NI>(acc, lds, p, tv, tok0, count, opaque_tid());
-    else head_leave_stats<DUO_NI>(acc, p, tv, tok0, count, opaque_tid());
+    if constexpr (GRAD) head_leave_grad<DUO_MI, DUO_NI>(acc, lds, p, tv, tok0, count, (int)threadIdx.x);
+    else head_leave_stats<DUO_MI, DUO_NI>(acc, p, tv, tok0, count, (int)threadIdx.x);
 }
 template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
 {
@@ -374,12 +377,6 @@ template <int THREADS> __device__ __forceinline__ void head_sum(const HeadSum &p
     if (last_) head_add_up<THREADS>(p);
 }
 
-__device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
-{
-    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
-    m = top;
-}
 struct HeadMerge {
     float *stats;          // [tokens]: lse, 0 in ignored rows
     const float2 *part;    // [parts][tokens], by place
@@ -480,7 +477,7 @@ __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], b
 #pragma unroll
         for (int q = 0; q < 32 / RPP; ++q) {
             const int row = q * RPP + lane / LPR, a = wm * DUO_MI * 32 + mi * 32 + row;
-            const uint32_t off = (a < na && b < nb) ? (uint32_t)(((int64_t)a * ld + b) * (int)sizeof(E)) : BUFFER_OOB_ANY;
+            const uint32_t off = (a < na && b < nb) ? (uint32_t)(((int64_t)a * ld + b) * (int)sizeof(E)) : HD_OOB;
             f32x4 v = *reinterpret_cast<const f32x4 *>(patch + row * LDP + col);
             if constexpr (sizeof(E) == 2) {
                 const f32x4 u = *reinterpret_cast<const f32x4 *>(patch + row * LDP + col + 4);
@@ -522,7 +519,7 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
         pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
         pb.set(p.x, p.ldx, b0, p.dim, count);
         duo_mainloop(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
-        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), opaque_tid());
+        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), (int)threadIdx.x);
     } else {
         const int tt = w / p.tiles_d % tiles_t, s = w / p.tiles_d / tiles_t, v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE;
         const int toks = min(HD_TILE, count - tok);
@@ -531,7 +528,7 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
         pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7);
         pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
         duo_mainloop(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
-        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, opaque_tid());
+        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, (int)threadIdx.x);
     }
 }
 
@@ -671,15 +668,17 @@ struct HeadPlan {
     bool backward, want_dx, want_dw, pack_w, pad_dw;
     bool direct;               // few tokens, forward: x as it is, ignored rows and all
     int64_t dp, vp;            // columns of the copies; classes of a piece
-    int pieces, bn, splits;
+    int pieces, splits;
+    bool few;                  // one tile of few tokens
+    int parts;                 // of a token's sum
     int64_t split_v;
     // offsets in the workspace
     int64_t xc, pos, count, lse2, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
 };
 // Tokens up to which a copy of the rows that count costs more than leaving some out gains: one tile of tokens either way.
-constexpr int64_t HD_FEW = 64;
+constexpr int64_t HD_FEW = HF_T;
 
-static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, bool backward, bool want_dx, bool want_dw, bool wide_x, bool pack_w)
+static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw, bool backward, bool want_dx, bool want_dw, bool wide_x, bool pack_w)
 {
     HeadPlan h = {};
     h.tokens = tokens;
@@ -695,14 +694,15 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.pack_w = !f32 && pack_w;
     h.pad_dw = !f32 && h.dp != dim;
     int64_t cols = (f32 ? 2 * HD_PIECE_BYTES : head_piece_bytes(tokens, dim)) / (es * tokens) / HD_TILE * HD_TILE;
-    if (f32) cols = std::min<int64_t>(cols, ((1ll << 29) - 1) / std::max<int64_t>(tokens, h.dp) / HD_TILE * HD_TILE);
-    else cols = std::min<int64_t>(cols, ((1ll << 28)) / h.dp / HD_TILE * HD_TILE);
+    // 32-bit offsets within a piece of the weight, and of dW
+    const int64_t far = std::max(h.dp, h.pack_w ? h.dp : ldw);
+    cols = std::min<int64_t>(cols, (f32 ? (1ll << 29) - 1 : 1ll << 28) / std::max(f32 ? tokens : 0, far) / HD_TILE * HD_TILE);
     cols = std::max<int64_t>(cols, HD_TILE);
     h.pieces = (int)cdiv(classes, cols);
     h.vp = cdiv(cdiv(classes, h.pieces), HD_TILE) * HD_TILE;
     if (f32 && h.pieces == 1) h.vp = classes;
     h.pieces = (int)cdiv(classes, h.vp);
-    h.bn = tokens <= HD_FEW ? 64 : HD_TOK;
+    h.few = tokens <= HD_FEW;
     const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, DUO_B);
     // Ranges of the classes, each with sums of dx of its own, until every block slot has a tile: at least 4 stages each, and 16 ranges or 16 MB of sums (24 tokens x 960 ->
     // 39040: 16 ranges of 38 stages 60 us, 64 of 10 35; 5 x 64 -> 1792: one of 28 24 us, 7 of 4 7).
@@ -729,7 +729,8 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
             h.picked = room(tokens * 4);
             h.g = room(tokens * h.vp * 4);
         } else {
-            h.part = room(2 * cdiv(classes, HD_TILE) * tokens * 8);
+            h.parts = h.few ? head_few_blocks(classes) : (int)(2 * cdiv(classes, HD_TILE));
+            h.part = room(h.parts * tokens * 8);
         }
     } else {
         if (!f32) {
@@ -812,24 +813,14 @@ static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
     return rc;
 }
 
-template <class K, class P> static int head_launch(K kernel, const P &p, int64_t items, size_t smem, hipStream_t s, const char *name)
+template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool few, hipStream_t s)
 {
-    if (int rl = reserve_lds(reinterpret_cast<const void *>(kernel), smem, name)) return rl;
-    int64_t blocks = std::max<int64_t>(8, num_compute_units() / 8 * 8);   // a multiple of 8: a block's tiles stay on one die's share of the list
-    blocks = std::min<int64_t>(blocks, (items + 7) / 8 * 8);
-    kernel<<<(unsigned)blocks, 256, smem, s>>>(p);
-    return check_launch(name);
-}
-template <int BN, bool GRAD> static int head_logits_on(const HeadLogits &p, hipStream_t s)
-{
-    return head_launch(head_logits_kernel<BN, GRAD>, p, (int64_t)p.tiles_v * p.tiles_t,
-                       big_smem<HD_TILE, BN, OperandTile<HD_TILE, 64, K_CONT>, OperandTile<BN, 64, K_CONT>>(), s, GRAD ? "head_logits_kernel<gradient>" : "head_logits_kernel");
-}
-template <bool GRAD> static int head_logits(HeadLogits &p, int bn, hipStream_t s)
-{
-    p.tiles_t = (int)cdiv(p.tokens, bn);
-    if (bn == 64) return head_logits_on<64, GRAD>(p, s);
-    head_logits_duo_kernel<GRAD><<<(unsigned)(((int64_t)p.tiles_v * p.tiles_t + 7) / 8 * 8), 256, 0, s>>>(p);
+    p.tiles_v = (int)cdiv(classes, few ? HF_V : HD_TILE);
+    if (few) {
+        head_logits_few_kernel<GRAD><<<(unsigned)(GRAD ? p.tiles_v : head_few_blocks(classes)), 256, 0, s>>>(p);
+        return check_launch(GRAD ? "head_logits_few_kernel<gradient>" : "head_logits_few_kernel");
+    }
+    head_logits_duo_kernel<GRAD><<<(unsigned)((p.tiles_v * cdiv(p.tokens, HD_TOK) + 7) / 8 * 8), 256, 0, s>>>(p);
     return check_launch(GRAD ? "head_logits_duo_kernel<gradient>" : "head_logits_duo_kernel");
 }
 
@@ -856,11 +847,10 @@ static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduc
     p.cleared = h.direct ? c.at<unsigned int>(h.count) + 1 : nullptr;
     p.dim = (int)h.dp;
     p.classes = (int)h.classes;
-    p.tiles_v = (int)cdiv(h.classes, HD_TILE);
     p.part = c.at<float2>(h.part);
     p.tokens = h.tokens;
-    if (int rc = head_logits<false>(p, h.bn, c.s)) return rc;
-    const HeadMerge m = {stats, p.part, h.direct ? nullptr : c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.classes, 2 * p.tiles_v, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
+    if (int rc = head_logits<false>(p, h.classes, h.few, c.s)) return rc;
+    const HeadMerge m = {stats, p.part, h.direct ? nullptr : c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.classes, h.parts, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
     // 16 lanes a token from as many tokens on as give every other compute unit a block of 64
     if (h.tokens >= 8192) head_merge_kernel<16><<<(unsigned)cdiv(h.tokens, 64), 1024, 0, c.s>>>(m);
     else head_merge_kernel<64><<<(unsigned)cdiv(h.tokens, 16), 1024, 0, c.s>>>(m);
@@ -897,7 +887,7 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         return p;
     };
     HeadLogits p = piece(0);
-    if (int rc = head_logits<true>(p, h.bn, c.s)) return rc;
+    if (int rc = head_logits<true>(p, std::min(h.vp, h.classes), h.few, c.s)) return rc;
     auto blocks_of = [](int64_t tiles) { return (int)((tiles + 7) / 8 * 8); };
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
@@ -1033,7 +1023,7 @@ using namespace rdb;
 static HeadPlan head_plan_of(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, bool backward, bool want_dx, bool want_dw)
 {
     const bool whole = dim % 8 == 0;
-    return head_plan(tokens, dim, classes, dtype, backward, want_dx, want_dw, whole && head_aligned(x, ldx, 2), !whole || !head_aligned(w, ldw, 2));
+    return head_plan(tokens, dim, classes, dtype, ldw, backward, want_dx, want_dw, whole && head_aligned(x, ldx, 2) && ldx < (1ll << 20), !whole || !head_aligned(w, ldw, 2));
 }
 
 extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,

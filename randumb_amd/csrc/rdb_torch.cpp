@@ -1121,11 +1121,14 @@ class CausalAttention : public Function<CausalAttention> {
 // loss of x (tokens, dim) against a weight (classes, dim) that never become logits; the argument checks are ops.linear_cross_entropy's
 class LinearCrossEntropy : public Function<LinearCrossEntropy> {
   public:
-    // unit inner stride, rows less than 2^20 values apart
-    static Tensor rows(const Tensor &t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) < (1 << 20) ? t : t.contiguous(); }
+    // unit inner stride, rows less than 2^20 values apart and (x) all of them less than 2^29
+    static Tensor rows(const Tensor &t, bool near = false)
+    {
+        return t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) < (1 << 20) && !(near && t.size(0) * t.stride(0) >= (1ll << 29)) ? t : t.contiguous();
+    }
     static Tensor forward(AutogradContext *ctx, const Tensor &x0, const Tensor &w0, const Tensor &target0, int64_t ignore, int64_t reduction)
     {
-        const Tensor x = rows(x0), w = rows(w0), target = target0.contiguous();
+        const Tensor x = rows(x0, true), w = rows(w0), target = target0.contiguous();
         const c10::OptionalDeviceGuard guard(x.device());
         const int64_t tokens = x.size(0), dim = x.size(1), classes = w.size(0);
         const auto f32 = x.options().dtype(at::kFloat);
@@ -1156,7 +1159,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const auto m = ctx->saved_data["m"].toIntVector();   // tokens, dim, classes, ignored label, reduction
         constexpr const char *who = "linear_cross_entropy (backward)";
         const Tensor dloss = grad.to(at::kFloat).contiguous();
-        const Tensor x = rows(restored(who, saved[0], dloss, {m[0], m[1]})), w = rows(restored(who, saved[1], dloss, {m[2], m[1]}));
+        const Tensor x = rows(restored(who, saved[0], dloss, {m[0], m[1]}), true), w = rows(restored(who, saved[1], dloss, {m[2], m[1]}));
         if (!readable(x.scalar_type()) || x.scalar_type() != w.scalar_type()) fail(PyExc_RuntimeError, std::string(who) + ": a saved tensor came back as something else");
         restored_values(who, saved[2], dloss, at::kLong, m[0]);
         restored_values(who, saved[3], dloss, at::kFloat, m[0] + 1);

@@ -62,6 +62,8 @@ class Rotary(nn.Module):
     frequencies are those of :func:`ops.rotary` and :func:`ops.rotary_frequencies`, on the GPU, the frequencies fp32 whatever the module's type:
     neighbouring pairs (``interleaved``), the first ``rotary_dim`` values of a head, ``scaling`` for longer contexts."""
 
+    stock = True   # also of a module that was stored before there was another
+
     def __init__(self, dim: int, base: float = 10000.0, *, interleaved: bool = False, rotary_dim: Optional[int] = None, **scaling):
         super().__init__()
         self.stock = not interleaved and rotary_dim is None and not scaling
@@ -131,13 +133,14 @@ class RT_CausalSelfAttention(nn.Module):
         B, T, D = x.shape
         qkv = self.c_qkv(x)
         ext = _fused(qkv)
-        if ext is not None and self.rotary.stock and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
+        stock = getattr(self.rotary, "stock", True)   # somebody's own rotation is called with one side at a time
+        if ext is not None and stock and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
             y = ext.causal_attention(qkv, self.rotary.inv_freq, self.n_head, _EPS)
             if y is not None:
                 return self.c_proj(y)
         q, k, v = qkv.view(B, T, 3, self.n_head, D // self.n_head).unbind(2)
         q, k = RT_norm(q), RT_norm(k)
-        q, k = (self.rotary(q), self.rotary(k)) if self.rotary.stock else self.rotary.both(q, k)
+        q, k = (self.rotary(q), self.rotary(k)) if stock else self.rotary.both(q, k)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
         return self.c_proj(y.transpose(1, 2).reshape(B, T, D))
 
@@ -253,6 +256,8 @@ def _embed(wte: nn.Module, idx: torch.Tensor) -> torch.Tensor:
 class RT_GPT(nn.Module):
     """Seeds are drawn qkv, proj, fc, mlp-proj per block, block after block."""
 
+    loss_without_logits = False
+
     def __init__(self, config: RT_GPTConfig):
         super().__init__()
         if config.random_embedding_and_head:
@@ -269,9 +274,9 @@ class RT_GPT(nn.Module):
             self.register_buffer("unit_coefs", torch.eye(self.lm_head.weight_coef.shape[1]), persistent=False)
 
     def _loss_without_logits(self, x: torch.Tensor, target: torch.Tensor) -> Optional[torch.Tensor]:
-        """The loss of the head's input; None where the head is more than its product, or not on the GPU."""
+        """The loss of the head's input; None where the head is more than its product, not on the GPU, or of more tokens than the operator takes."""
         head = self.lm_head
-        if not x.is_cuda or torch.is_autocast_enabled():
+        if not x.is_cuda or torch.is_autocast_enabled() or x.numel() >= 1 << 28 or target.numel() >= 1 << 21:
             return None
         if type(head) is nn.Linear and nn.Linear.forward is _DENSE_FORWARD:
             w = head._parameters.get("weight")

@@ -868,16 +868,17 @@ def set_big_tiles(mode: int) -> int:
 
 
 # ------------------------------------------------------------------------------------------------ ends of a language model
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A matrix as the head's kernels read it: unit inner stride, rows less than 2^20 values apart."""
-    return t if t.stride(1) == 1 and t.shape[1] <= t.stride(0) < 1 << 20 else t.contiguous()
+def _rows(t: torch.Tensor, near: bool = False) -> torch.Tensor:
+    """A matrix as the head's kernels read it: unit inner stride, rows less than 2^20 values apart and (``near``) all of them less than 2^29."""
+    fits = t.stride(1) == 1 and t.shape[1] <= t.stride(0) < 1 << 20 and not (near and t.shape[0] * t.stride(0) >= 1 << 29)
+    return t if fits else t.contiguous()
 
 
 def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int):
     """``(loss, stats)`` of the rows ``x`` (tokens, dim) and the weight (classes, dim), both fp32 or both bf16, for int64 targets; reduction 0: a loss
     for each row, 1: their mean, 2: their sum.  ``stats`` (fp32, tokens + 1) is what the backward call needs."""
     _need_gpu("linear_cross_entropy", x, weight, target)
-    x, w, t = _rows(x), _rows(weight), target.contiguous()
+    x, w, t = _rows(x, True), _rows(weight), target.contiguous()
     tokens, dim = x.shape
     dev, L = x.device, _lib.load()
     loss = torch.empty((tokens,) if reduction == 0 else (), dtype=torch.float32, device=dev)
@@ -897,7 +898,7 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
                              want_dx: bool = True, want_dw: bool = True):
     """``(dx, dweight)`` of :func:`linear_cross_entropy_fwd`, ``None`` where not wanted; ``dloss`` one value, or one for each row with reduction 0."""
     _need_gpu("linear_cross_entropy", dloss, stats, x, weight, target)
-    x, w, t, d, stats = _rows(x), _rows(weight), target.contiguous(), dloss.to(torch.float32).contiguous(), stats.contiguous()
+    x, w, t, d, stats = _rows(x, True), _rows(weight), target.contiguous(), dloss.to(torch.float32).contiguous(), stats.contiguous()
     tokens, dim = x.shape
     if d.numel() != (tokens if reduction == 0 else 1) or stats.dtype != torch.float32 or stats.numel() != tokens + 1:
         raise ValueError("linear_cross_entropy: a gradient or statistics of another size")
