@@ -150,9 +150,10 @@ template <typename E, bool INTERLEAVED, int N> __global__ __launch_bounds__(256)
 }
 
 // Whether rows may be taken n values at a time.
-static bool rt_pieces(const rdb_rotary_rows *x, int es, int n)
+static bool rt_pieces(const rdb_rotary_rows *x, int es, int n, int64_t batch, int64_t seq)
 {
-    return !(((uintptr_t)x->in | (uintptr_t)x->out) & (n * es - 1)) && x->stride_batch % n == 0 && x->stride_token % n == 0 && x->stride_head % n == 0;
+    auto whole = [&](int64_t count, int64_t stride) { return count == 1 || stride % n == 0; };
+    return !(((uintptr_t)x->in | (uintptr_t)x->out) & (n * es - 1)) && whole(batch, x->stride_batch) && whole(seq, x->stride_token) && whole(x->heads, x->stride_head);
 }
 template <typename E, bool INTERLEAVED, int N> static int launch_rotary(const RotaryParams &p, int64_t blocks, hipStream_t s)
 {
@@ -211,7 +212,7 @@ extern "C" int rdb_rotary(const rdb_rotary_rows *q, const rdb_rotary_rows *k, in
     const int64_t blocks = batch * p.blocks_per_seq;
     if (blocks >= (1ll << 31)) return set_error(RDB_E_UNSUPPORTED, "rdb_rotary: too many sequences");
     int n = 16 / es;   // values a lane takes at once
-    while (n > 1 && !(rt_pieces(q, es, n) && (!k || rt_pieces(k, es, n)) && head_dim % n == 0 && (interleaved ? 2 * pairs : pairs) % n == 0)) n /= 2;
+    while (n > 1 && !(rt_pieces(q, es, n, batch, seq) && (!k || rt_pieces(k, es, n, batch, seq)) && head_dim % n == 0 && (interleaved ? 2 * pairs : pairs) % n == 0)) n /= 2;
     const int64_t paired = interleaved && n > 1 ? 2 * pairs / n : pairs / n;
     p.units = rt_divide(paired + (head_dim - 2 * pairs) / n);
     const auto stream_ = (hipStream_t)stream;

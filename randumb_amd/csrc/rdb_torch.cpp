@@ -1121,10 +1121,12 @@ class CausalAttention : public Function<CausalAttention> {
 // loss of x (tokens, dim) against a weight (classes, dim) that never become logits; the argument checks are ops.linear_cross_entropy's
 class LinearCrossEntropy : public Function<LinearCrossEntropy> {
   public:
+    // how far apart rows lie; of a single one, whose stride may be anything, its length
+    static int64_t ld(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
     // unit inner stride, rows less than 2^20 values apart and (x) all of them less than 2^29
     static Tensor rows(const Tensor &t, bool near = false)
     {
-        return t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) < (1 << 20) && !(near && t.size(0) * t.stride(0) >= (1ll << 29)) ? t : t.contiguous();
+        return t.stride(1) == 1 && ld(t) >= t.size(1) && ld(t) < (1 << 20) && !(near && t.size(0) * ld(t) >= (1ll << 29)) ? t : t.contiguous();
     }
     static Tensor forward(AutogradContext *ctx, const Tensor &x0, const Tensor &w0, const Tensor &target0, int64_t ignore, int64_t reduction)
     {
@@ -1134,9 +1136,9 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const auto f32 = x.options().dtype(at::kFloat);
         Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32);
         if (tokens) {
-            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), 0, 0, 0);
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), 0, 0, 0);
             const Tensor ws = bytes(need, x);
-            check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), code(x.scalar_type()),
+            check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), ld(x), w.data_ptr(), ld(w), code(x.scalar_type()),
                                                target.data_ptr<int64_t>(), tokens, dim, classes, ignore, (int)reduction, ptr(ws), need, stream_of(x)),
                   "rdb_linear_cross_entropy_fwd");
         } else {
@@ -1169,9 +1171,9 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         if (want_x) dx = at::empty({m[0], m[1]}, x.options());
         if (want_w) dw = m[0] ? at::empty({m[2], m[1]}, w.options()) : at::zeros({m[2], m[1]}, w.options());
         if (m[0] && (want_x || want_w)) {
-            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), 1, want_x, want_w);
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), 1, want_x, want_w);
             const Tensor ws = bytes(need, x);
-            check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+            check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), x.data_ptr(), ld(x), w.data_ptr(), ld(w),
                                                code(x.scalar_type()), saved[2].data_ptr<int64_t>(), m[0], m[1], m[2], m[3], (int)m[4], ptr(ws), need, stream_of(x)),
                   "rdb_linear_cross_entropy_bwd");
         }

@@ -868,9 +868,14 @@ def set_big_tiles(mode: int) -> int:
 
 
 # ------------------------------------------------------------------------------------------------ ends of a language model
+def _ld(t: torch.Tensor) -> int:
+    """How far apart a matrix's rows lie; of a single one, whose stride may be anything, its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _rows(t: torch.Tensor, near: bool = False) -> torch.Tensor:
     """A matrix as the head's kernels read it: unit inner stride, rows less than 2^20 values apart and (``near``) all of them less than 2^29."""
-    fits = t.stride(1) == 1 and t.shape[1] <= t.stride(0) < 1 << 20 and not (near and t.shape[0] * t.stride(0) >= 1 << 29)
+    fits = t.stride(1) == 1 and t.shape[1] <= _ld(t) < 1 << 20 and not (near and t.shape[0] * _ld(t) >= 1 << 29)
     return t if fits else t.contiguous()
 
 
@@ -886,9 +891,9 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
     if tokens == 0:
         return loss.fill_(float("nan") if reduction == 1 else 0.0), stats.zero_()
     with _on(dev):
-        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), x.stride(0), _p(w), w.stride(0), 0, 0, 0))
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), _ld(x), _p(w), _ld(w), 0, 0, 0))
         ws = _workspace(n, dev)
-        rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
+        rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
                                             _p(ws), n, _stream(dev))
     _lib.check(rc, "rdb_linear_cross_entropy_fwd")
     return loss, stats
@@ -908,9 +913,9 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
     if tokens == 0:
         return dx, None if dw is None else dw.zero_()
     with _on(dev):
-        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), x.stride(0), _p(w), w.stride(0), 1, want_dx, want_dw))
+        n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), _ld(x), _p(w), _ld(w), 1, want_dx, want_dw))
         ws = _workspace(n, dev)
-        rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), _p(x), x.stride(0), _p(w), w.stride(0), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
+        rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
                                             ignore_index, reduction, _p(ws), n, _stream(dev))
     _lib.check(rc, "rdb_linear_cross_entropy_bwd")
     return dx, dw

@@ -176,6 +176,11 @@ def test_strides_shapes_and_types_of_the_targets(dtype):
     ones = both(x, w, t, "none", torch.ones(1, device="cuda").expand(tokens))
     for p, q in zip(ones, both(x, w, t, "none", torch.ones(tokens, device="cuda"))):
         assert torch.equal(p, q)
+    # a single row, and a single class, with a stride of its own
+    for a, b in ((x[:1].T.contiguous().T, w), (x[3:4].expand(1, dim), w), (x[:1], w[:1].T.contiguous().T), (x[0].as_strided((1, dim), (0, 1)), w[5].as_strided((1, dim), (1, 1)))):
+        one = t[:1].clamp(0, b.shape[0] - 1)
+        for p, q in zip(both(a.contiguous().clone(), b.contiguous().clone(), one, "mean"), both(a, b, one, "mean")):
+            assert torch.equal(p, q)
     # no tokens
     empty = both(x[:0], w, t[:0], "mean")
     assert bool(empty[0].isnan()) and empty[2].shape == (0, dim) and not bool(empty[3].any())
@@ -271,3 +276,23 @@ def test_the_stock_operators_say_the_same():
     assert float((loss - want.detach()).abs()) < 1e-5
     for p, q in zip((dx, dw), torch.autograd.grad(want, [a, b], dloss)):
         assert float((p - q).norm() / q.norm()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_lie_far_apart(dtype):
+    """Offsets past 32 bits: a weight whose rows are 2^19 values apart (three pieces of it are more than 2^31 bytes), hidden states 2^18 apart."""
+    tokens, dim, classes = 40, 64, 2100
+    x, w, t = inputs(tokens, dim, classes, dtype, 15, 0.1)
+    wide = torch.zeros(classes, 1 << 19, dtype=dtype, device="cuda")
+    wide[:, 8:8 + dim] = w
+    far = torch.zeros(tokens, 1 << 18, dtype=dtype, device="cuda")
+    far[:, 16:16 + dim] = x
+    for p, q in zip(both(x, w, t, "mean"), both(far[:, 16:16 + dim], wide[:, 8:8 + dim], t, "mean")):
+        assert float((p.float() - q.float()).norm()) <= 2 * torch.finfo(dtype).eps * float(q.float().norm())   # dx in other ranges of the classes
+    del wide
+    tokens = 5000   # and enough tokens to be gathered
+    x, w, t = inputs(tokens, dim, classes, dtype, 16, 0.1)
+    far = torch.zeros(tokens, 1 << 19, dtype=dtype, device="cuda")
+    far[:, :dim] = x
+    for p, q in zip(both(x, w, t, "mean"), both(far[:, :dim], w, t, "mean")):
+        assert torch.equal(p, q)
