@@ -250,13 +250,15 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *_
     }
 }
 
-// Few tokens, one tile of them: bound by the weight, which is read once.  Tiles of 64 classes, so that many blocks have loads on their way, four stages of 64 x 64 each
-// ahead; statistics by up to two blocks a compute unit, each with several tiles in turn and one part for all of them: parts are what the merging kernel's time goes by.
-// us a forward call, 256 x 64 tiles of rdb_big.hpp -> so: 64 tokens x 4096 -> 16384 57 -> 32, 32 x 1000 -> 100000 58.6 -> 56.9, 16 x 768 -> 50304 22.7 -> 23.8
-// (77 MB of weight: 15 at the rate of a large copy); 256 x 128 on two blocks a compute unit 75, 60.5, 26.1.
-constexpr int HF_V = 64, HF_T = 64, HF_AHEAD = 4;
-template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_few_kernel(HeadLogits p)
+// Few tokens, one tile of them: bound by the weight, which is read once.  Tiles of 64 classes with four stages of 64 on their way, of 128 with two where these give every
+// compute unit a block; statistics by up to two blocks a compute unit, each with several tiles in turn and one part for all of them: parts are what the merging
+// kernel's time goes by.  us a forward call, 256 x 64 tiles of rdb_big.hpp | 64 x 64 | 128 x 64 (four stages: 23.5, 32.1, 59.6): 16 tokens x 768 -> 50304 22.7 | 23.8 | 22.3,
+// 64 x 4096 -> 16384 57 | 32.1 | 33.1, 32 x 1000 -> 100000 58.6 | 57.0 | 57.2 (77, 134 and 200 MB of weight: 15, 26 and 39 at the rate of a large copy);
+// 256 x 128 on two blocks a compute unit 26.1, 75, 60.5.
+constexpr int HF_T = 64;
+template <bool GRAD, int HF_V> __global__ __launch_bounds__(256, 2) void head_logits_few_kernel(HeadLogits p)
 {
+    constexpr int MI = HF_V / 64, AHEAD = 4 / MI;
     typedef GlobalOperand<HF_V, 64, K_CONT> PA;
     typedef GlobalOperand<HF_T, 64, K_CONT> PB;
     __shared__ __align__(16) bf16_t lds[2 * (PA::Tile::LDS_ELEMS + PB::Tile::LDS_ELEMS)];
@@ -270,14 +272,16 @@ template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_few_k
         const int row = p.v0 + tv * HF_V, rows = min(HF_V, p.classes - row);
         PA pa = {p.w + (int64_t)row * p.ldw, p.ldw, 0, rows, p.dim, (int64_t)(rows - 1) * p.ldw + p.dim};
         PB pb = {p.x, p.ldx, 0, count, p.dim, (int64_t)(count - 1) * p.ldx + p.dim};
-        f32x16 acc[1][1] = {{zero16()}};
-        gemm_mainloop<HF_V, HF_T, 64, HF_AHEAD, HF_AHEAD>(acc, lds, pa, pb, 0, (p.dim + 63) / 64);
+        f32x16 acc[MI][1];
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) acc[mi][0] = zero16();
+        gemm_mainloop<HF_V, HF_T, 64, AHEAD, AHEAD>(acc, lds, pa, pb, 0, (p.dim + 63) / 64);
         if constexpr (GRAD) {
-            head_leave_grad<1, 1>(acc, lds, p, tv, 0, count, t);
+            head_leave_grad<MI, 1>(acc, lds, p, tv, 0, count, t);
             __syncthreads();
         } else {
             float m2, s2;
-            head_stats(acc, 0, p.classes - (row + wm * 32), g, m2, s2);
+            head_stats(acc, 0, p.classes - (row + wm * MI * 32), g, m2, s2);
             head_join(m, s, m2, s2);
         }
     }
@@ -293,7 +297,8 @@ template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_few_k
         }
     }
 }
-static int head_few_blocks(int64_t classes) { return (int)std::min<int64_t>(cdiv(classes, HF_V), 2 * num_compute_units()); }
+static int head_few_tile(int64_t classes) { return cdiv(classes, 128) >= num_compute_units() ? 128 : 64; }
+static int head_few_blocks(int64_t classes) { return (int)std::min<int64_t>(cdiv(classes, head_few_tile(classes)), 2 * num_compute_units()); }
 
 // The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
 template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
@@ -819,9 +824,11 @@ static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
 
 template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool few, hipStream_t s)
 {
-    p.tiles_v = (int)cdiv(classes, few ? HF_V : HD_TILE);
+    p.tiles_v = (int)cdiv(classes, few ? head_few_tile(classes) : HD_TILE);
     if (few) {
-        head_logits_few_kernel<GRAD><<<(unsigned)(GRAD ? p.tiles_v : head_few_blocks(classes)), 256, 0, s>>>(p);
+        const unsigned blocks = (unsigned)(GRAD ? p.tiles_v : head_few_blocks(classes));
+        if (head_few_tile(classes) == 128) head_logits_few_kernel<GRAD, 128><<<blocks, 256, 0, s>>>(p);
+        else head_logits_few_kernel<GRAD, 64><<<blocks, 256, 0, s>>>(p);
         return check_launch(GRAD ? "head_logits_few_kernel<gradient>" : "head_logits_few_kernel");
     }
     head_logits_duo_kernel<GRAD><<<(unsigned)((p.tiles_v * cdiv(p.tokens, HD_TOK) + 7) / 8 * 8), 256, 0, s>>>(p);

@@ -2,8 +2,8 @@
 // pair i at position p becomes (a cos + b sin, b cos - a sin) with the angle p * inv_freq[i] and both factors times `scale`; the
 // pairs are values i and P + i, or (interleaved) 2 i and 2 i + 1.  The other values are copied.  The gradient is the same with the sine's sign turned.
 //
-// Bound by memory: every value is read once and written once, queries and keys in one launch.  A block takes a few tokens of one sequence: cosines and
-// sines once a token, into LDS, then 16 bytes a lane and step over all heads.  The angle is formed and reduced to an eighth of
+// Bound by memory: every value is read once and written once, queries and keys in one launch (32768 tokens x 40 heads of 128, bf16: 5.4 TB/s; a large copy: 5.1).  A block takes
+// one or a few tokens of one sequence: cosines and sines once a token, into LDS, then 16 bytes a lane and step over all heads.  The angle is formed and reduced to an eighth of
 // a turn in 64 bits: at position 10^6 an angle in 32 bits is off by 0.03.
 #include "rdb_common.hpp"
 #include <algorithm>
@@ -13,6 +13,8 @@ namespace rdb {
 int num_compute_units();
 
 constexpr int RT_TOKENS = 8;       // at most, of a block
+constexpr int RT_PIECES = 192;     // of a block's tokens, about
+constexpr int64_t RT_CACHE_BYTES = 256ll << 20;
 constexpr int RT_PAIRS = 1024;     // pairs of cosine and sine of a block at most
 
 // n / d for n < 2^31: (n + (n m >> 32)) >> l with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1
@@ -42,12 +44,19 @@ struct RotaryParams {
     int64_t pb, pt;       // strides of positions
     int pos_bytes;        // 0: a token's index is its position
     int seq, dim, pairs, tokens, blocks_per_seq;
+    bool stream;
     float scale, sign;
 };
 
 // N values at once
 template <int N> __device__ __forceinline__ void rt_load(float (&v)[N], const float *p) { __builtin_memcpy(v, __builtin_assume_aligned(p, N * 4), N * 4); }
-template <int N> __device__ __forceinline__ void rt_store(float *p, const float (&v)[N]) { __builtin_memcpy(__builtin_assume_aligned(p, N * 4), v, N * 4); }
+// stream: past the caches (whole pieces of 16 bytes)
+template <int N> __device__ __forceinline__ void rt_store(float *p, const float (&v)[N], bool stream)
+{
+    if constexpr (N == 4)
+        if (stream) return store_stream(reinterpret_cast<f32x4 *>(p), f32x4{v[0], v[1], v[2], v[3]});
+    __builtin_memcpy(__builtin_assume_aligned(p, N * 4), v, N * 4);
+}
 template <int N> __device__ __forceinline__ void rt_load(float (&v)[N], const bf16_t *p)
 {
     if constexpr (N == 1) {
@@ -62,7 +71,7 @@ template <int N> __device__ __forceinline__ void rt_load(float (&v)[N], const bf
         }
     }
 }
-template <int N> __device__ __forceinline__ void rt_store(bf16_t *p, const float (&v)[N])
+template <int N> __device__ __forceinline__ void rt_store(bf16_t *p, const float (&v)[N], bool stream)
 {
     if constexpr (N == 1) {
         *p = f32_to_bf16(v[0]);
@@ -70,6 +79,8 @@ template <int N> __device__ __forceinline__ void rt_store(bf16_t *p, const float
         uint32_t w[N / 2];
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) w[e] = f32x2_to_bf16x2(v[2 * e], v[2 * e + 1]);
+        if constexpr (N == 8)
+            if (stream) return store_stream(reinterpret_cast<u32x4 *>(p), u32x4{w[0], w[1], w[2], w[3]});
         __builtin_memcpy(__builtin_assume_aligned(p, N * 2), w, N * 2);
     }
 }
@@ -105,7 +116,7 @@ __device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows 
             const int c = 2 * p.pairs + (int)(u - paired) * N;
             float a[N];
             rt_load(a, src + c);
-            rt_store(dst + c, a);
+            rt_store(dst + c, a, p.stream);
             continue;
         }
         const float2 *w = cs + t * p.pairs + u * P;
@@ -118,7 +129,7 @@ __device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows 
                 a[2 * e] = v * w[e].x + a[2 * e + 1] * w[e].y;
                 a[2 * e + 1] = a[2 * e + 1] * w[e].x - v * w[e].y;
             }
-            rt_store(dst + u * N, a);
+            rt_store(dst + u * N, a, p.stream);
         } else {
             const int ia = INTERLEAVED ? 2 * (int)u : (int)u * N, ib = INTERLEAVED ? ia + 1 : p.pairs + ia;
             float a[N], c[N];
@@ -130,8 +141,8 @@ __device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows 
                 a[e] = v * w[e].x + c[e] * w[e].y;
                 c[e] = c[e] * w[e].x - v * w[e].y;
             }
-            rt_store(dst + ia, a);
-            rt_store(dst + ib, c);
+            rt_store(dst + ia, a, p.stream);
+            rt_store(dst + ib, c, p.stream);
         }
     }
 }
@@ -204,17 +215,21 @@ extern "C" int rdb_rotary(const rdb_rotary_rows *q, const rdb_rotary_rows *k, in
     p.pairs = (int)pairs;
     p.scale = scale;
     p.sign = inverse ? -1.0f : 1.0f;
-    // tokens of a block: as many as leave the chip 8 blocks a compute unit
-    int64_t tokens = std::min<int64_t>(RT_TOKENS, batch * seq / (8 * num_compute_units()));
-    if (pairs) tokens = std::min<int64_t>(tokens, RT_PAIRS / pairs);
-    p.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(tokens, seq));
-    p.blocks_per_seq = (int)cdiv(seq, p.tokens);
-    const int64_t blocks = batch * p.blocks_per_seq;
-    if (blocks >= (1ll << 31)) return set_error(RDB_E_UNSUPPORTED, "rdb_rotary: too many sequences");
     int n = 16 / es;   // values a lane takes at once
     while (n > 1 && !(rt_pieces(q, es, n, batch, seq) && (!k || rt_pieces(k, es, n, batch, seq)) && head_dim % n == 0 && (interleaved ? 2 * pairs : pairs) % n == 0)) n /= 2;
     const int64_t paired = interleaved && n > 1 ? 2 * pairs / n : pairs / n;
     p.units = rt_divide(paired + (head_dim - 2 * pairs) / n);
+    // A token a block, or as many as give its lanes a piece each or nearly so: what is read and written at a time stays close together.  us with 8 tokens, 2, 1: 32768 tokens x
+    // 40 heads of 128 (640 pieces a token) 148, 136, 133; 16384 x 32 x 80, fp32 (640) 67.5, 65.6, 60.4; 8192 x 24 x 64 (96) 10.9 (4 tokens), 10.8, 12.2.
+    const int64_t pieces = (q->heads + (k ? k->heads : 0)) * (int64_t)p.units.d;
+    int64_t tokens = std::min<int64_t>(RT_TOKENS, std::max<int64_t>(1, RT_PIECES / pieces));
+    if (pairs) tokens = std::min<int64_t>(tokens, RT_PAIRS / pairs);
+    p.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(tokens, seq));
+    // What the last-level cache does not hold goes past it (the first of these 133 -> 123 us); what it holds is for the next launch to find there.
+    p.stream = batch * seq * (q->heads + (k ? k->heads : 0)) * head_dim * es > RT_CACHE_BYTES;
+    p.blocks_per_seq = (int)cdiv(seq, p.tokens);
+    const int64_t blocks = batch * p.blocks_per_seq;
+    if (blocks >= (1ll << 31)) return set_error(RDB_E_UNSUPPORTED, "rdb_rotary: too many sequences");
     const auto stream_ = (hipStream_t)stream;
     if (dtype == RDB_BF16) return interleaved ? launch_rotary<bf16_t, true>(p, blocks, n, stream_) : launch_rotary<bf16_t, false>(p, blocks, n, stream_);
     return interleaved ? launch_rotary<float, true>(p, blocks, n, stream_) : launch_rotary<float, false>(p, blocks, n, stream_);

@@ -143,3 +143,17 @@ def test_streams_and_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+@pytest.mark.parametrize("heads", [40, 256])
+def test_large_ones(heads):
+    """More than the chip's last-level cache holds, and more than 2^31 values: the first, the middle and the last positions."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.empty(2, 35000, heads, 128, device="cuda", dtype=torch.bfloat16).uniform_(-1, 1, generator=g)
+    freq, _ = ops.rotary_frequencies(128, device="cuda")
+    for interleaved in (False, True):
+        out = ops.rotary(q, None, freq, interleaved=interleaved)[0]
+        for at in (slice(0, 40), slice(17000, 17040), slice(34960, 35000)):
+            pos = torch.arange(35000, device="cuda")[at].expand(2, 40)
+            close(out[:, at], q[:, at], turned(q[:, at], freq, pos, interleaved, 1.0), freq, interleaved, 1.0)
+        del out
