@@ -1027,6 +1027,8 @@ static int check_head(const char *who, int64_t tokens, int64_t dim, int64_t clas
     // 32-bit offsets within an operand: x in rows of a multiple of 8 values, a tile of W's rows, a piece of G
     if ((dim + 7) / 8 * 8 * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29) || tokens >= (1ll << 21) || ldw >= (1ll << 20))
         return set_error(RDB_E_UNSUPPORTED, "%s: x of less than 2^29 values and 2^21 rows, rows of w less than 2^20 apart", who);
+    if (dtype == RDB_BF16 && cdiv(classes, HD_TILE) * cdiv(tokens, HD_TOK) >= (1ll << 23))   // a launch has less than 2^32 threads
+        return set_error(RDB_E_UNSUPPORTED, "%s: less than 2^38 logits in bf16", who);
     return RDB_OK;
 }
 

@@ -44,6 +44,7 @@ struct RotaryParams {
     int64_t pb, pt;       // strides of positions
     int pos_bytes;        // 0: a token's index is its position
     int seq, dim, pairs, tokens, blocks_per_seq;
+    int first;            // block of this launch
     bool stream;
     float scale, sign;
 };
@@ -149,8 +150,9 @@ __device__ __forceinline__ void rt_rows(const RotaryParams &p, const RotaryRows 
 template <typename E, bool INTERLEAVED, int N> __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p)
 {
     __shared__ float2 cs[RT_PAIRS];
-    const int64_t b = blockIdx.x / p.blocks_per_seq;
-    const int t0 = (int)(blockIdx.x - b * p.blocks_per_seq) * p.tokens, nt = min(p.tokens, p.seq - t0);
+    const int block = p.first + (int)blockIdx.x;
+    const int64_t b = block / p.blocks_per_seq;
+    const int t0 = (int)(block - b * p.blocks_per_seq) * p.tokens, nt = min(p.tokens, p.seq - t0);
     for (int i = threadIdx.x; i < nt * p.pairs; i += 256) {
         const int t = i / p.pairs;
         cs[i] = rt_turn(p, b, t0 + t, i - t * p.pairs);
@@ -166,10 +168,15 @@ static bool rt_pieces(const rdb_rotary_rows *x, int es, int n, int64_t batch, in
     auto whole = [&](int64_t count, int64_t stride) { return count == 1 || stride % n == 0; };
     return !(((uintptr_t)x->in | (uintptr_t)x->out) & (n * es - 1)) && whole(batch, x->stride_batch) && whole(seq, x->stride_token) && whole(x->heads, x->stride_head);
 }
-template <typename E, bool INTERLEAVED, int N> static int launch_rotary(const RotaryParams &p, int64_t blocks, hipStream_t s)
+// A launch has less than 2^32 threads.
+template <typename E, bool INTERLEAVED, int N> static int launch_rotary(RotaryParams p, int64_t blocks, hipStream_t s)
 {
-    rotary_kernel<E, INTERLEAVED, N><<<(unsigned)blocks, 256, 0, s>>>(p);
-    return check_launch("rotary_kernel");
+    for (int64_t first = 0; first < blocks; first += 1 << 23) {
+        p.first = (int)first;
+        rotary_kernel<E, INTERLEAVED, N><<<(unsigned)std::min<int64_t>(blocks - first, 1 << 23), 256, 0, s>>>(p);
+        if (int rc = check_launch("rotary_kernel")) return rc;
+    }
+    return RDB_OK;
 }
 template <typename E, bool INTERLEAVED> static int launch_rotary(const RotaryParams &p, int64_t blocks, int n, hipStream_t s)
 {

@@ -276,7 +276,7 @@ class RT_GPT(nn.Module):
     def _loss_without_logits(self, x: torch.Tensor, target: torch.Tensor) -> Optional[torch.Tensor]:
         """The loss of the head's input; None where the head is more than its product, not on the GPU, or of more tokens than the operator takes."""
         head = self.lm_head
-        if not x.is_cuda or torch.is_autocast_enabled() or x.numel() >= 1 << 28 or target.numel() >= 1 << 21:
+        if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float32) or torch.is_autocast_enabled() or x.numel() >= 1 << 28 or target.numel() >= 1 << 21:
             return None
         if type(head) is nn.Linear and nn.Linear.forward is _DENSE_FORWARD:
             w = head._parameters.get("weight")

@@ -120,3 +120,13 @@ def test_the_library_refuses():
                                             scale=1.0, inverse=0, stream=None), **k}.values())
     assert rot(dtype=3) == -3 and rot(q=None) == -1 and rot(freq=None) == -1 and rot(pairs=9) == -2 and rot(dim=0) == -2 and rot(pos=one, pos_bytes=2) == -3
     assert rot(dim=4096, pairs=1025) == -5 and rot(batch=0) == 0 and rot(q=rows(0)) == 0
+
+
+def test_more_logits_than_a_launch_has_threads_are_refused():
+    """2^21 - 1 tokens of 8 values and 2^30 classes: by memory they would fit; the number of tiles is past 2^32."""
+    L = _lib.load()
+    sizes = ((1 << 21) - 1, 8, 1 << 30)
+    for tokens, dim, classes in (sizes, (1 << 20, 8, 1 << 18)):
+        assert L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, _lib.RDB_BF16, 4096, 8, 4096, 8, 0, 0, 0) == 0
+        assert L.rdb_linear_cross_entropy_fwd(4096, 4096, 4096, 8, 4096, 8, _lib.RDB_BF16, 4096, tokens, dim, classes, -100, 1, 4096, 1 << 62, None) == -5
+    assert L.rdb_linear_cross_entropy_workspace_bytes((1 << 20) - 128, 8, 1 << 18, _lib.RDB_BF16, 4096, 8, 4096, 8, 0, 0, 0) > 0

@@ -157,3 +157,14 @@ def test_large_ones(heads):
             pos = torch.arange(35000, device="cuda")[at].expand(2, 40)
             close(out[:, at], q[:, at], turned(q[:, at], freq, pos, interleaved, 1.0), freq, interleaved, 1.0)
         del out
+
+
+def test_more_blocks_than_one_launch():
+    """2^24 + 5 sequences of one token, a block each: the first, the last, and those around the ends of a launch."""
+    n = (1 << 24) + 5
+    q = torch.arange(n, device="cuda", dtype=torch.int32).remainder(251).sub(125).div(125).to(torch.bfloat16).view(n, 1, 1, 1).expand(n, 1, 1, 4).contiguous()
+    pos = torch.arange(n, device="cuda", dtype=torch.int32).view(n, 1)
+    freq, _ = ops.rotary_frequencies(4, device="cuda")
+    out = ops.rotary(q, None, freq, pos)[0]
+    for at in (slice(0, 40), slice((1 << 23) - 20, (1 << 23) + 20), slice((1 << 24) - 20, (1 << 24) + 5)):
+        close(out[at], q[at], turned(q[at], freq, pos[at], False, 1.0), freq, False, 1.0)
