@@ -85,8 +85,8 @@ __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
         }
     }
     __syncthreads();
-    // 8 values a lane, at any address; a ragged piece of the last row that there is one by one: 16 bytes would reach behind it
-    const int chunks = (int)(p.ldc / 8), dim = (int)p.dim, total = mine * chunks, whole = dim % 8 && r0 + mine == p.tokens ? total - 1 : total;
+    // 8 values a lane, at any address; a ragged piece of the last row that there is, and rows of less than 8 values, one by one: 16 bytes would reach behind the last of them
+    const int chunks = (int)(p.ldc / 8), dim = (int)p.dim, total = mine * chunks, whole = dim < 8 ? 0 : dim % 8 && r0 + mine == p.tokens ? total - 1 : total;
     for (int i0 = t; i0 < whole; i0 += 1024) {
         u32x4 v[4];
         bf16_t *to[4];
@@ -102,9 +102,9 @@ __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
         for (int q = 0; q < 4; ++q)
             if (to[q]) *reinterpret_cast<u32x4 *>(to[q]) = v[q];
     }
-    if (whole < total && t < 8 && place_[mine - 1] >= 0) {
-        const int col = (chunks - 1) * 8 + t;
-        p.xc[(int64_t)place_[mine - 1] * p.ldc + col] = col < dim ? p.x[(p.tokens - 1) * p.ldx + col] : (bf16_t)0;
+    for (int i = whole * 8 + t; i < total * 8; i += 256) {
+        const int row = i / 8 / chunks, col = i - row * chunks * 8, at = place_[row];
+        if (at >= 0) p.xc[(int64_t)at * p.ldc + col] = col < dim ? p.x[(r0 + row) * p.ldx + col] : (bf16_t)0;
     }
 }
 
