@@ -51,11 +51,11 @@ struct HeadGather {
     int rows;                // per block
 };
 // Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.
-__global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
+__device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
 {
     __shared__ int before_[4], place_[64];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int64_t r0 = (int64_t)blockIdx.x * p.rows;
+    const int64_t r0 = (int64_t)block * p.rows;
     const int mine = p.tokens - r0 < p.rows ? (int)(p.tokens - r0) : p.rows;
     const int64_t c = wave == 0 && lane < mine ? p.target[r0 + lane] : p.ignore;
     int n = 0;
@@ -110,14 +110,22 @@ __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p)
 
 // Rows of `cols` bf16 values into rows of a multiple of 8 of them (PAD, zeros behind the last ones) or out of them into rows without gaps; a lane reads 8 values at any address
 // and writes them to a multiple of 16 bytes.  per_block: a multiple of 8, at most 8192 values; out of padded rows it reads up to 14 bytes behind the last of them.
-template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf16_t *__restrict__ dst, const bf16_t *__restrict__ src, int64_t lds, int64_t rows, int cols, int per_block)
+struct HeadRepack {
+    bf16_t *dst;
+    const bf16_t *src;
+    int64_t ld, rows;   // of src
+    int cols, per_block, blocks;
+};
+template <bool PAD> __device__ __forceinline__ void head_repack_rows(const HeadRepack &p, int block)
 {
-    const int64_t r0 = (int64_t)blockIdx.x * per_block;
-    const int mine = rows - r0 < per_block ? (int)(rows - r0) : per_block, out_cols = PAD ? (cols + 7) & ~7 : cols, total = mine * out_cols;
+    const int64_t r0 = (int64_t)block * p.per_block, lds = p.ld;
+    const bf16_t *__restrict__ src = p.src;
+    bf16_t *__restrict__ dst = p.dst;
+    const int cols = p.cols, mine = p.rows - r0 < p.per_block ? (int)(p.rows - r0) : p.per_block, out_cols = PAD ? (cols + 7) & ~7 : cols, total = mine * out_cols;
     src += r0 * lds;
     dst += r0 * out_cols;
     // whole pieces, but for those that would read behind the last row that there is
-    const int whole = cols < 8 ? 0 : PAD && r0 + mine == rows ? total - out_cols : total & ~7;
+    const int whole = cols < 8 ? 0 : PAD && r0 + mine == p.rows ? total - out_cols : total & ~7;
     for (int i0 = threadIdx.x * 8; i0 < whole; i0 += 4 * 2048) {
         u32x4 v[4], u[4];
         int left[4];
@@ -145,6 +153,12 @@ template <bool PAD> __global__ __launch_bounds__(256) void head_repack_kernel(bf
         const int row = i / out_cols, c = i - row * out_cols;
         dst[i] = c < cols ? src[(int64_t)row * lds + c] : (bf16_t)0;
     }
+}
+// The rows that count and, where it needs one, the weight's copy, in one launch (three launches less with dW's, 1025 x 999 -> 10001: a step 136 -> 126.5 us).
+__global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p, HeadRepack w, int gathering)
+{
+    if ((int)blockIdx.x < gathering) head_gather_rows(p, (int)blockIdx.x);
+    else head_repack_rows<true>(w, (int)blockIdx.x - gathering);
 }
 
 // ----------------------------------------------------------------------------------------------- logits, in the accumulators
@@ -541,15 +555,17 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
     }
 }
 
-// dx[row] = factor * the sums of its place over the splits, rounded once; zeros in ignored rows
+// dx[row] = factor * the sums of its place over the splits, rounded once; zeros in ignored rows.  The blocks behind those bring dW into rows without gaps.
 __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, const float *__restrict__ sums, const int *__restrict__ pos, int64_t tokens, int dim,
-                                                      int64_t ld, int64_t stride, int splits, HeadScale scale)
+                                                      int64_t ld, int64_t stride, int splits, HeadScale scale, HeadRepack dw)
 {
+    const int summing = (int)gridDim.x - dw.blocks;
+    if ((int)blockIdx.x >= summing) return head_repack_rows<false>(dw, (int)blockIdx.x - summing);
     const float f = scale.value();
     const int chunks = (int)(ld / 4);
     const int64_t n = tokens * chunks;
     const bool whole = dim % 4 == 0;   // rows of dx begin on 8 bytes then
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)summing * 256) {
         const int64_t row = i / chunks;
         const int c = (int)(i - row * chunks) * 4, at = pos[row];
         f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -777,49 +793,50 @@ struct HeadCall {
 };
 static bool head_aligned(const void *p, int64_t ld, int es) { return !((uintptr_t)p & 15) && ld * es % 16 == 0; }
 
-static int head_gather(const HeadCall &c, const float *stats, const float *dloss_rows)
+static HeadRepack head_repack(bf16_t *dst, const bf16_t *src, int64_t ld, int64_t rows, int64_t cols)
+{
+    const int64_t per_block = std::max<int64_t>(1, 1024 / cols) * 8;   // four pieces a lane
+    return {dst, src, ld, rows, (int)cols, (int)per_block, (int)cdiv(rows, per_block)};
+}
+// The rows that count and the weight as the tiles read it: rows from 16-byte boundaries on
+static int head_gather(const HeadCall &c, const float *stats, const float *dloss_rows, const bf16_t **w, int64_t *ldw)
 {
     const HeadPlan &h = c.h;
     HeadGather p = {};
-    p.xc = c.at<bf16_t>(h.xc);
-    p.x = static_cast<const bf16_t *>(c.x);
-    p.ldx = c.ldx;
-    p.ldc = h.dp;
-    p.target = c.target;
-    p.pos = c.at<int>(h.pos);
-    p.count = c.at<int>(h.count);
-    if (h.backward) {
-        p.lse2 = c.at<float>(h.lse2);
-        p.factor = c.at<float>(h.factor);
-        p.label = c.at<int>(h.label);
-        p.stats = stats;
-        p.dloss = dloss_rows;
-    }
-    p.tokens = h.tokens;
-    p.dim = h.dim;
-    p.classes = h.classes;
-    p.ignore = c.ignore;
-    p.rows = h.tokens > 16384 ? 64 : h.tokens > 4096 ? 8 : 4;
-    head_gather_kernel<<<(unsigned)cdiv(h.tokens, p.rows), 256, 0, c.s>>>(p);
-    return check_launch("head_gather_kernel");
-}
-template <bool PAD> static int head_repack(bf16_t *dst, const bf16_t *src, int64_t lds, int64_t rows, int64_t cols, hipStream_t s)
-{
-    const int64_t per_block = std::max<int64_t>(1, 1024 / cols) * 8;   // four pieces a lane
-    head_repack_kernel<PAD><<<(unsigned)cdiv(rows, per_block), 256, 0, s>>>(dst, src, lds, rows, (int)cols, (int)per_block);
-    return check_launch("head_repack_kernel");
-}
-// the weight as the tiles read it: rows from 16-byte boundaries on
-static int head_weight(const HeadCall &c, const bf16_t **w, int64_t *ldw)
-{
+    HeadRepack r = {};
+    int64_t gathering = 0;
     *w = static_cast<const bf16_t *>(c.w);
     *ldw = c.ldw;
-    if (!c.h.pack_w) return RDB_OK;
-    bf16_t *wc = c.at<bf16_t>(c.h.wc);
-    const int rc = head_repack<true>(wc, *w, c.ldw, c.h.classes, c.h.dim, c.s);
-    *w = wc;
-    *ldw = c.h.dp;
-    return rc;
+    if (h.pack_w) {
+        r = head_repack(c.at<bf16_t>(h.wc), *w, c.ldw, h.classes, h.dim);
+        *w = r.dst;
+        *ldw = h.dp;
+    }
+    if (!h.direct) {
+        p.xc = c.at<bf16_t>(h.xc);
+        p.x = static_cast<const bf16_t *>(c.x);
+        p.ldx = c.ldx;
+        p.ldc = h.dp;
+        p.target = c.target;
+        p.pos = c.at<int>(h.pos);
+        p.count = c.at<int>(h.count);
+        if (h.backward) {
+            p.lse2 = c.at<float>(h.lse2);
+            p.factor = c.at<float>(h.factor);
+            p.label = c.at<int>(h.label);
+            p.stats = stats;
+            p.dloss = dloss_rows;
+        }
+        p.tokens = h.tokens;
+        p.dim = h.dim;
+        p.classes = h.classes;
+        p.ignore = c.ignore;
+        p.rows = h.tokens > 16384 ? 64 : h.tokens > 4096 ? 8 : 4;
+        gathering = cdiv(h.tokens, p.rows);
+    }
+    if (!gathering && !r.blocks) return RDB_OK;
+    head_gather_kernel<<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
+    return check_launch("head_gather_kernel");
 }
 
 template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool few, hipStream_t s)
@@ -844,11 +861,9 @@ static HeadSum head_sum_of(const HeadCall &c, float *loss, float *stats, int red
 static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
-    if (!h.direct)
-        if (int rc = head_gather(c, nullptr, nullptr)) return rc;
     const bf16_t *w;
     int64_t ldw;
-    if (int rc = head_weight(c, &w, &ldw)) return rc;
+    if (int rc = head_gather(c, nullptr, nullptr, &w, &ldw)) return rc;
     HeadLogits p = {};
     p.x = h.direct ? static_cast<const bf16_t *>(c.x) : c.at<bf16_t>(h.xc);
     p.ldx = h.direct ? c.ldx : h.dp;
@@ -870,10 +885,9 @@ static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduc
 static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float *dloss, const float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
-    if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr)) return rc;
     const bf16_t *w;
     int64_t ldw;
-    if (int rc = head_weight(c, &w, &ldw)) return rc;
+    if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr, &w, &ldw)) return rc;
     const HeadScale scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
     bf16_t *dwc = h.pad_dw && dw ? c.at<bf16_t>(h.dw) : dw;
     const int *count = c.at<int>(h.count);
@@ -939,13 +953,12 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
         else head_products_kernel<false><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
         if (int rc = check_launch("head_products_kernel")) return rc;
     }
-    if (dx) {
-        const int64_t blocks = std::min<int64_t>(cdiv(h.tokens * h.dp / 4, 256), 8192);
-        head_dx_kernel<<<(unsigned)blocks, 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale);
-        if (int rc = check_launch("head_dx_kernel")) return rc;
-    }
-    if (dw && h.pad_dw) return head_repack<false>(dw, dwc, h.dp, h.classes, h.dim, c.s);
-    return RDB_OK;
+    HeadRepack r = {};
+    if (dw && h.pad_dw) r = head_repack(dw, dwc, h.dp, h.classes, h.dim);
+    const int64_t summing = dx ? std::min<int64_t>(cdiv(h.tokens * h.dp / 4, 256), 8192) : 0;
+    if (!summing && !r.blocks) return RDB_OK;
+    head_dx_kernel<<<(unsigned)(summing + r.blocks), 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale, r);
+    return check_launch("head_dx_kernel");
 }
 
 static HeadRows head_rows(const HeadCall &c)
