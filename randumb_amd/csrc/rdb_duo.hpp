@@ -14,7 +14,7 @@ namespace rdb {
 
 constexpr int DUO_A = 256, DUO_B = 128, DUO_K = 64;
 constexpr int DUO_MI = 4, DUO_NI = 2;                         // 32 x 32 blocks of a wave
-constexpr int DUO_LDS = (2 * DUO_A + DUO_B) * DUO_K;          // elements
+constexpr int DUO_LDS = (2 * DUO_A + DUO_B) * DUO_K, SOLO_LDS = 3 * (DUO_A + DUO_B) * DUO_K;   // elements
 
 // One operand's tile: where its 16-byte pieces lie in LDS, and which of them a lane requests.
 template <int ROWS, int LAYOUT> struct DuoOperand {
@@ -78,20 +78,22 @@ __device__ __forceinline__ uint32_t duo_lds_address(const bf16_t *p)
     return __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const bf16_t __attribute__((address_space(3))) *)p);
 }
 
-// Contracts `nstage` stages of 64 into acc (at least one: of no contraction values it is a stage of zeros).  lds: DUO_LDS elements, free on entry and again on return.
+// Contracts `nstage` stages of 64 into acc (at least one: of no contraction values it is a stage of zeros).  lds: DUO_LDS (SOLO_LDS) elements, free on entry and again on return.
 // A stage's last k-step waits in registers and is multiplied behind the next barrier, while that stage's first fragments come in (as in big_stage).
-template <class PA, class PB>
+// SOLO: one block a compute unit, for launches that have no second one for it: all of LDS holds three stages of both, and two are on their way.
+template <bool SOLO, class PA, class PB>
 __device__ __forceinline__ void duo_mainloop(f32x16 (&acc)[DUO_MI][DUO_NI], bf16_t *__restrict__ lds, const PA &pa, const PB &pb, int nstage)
 {
     const int t = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, arow = (wave >> 1) * DUO_MI * 32, brow = (wave & 1) * DUO_NI * 32;
-    const uint32_t base = duo_lds_address(lds) + (uint32_t)wave * 1024u, b_at = base + 4u * PA::ELEMS;
-    const bf16_t *Bs = lds + 2 * PA::ELEMS;
-    {
-        const uint32_t at_a = pa.stage(0), at_b = pb.stage(0);
+    constexpr int AHEAD = SOLO ? 2 : 1, BUFFERS = AHEAD + 1;   // stages on their way; of A
+    const uint32_t base = duo_lds_address(lds) + (uint32_t)wave * 1024u, b_base = base + BUFFERS * 2u * PA::ELEMS;
 #pragma unroll
-        for (int p = 0; p < PA::PER_WAVE; ++p) pa.request(at_a, p, base);
+    for (int s = 0; s < AHEAD; ++s) {
+        const uint32_t at_a = pa.stage(s), at_b = pb.stage(s);
 #pragma unroll
-        for (int p = 0; p < PB::PER_WAVE; ++p) pb.request(at_b, p, b_at);
+        for (int p = 0; p < PA::PER_WAVE; ++p) pa.request(at_a, p, base + s * (2u * PA::ELEMS));
+#pragma unroll
+        for (int p = 0; p < PB::PER_WAVE; ++p) pb.request(at_b, p, b_base + s * (2u * PB::ELEMS));
     }
     bf16x8 fa[2][DUO_MI], fb[4][DUO_NI];
 #pragma unroll
@@ -105,13 +107,15 @@ __device__ __forceinline__ void duo_mainloop(f32x16 (&acc)[DUO_MI][DUO_NI], bf16
     constexpr int N = DUO_MI * DUO_NI;
     auto multiply = [&](int i, int a, int b) { acc[i >> 1][i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[a][i >> 1], fb[b][i & 1], acc[i >> 1][i & 1], 0, 0, 0); };
     int s = 0;
-    uint32_t odd = 0;   // which of A's buffers holds stage s
+    uint32_t now = 0, then = AHEAD;   // the buffers of stages s and s + AHEAD
     do {
         // stage s has arrived, and nobody reads the buffer of stage s - 1 any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const bf16_t *As = lds + odd * PA::ELEMS;
-        odd ^= 1;
-        const uint32_t to = base + odd * (2u * PA::ELEMS), at_a = pa.stage(s + 1), at_b = pb.stage(s + 1);
+        if constexpr (SOLO) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PA::PER_WAVE + PB::PER_WAVE) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const bf16_t *As = lds + now * PA::ELEMS, *Bs = lds + BUFFERS * PA::ELEMS + (SOLO ? now * PB::ELEMS : 0u);
+        const uint32_t to = base + then * (2u * PA::ELEMS), b_to = b_base + (SOLO ? then * (2u * PB::ELEMS) : 0u), at_a = pa.stage(s + AHEAD), at_b = pb.stage(s + AHEAD);
+        now = now == AHEAD ? 0 : now + 1;
+        then = then == AHEAD ? 0 : then + 1;
         // Fragments and requests a few in front of each matrix instruction: requests all at once hold a wave up for as long as the compute unit takes to look
         // them up, with its matrix instructions behind them.
 #pragma unroll
@@ -148,10 +152,10 @@ __device__ __forceinline__ void duo_mainloop(f32x16 (&acc)[DUO_MI][DUO_NI], bf16
             multiply(i, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // B is in everybody's registers
+        if constexpr (!SOLO) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // B is in everybody's registers
 #pragma unroll
         for (int i = 0; i < N; ++i) {   // k-step 1
-            if (i < PB::PER_WAVE) pb.request(at_b, i, b_at);
+            if (i < PB::PER_WAVE) pb.request(at_b, i, b_to);
             if (i == 1 || i == 2) {
                 fa[0][2 * i - 2] = PA::frag(As, arow + (2 * i - 2) * 32, 2, lane);
                 fa[0][2 * i - 1] = PA::frag(As, arow + (2 * i - 1) * 32, 2, lane);

@@ -10,7 +10,8 @@
 // bf16 (products on the tiles of rdb_duo.hpp, of few tokens on those of rdb_gemm.hpp):
 //   head_gather_kernel      the rows that count, one after the other, in rows of a multiple of 8 values
 //   head_logits_duo_kernel  a tile of logits in the accumulators -> its maximum and its sum of exponentials for each token; or (backward), a piece of the
-//   head_logits_few_kernel  vocabulary's logits once more -> G, in bf16, for the next launch
+//   head_logits_solo_kernel vocabulary's logits once more -> G, in bf16, for the next launch
+//   head_logits_few_kernel
 //   head_merge_kernel       the tiles of a token together, the target's logit, nll; the last block adds up the tokens
 //   head_products_kernel    dx += G . W and dW = G^T . x of the piece, and the next piece's G, one list of tiles
 //   head_dx_kernel          dx from its sums, back in the rows' own places
@@ -315,7 +316,7 @@ static int head_few_tile(int64_t classes) { return cdiv(classes, 128) >= num_com
 static int head_few_blocks(int64_t classes) { return (int)std::min<int64_t>(cdiv(classes, head_few_tile(classes)), 2 * num_compute_units()); }
 
 // The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
-template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
+template <bool GRAD, bool SOLO> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
 {
     const int tiles_t = (count + HD_TOK - 1) / HD_TOK, total = p.tiles_v * tiles_t, per_die = (total + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
     if ((block >> 3) >= per_die || w >= total) return;
@@ -327,14 +328,19 @@ template <bool GRAD> __device__ __forceinline__ void head_logits_tile(const Head
     pb.set(p.x + (int64_t)tok0 * p.ldx, p.ldx, 0, min(HD_TOK, count - tok0), p.dim);
     f32x16 acc[DUO_MI][DUO_NI];
     duo_zero(acc);
-    duo_mainloop(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
+    duo_mainloop<SOLO>(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
     if constexpr (GRAD) head_leave_grad<DUO_MI, DUO_NI>(acc, lds, p, tv, tok0, count, (int)threadIdx.x);
     else head_leave_stats<DUO_MI, DUO_NI>(acc, p, tv, tok0, count, (int)threadIdx.x);
 }
 template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
-    head_logits_tile<GRAD>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
+    head_logits_tile<GRAD, false>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
+}
+template <bool GRAD> __global__ __launch_bounds__(256, 1) void head_logits_solo_kernel(HeadLogits p)
+{
+    __shared__ __align__(16) bf16_t lds[SOLO_LDS];
+    head_logits_tile<GRAD, true>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------- loss
@@ -527,7 +533,7 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
     const int count = *p.count;
     int block = (int)blockIdx.x;
-    if (block >= p.blocks_dw + p.blocks_dx) return head_logits_tile<true>(next, lds, count, block - p.blocks_dw - p.blocks_dx);
+    if (block >= p.blocks_dw + p.blocks_dx) return head_logits_tile<true, false>(next, lds, count, block - p.blocks_dw - p.blocks_dx);
     const bool dw = block < p.blocks_dw;
     if (!dw) block -= p.blocks_dw;
     const int tiles_t = (count + HD_TILE - 1) / HD_TILE, n = (dw ? p.tiles_v : p.splits * tiles_t) * p.tiles_d, per_die = (n + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
@@ -541,7 +547,7 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
         DuoOperand<DUO_B, M_CONT> pb;   // x: rows = its columns
         pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
         pb.set(p.x, p.ldx, b0, p.dim, count);
-        duo_mainloop(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
+        duo_mainloop<false>(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
         head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), (int)threadIdx.x);
     } else {
         const int tt = w / p.tiles_d % tiles_t, s = w / p.tiles_d / tiles_t, v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE;
@@ -550,7 +556,7 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
         DuoOperand<DUO_B, M_CONT> pb;   // W: rows = its columns
         pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7);
         pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
-        duo_mainloop(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
+        duo_mainloop<false>(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
         head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, (int)threadIdx.x);
     }
 }
@@ -839,6 +845,9 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
     return check_launch("head_gather_kernel");
 }
 
+// One block a compute unit where there are no more tiles than that, and stages enough to have two on their way.  us a forward call, two blocks a unit | one: 97 tokens x 640 -> 44480
+// 29.1 | 26.6, 717 x 1000 -> 10001 34.6 | 31.9, 2048 x 2048 -> 4000 51.8 | 49.5; 2048 x 256 -> 4000 21.4 | 22.2, 1300 x 64 -> 6000 18.9 | 19.3.
+constexpr int HD_SOLO_DIM = 512;
 template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool few, hipStream_t s)
 {
     p.tiles_v = (int)cdiv(classes, few ? head_few_tile(classes) : HD_TILE);
@@ -848,7 +857,12 @@ template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool
         else head_logits_few_kernel<GRAD, 64><<<blocks, 256, 0, s>>>(p);
         return check_launch(GRAD ? "head_logits_few_kernel<gradient>" : "head_logits_few_kernel");
     }
-    head_logits_duo_kernel<GRAD><<<(unsigned)((p.tiles_v * cdiv(p.tokens, HD_TOK) + 7) / 8 * 8), 256, 0, s>>>(p);
+    const int64_t tiles = p.tiles_v * cdiv(p.tokens, HD_TOK);
+    if (tiles <= num_compute_units() && p.dim >= HD_SOLO_DIM) {
+        head_logits_solo_kernel<GRAD><<<(unsigned)((tiles + 7) / 8 * 8), 256, 0, s>>>(p);
+        return check_launch(GRAD ? "head_logits_solo_kernel<gradient>" : "head_logits_solo_kernel");
+    }
+    head_logits_duo_kernel<GRAD><<<(unsigned)((tiles + 7) / 8 * 8), 256, 0, s>>>(p);
     return check_launch(GRAD ? "head_logits_duo_kernel<gradient>" : "head_logits_duo_kernel");
 }
 

@@ -296,3 +296,13 @@ def test_rows_that_lie_far_apart(dtype):
     far[:, :dim] = x
     for p, q in zip(both(x, w, t, "mean"), both(far[:, :dim], w, t, "mean")):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("tokens,dim,classes", [(1300, 72, 7000), (1300, 64, 6000), (130, 200, 33000), (130, 600, 32000), (2100, 520, 4000), (1900, 1000, 4300), (700, 1024, 9000)])
+def test_fewer_and_more_tiles_than_compute_units(tokens, dim, classes):
+    """One and two blocks a compute unit, one stage of the contraction and several, rows that are left out among them."""
+    print(f"case head loss {tokens} x {dim} -> {classes}", flush=True)
+    for reduction, ignored in (("mean", 0.0), ("none", 0.2)):
+        x, w, t = inputs(tokens, dim, classes, torch.bfloat16, tokens + classes, ignored)
+        loss, dloss, dx, dw = both(x, w, t, reduction)
+        check(x, w, t, reduction, loss, dloss, dx, dw)
