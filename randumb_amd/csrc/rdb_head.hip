@@ -11,13 +11,13 @@
 //   head_gather_kernel      the rows that count, one after the other, in rows of a multiple of 8 values
 //   head_logits_duo_kernel  a tile of logits in the accumulators -> its maximum and its sum of exponentials for each token; or (backward), a piece of the
 //   head_logits_solo_kernel vocabulary's logits once more -> G, in bf16, for the next launch
-//   head_logits_few_kernel
+//   head_logits_few_kernel  (all tokens in one tile)
 //   head_merge_kernel       the tiles of a token together, the target's logit, nll; the last block adds up the tokens
 //   head_products_kernel    dx += G . W and dW = G^T . x of the piece, and the next piece's G, one list of tiles
 //   head_dx_kernel          dx from its sums, back in the rows' own places
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
 // which are nearly all of the gradient, would all be off by the same rounding.
-// fp32: the products of rdb_f32.hip, logits of a piece in fp32 in between; ignored rows are rows of zeros of G there.
+// fp32: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between; ignored rows are rows of zeros of G there.
 //
 // Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 68 % of the time at
 // 1.7 GHz in the statistics and in the products alike (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
@@ -677,6 +677,142 @@ __global__ __launch_bounds__(256) void head_add_kernel(float *__restrict__ out, 
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] += a[i];
 }
 
+// fp32, up to 32 tokens: both products that read the weight, bound by reading it, on the fp32 matrix instructions, which here are faster than splitting the weight for the bf16 ones.
+// us a product, split | these: 12 tokens x 2048 -> 47643 (390 MB, 70 by reading alone) logits 144 | 100, dx 142 | 95; steps of 3 x 1024 -> 72064 389 | 350, 32 x 1024 -> 30000
+// 167 | 163.  With two tiles of tokens they lose (64 x 1024 -> 30000: logits 44 | 87); without the way through LDS, each lane reading a row, the logits take 142.
+constexpr int HS_T = 32;   // tokens, at most
+struct HeadFew {
+    const float *x, *w;    // logits: hidden states [tokens][ldx]; dx: G
+    int64_t ldx, ldw;
+    float *out;            // logits [tokens][classes]; dx: [ranges][tokens][dim] sums
+    int tokens, dim, classes;
+    int range;             // dx: classes of a range, a multiple of 32
+};
+__device__ __forceinline__ f32x4 head_load4(const float *p, int left, bool whole)
+{
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (whole) __builtin_memcpy(&v, p, 16);   // at any address
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) v[e] = p[e];
+    return v;
+}
+// The waves' sums one after the other: deterministic.  COLS values a token.
+template <int COLS, typename F> __device__ __forceinline__ void head_add_waves(float (&sums)[HS_T][COLS + 4], int wave, F value)
+{
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) value([&](int tok, int col, float v) { sums[tok][col] = w ? sums[tok][col] + v : v; });
+        __syncthreads();
+    }
+}
+// Logits of 64 classes: a wave takes every fourth 32 of the contraction, in whole lines of memory, through LDS of its own (16-byte piece c of row r at c ^ (r & 7)); a lane has four
+// neighbours of a class's row and of a token's there (which instruction multiplies which of them is the same for both).
+__global__ __launch_bounds__(256, 2) void head_few_logits_kernel(HeadFew p)
+{
+    constexpr int V = 64, ROWS = V + HS_T, LOADS = ROWS / 8;
+    __shared__ __align__(16) float rows_[4][ROWS * 32];
+    __shared__ float sums[HS_T][V + 4];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, v0 = (int)blockIdx.x * V, piece = lane & 7;
+    const float *from[LOADS];
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+        const int row = q * 8 + (lane >> 3);
+        from[q] = row < V ? p.w + (int64_t)min(v0 + row, p.classes - 1) * p.ldw : p.x + (int64_t)min(row - V, p.tokens - 1) * p.ldx;
+    }
+    float *lds = rows_[wave], *to = lds + (lane >> 3) * 32 + (piece ^ (lane >> 3)) * 4;
+    f32x16 acc[2] = {zero16(), zero16()};
+    f32x4 next[LOADS];
+    auto load = [&](int k) {
+        const bool whole = k + 32 <= p.dim;
+        const int at = k + piece * 4;
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q) next[q] = head_load4(from[q] + at, p.dim - at, whole);
+    };
+    load(wave * 32);
+    for (int k = wave * 32; k < p.dim; k += 128) {   // behind the last value: zeros
+#pragma unroll
+        for (int q = 0; q < LOADS; ++q) *reinterpret_cast<f32x4 *>(to + q * 256) = next[q];
+        load(k + 128);
+        __builtin_amdgcn_wave_barrier();   // LDS serves a wave's instructions in order: the reads see these writes, and the next writes come behind the reads
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f32x4 v[3];
+#pragma unroll
+            for (int m = 0; m < 3; ++m) v[m] = *reinterpret_cast<const f32x4 *>(lds + (m * 32 + r) * 32 + (((q * 2 + g) ^ (r & 7)) * 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int mi = 0; mi < 2; ++mi) acc[mi] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[mi][e], v[2][e], acc[mi], 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    head_add_waves<V>(sums, wave, [&](auto add) {
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) add(r, mi * 32 + head_row(j, g), acc[mi][j]);
+    });
+    for (int i = t; i < HS_T * V; i += 256) {
+        const int tok = i / V, v = i % V;
+        if (tok < p.tokens && v0 + v < p.classes) p.out[(int64_t)tok * p.classes + v0 + v] = sums[tok][v];
+    }
+}
+// dx, 128 columns and a range of the classes: a wave takes every fourth 8 of them, a lane four neighbouring columns of a class's row, which go to four accumulators.
+__global__ __launch_bounds__(256, 2) void head_few_dx_kernel(HeadFew p)
+{
+    __shared__ float sums[HS_T][128 + 4];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, d0 = (int)blockIdx.x * 128, d = d0 + r * 4;
+    const int begin = (int)blockIdx.y * p.range, end = min(p.classes, begin + p.range), left = p.dim - d;
+    const float *w = p.w + (left > 0 ? d : 0), *x = p.x + (int64_t)min(r, p.tokens - 1) * p.ldx;   // columns behind the last are nobody's
+    f32x16 acc[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = zero16();
+    f32x4 a[2][4], b[2];
+    auto load = [&](int i, int v) {
+        const bool whole = v + 8 <= end, columns = whole && p.dim % 4 == 0;
+        v += g * 4;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[i][s] = head_load4(w + (int64_t)min(v + s, p.classes - 1) * p.ldw, v + s < end ? left : 0, columns);
+        b[i] = head_load4(x + v, end - v, whole);
+    };
+    auto multiply = [&](int i) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][s][e], b[i][s], acc[e], 0, 0, 0);
+    };
+    load(0, begin + wave * 8);
+    for (int v = begin + wave * 8; v < end; v += 64) {
+        load(1, v + 32);
+        multiply(0);
+        load(0, v + 64);
+        multiply(1);
+    }
+    head_add_waves<128>(sums, wave, [&](auto add) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) add(r, 4 * head_row(j, g) + e, acc[e][j]);
+    });
+    float *out = p.out + (int64_t)blockIdx.y * p.tokens * p.dim;
+    for (int i = t; i < HS_T * 128; i += 256) {
+        const int tok = i / 128, c = d0 + i % 128;
+        if (tok < p.tokens && c < p.dim) out[(int64_t)tok * p.dim + c] = sums[tok][i % 128];
+    }
+}
+// out = the ranges' sums, and what is there
+__global__ __launch_bounds__(256) void head_few_sum_kernel(float *__restrict__ out, const float *__restrict__ sums, int64_t n, int ranges, bool add)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float v = add ? out[i] : 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < ranges; ++s) v += sums[s * n + i];
+    out[i] = v;
+}
+
 // ----------------------------------------------------------------------------------------------- plan and calls
 // Bytes of a piece's G (bf16) or logits (fp32).  Such an amount the next launch finds in the chip's last-level cache.  A piece of G is twice or four times as large where
 // its launch (dW, dx and the next piece's logits) would otherwise end with dW's tiles, which contract all tokens: in units of a stage of 64, as long as a block
@@ -701,6 +837,7 @@ struct HeadPlan {
     int64_t dp, vp;            // columns of the copies; classes of a piece
     int pieces, splits;
     bool few;                  // one tile of few tokens
+    int64_t range;             // fp32, few: classes of a range of dx
     int parts;                 // of a token's sum
     int64_t split_v;
     // offsets in the workspace
@@ -734,6 +871,10 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     if (f32 && h.pieces == 1) h.vp = classes;
     h.pieces = (int)cdiv(classes, h.vp);
     h.few = tokens <= HD_FEW;
+    if (f32 && tokens <= HS_T) {   // ranges of dx: four blocks a compute unit, at least 128 classes each, sums of at most an eighth of the weight's bytes
+        const int64_t most = std::min(4 * num_compute_units() / cdiv(dim, 128), std::min(h.vp / 128, h.vp / (8 * tokens)));
+        h.range = cdiv(cdiv(h.vp, std::max<int64_t>(1, most)), 32) * 32;
+    }
     const int64_t tiles = cdiv(tokens, HD_TILE) * cdiv(dim, DUO_B);
     // Ranges of the classes, each with sums of dx of its own, until every block slot has a tile: at least 4 stages each, and 16 ranges or 16 MB of sums (24 tokens x 960 ->
     // 39040: 16 ranges of 38 stages 60 us, 64 of 10 35; 5 x 64 -> 1792: one of 28 24 us, 7 of 4 7).
@@ -770,7 +911,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
             h.label = room(tokens * 4);
         }
         h.g = room(tokens * h.vp * es * (!f32 && h.pieces > 1 ? 2 : 1));   // bf16: a piece's, and the next one's beside it
-        if (want_dx && (!f32 || h.pieces > 1)) h.dx = room((f32 ? 1 : h.splits) * tokens * (f32 ? dim : h.dp) * 4);
+        if (want_dx && (!f32 || h.range || h.pieces > 1)) h.dx = room((!f32 ? h.splits : h.range ? cdiv(h.vp, h.range) : 1) * tokens * h.dp * 4);
         if (want_dw && h.pad_dw) h.dw = room(classes * h.dp * 2 + 16);
     }
     if (f32) {
@@ -984,6 +1125,36 @@ static HeadRows head_rows(const HeadCall &c)
     p.sum.ignore = c.ignore;
     return p;
 }
+// logits of classes v0 .. v0 + n
+static int head_logits_f32(const HeadCall &c, float *logits, int64_t v0, int64_t n)
+{
+    const HeadPlan &h = c.h;
+    const float *x = static_cast<const float *>(c.x), *w = static_cast<const float *>(c.w) + v0 * c.ldw;
+    if (!h.range) return rdb_product_f32(logits, x, c.ldx, 0, w, c.ldw, 0, nullptr, h.tokens, n, h.dim, c.at<void>(h.product), h.product_bytes, c.s);
+    const HeadFew p = {x, w, c.ldx, c.ldw, logits, (int)h.tokens, (int)h.dim, (int)n, 0};
+    head_few_logits_kernel<<<(unsigned)cdiv(n, 64), 256, 0, c.s>>>(p);
+    return check_launch("head_few_logits_kernel");
+}
+// dx, or what these classes add to it
+static int head_dx_f32(const HeadCall &c, float *dx, const float *g, int64_t v0, int64_t n, bool add)
+{
+    const HeadPlan &h = c.h;
+    const float *w = static_cast<const float *>(c.w) + v0 * c.ldw;
+    const int64_t count = h.tokens * h.dim;
+    if (h.range) {
+        const HeadFew p = {g, w, n, c.ldw, c.at<float>(h.dx), (int)h.tokens, (int)h.dim, (int)n, (int)h.range};
+        const dim3 grid((unsigned)cdiv(h.dim, 128), (unsigned)cdiv(n, h.range));
+        head_few_dx_kernel<<<grid, 256, 0, c.s>>>(p);
+        if (int rc = check_launch("head_few_dx_kernel")) return rc;
+        head_few_sum_kernel<<<(unsigned)cdiv(count, 256), 256, 0, c.s>>>(dx, p.out, count, (int)grid.y, add);
+        return check_launch("head_few_sum_kernel");
+    }
+    float *to = add ? c.at<float>(h.dx) : dx;
+    if (int rc = rdb_product_f32(to, g, n, 0, w, c.ldw, 1, nullptr, h.tokens, h.dim, n, c.at<void>(h.product), h.product_bytes, c.s)) return rc;
+    if (!add) return RDB_OK;
+    head_add_kernel<<<(unsigned)std::min<int64_t>(cdiv(count, 1024), 4096), 256, 0, c.s>>>(dx, to, count);
+    return check_launch("head_add_kernel");
+}
 static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
@@ -994,9 +1165,7 @@ static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduct
     p.sum = head_sum_of(c, loss, stats, reduction);
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
-        if (int rc = rdb_product_f32(p.logits, static_cast<const float *>(c.x), c.ldx, 0, static_cast<const float *>(c.w) + v0 * c.ldw, c.ldw, 0, nullptr, h.tokens, n, h.dim,
-                                     c.at<void>(h.product), h.product_bytes, c.s))
-            return rc;
+        if (int rc = head_logits_f32(c, p.logits, v0, n)) return rc;
         p.n = (int)n;
         p.v0 = (int)v0;
         p.first = i == 0;
@@ -1022,25 +1191,17 @@ static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dl
     p.dim = (int)h.dim;
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
-        const float *w = static_cast<const float *>(c.w) + v0 * c.ldw;
-        void *room = c.at<void>(h.product);
-        if (int rc = rdb_product_f32(p.logits, p.x, c.ldx, 0, w, c.ldw, 0, nullptr, h.tokens, n, h.dim, room, h.product_bytes, c.s)) return rc;
+        if (int rc = head_logits_f32(c, p.logits, v0, n)) return rc;
         p.n = (int)n;
         p.v0 = (int)v0;
         p.xc = dw && i == 0 ? c.at<float>(h.xc) : nullptr;
         p.columns = h.tokens < 2 * num_compute_units() ? 4096 : p.n;
         head_rows_grad_kernel<<<dim3((unsigned)h.tokens, (unsigned)cdiv(n, p.columns)), 256, 0, c.s>>>(p);
         if (int rc = check_launch("head_rows_grad_kernel")) return rc;
-        if (dx) {
-            float *to = i ? c.at<float>(h.dx) : dx;
-            if (int rc = rdb_product_f32(to, p.logits, n, 0, w, c.ldw, 1, nullptr, h.tokens, h.dim, n, room, h.product_bytes, c.s)) return rc;
-            if (i) {
-                head_add_kernel<<<(unsigned)std::min<int64_t>(cdiv(h.tokens * h.dim, 1024), 4096), 256, 0, c.s>>>(dx, to, h.tokens * h.dim);
-                if (int rc = check_launch("head_add_kernel")) return rc;
-            }
-        }
+        if (dx)
+            if (int rc = head_dx_f32(c, dx, p.logits, v0, n, i > 0)) return rc;
         if (dw)
-            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, c.at<float>(h.xc), h.dim, 1, nullptr, n, h.dim, h.tokens, room, h.product_bytes, c.s)) return rc;
+            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, c.at<float>(h.xc), h.dim, 1, nullptr, n, h.dim, h.tokens, c.at<void>(h.product), h.product_bytes, c.s)) return rc;
     }
     return RDB_OK;
 }

@@ -306,3 +306,16 @@ def test_fewer_and_more_tiles_than_compute_units(tokens, dim, classes):
         x, w, t = inputs(tokens, dim, classes, torch.bfloat16, tokens + classes, ignored)
         loss, dloss, dx, dw = both(x, w, t, reduction)
         check(x, w, t, reduction, loss, dloss, dx, dw)
+
+
+@pytest.mark.parametrize("tokens,dim,classes", [(1, 1000, 3001), (5, 259, 5000), (12, 2048, 1500), (32, 128, 2048), (33, 1030, 3001), (64, 300, 4099), (64, 8, 1100000)])
+def test_few_tokens_in_fp32(tokens, dim, classes):
+    """Whole and ragged columns, ranges of the classes and (the last one) pieces of them, strides of single values."""
+    print(f"case head loss {tokens} x {dim} -> {classes} fp32", flush=True)
+    for reduction, ignored in (("mean", 0.0), ("none", 0.3)):
+        x, w, t = inputs(tokens, dim, classes, torch.float32, tokens + classes, ignored)
+        wide_x, wide_w = torch.full((tokens, dim + 3), float("nan"), device="cuda"), torch.full((classes, dim + 1), float("nan"), device="cuda")
+        wide_x[:, 1:dim + 1], wide_w[:, :dim] = x, w
+        for a, b in ((x, w), (wide_x[:, 1:dim + 1], wide_w[:, :dim])):
+            loss, dloss, dx, dw = both(a, b, t, reduction)
+            check(x, w, t, reduction, loss, dloss, dx, dw)
