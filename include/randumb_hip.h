@@ -553,7 +553,7 @@ int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const vo
                              int64_t batch, int64_t T, int64_t heads, float eps, void *stream);
 
 /* ------------------------------------------------------------------------------------------ ends of a language model
- * Softmax cross entropy of an output head without its logits: F.cross_entropy(F.linear(x, w), target) of modded-nanogpt/gpt_models.py's head and loss, x [tokens x dim]
+ * Softmax cross entropy of an output head in pieces of its logits: F.cross_entropy(F.linear(x, w), target) of modded-nanogpt/gpt_models.py's head and loss, x [tokens x dim]
  * and w [classes x dim] both of `dtype` (RDB_F32 or RDB_BF16) with unit inner stride, target int64.  Products, exponentials and sums in fp32 (bf16: on the matrix cores with fp32
  * sums; fp32: rdb_product_f32's).
  *   reduction  0: loss[tokens] (0 where target == ignore_index); 1: loss[0], the mean over the other rows (NaN of none); 2: loss[0], their sum
@@ -566,10 +566,13 @@ int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const vo
  * 2^38 bf16 logits or more in tiles of 128 x 256 (size query: 0). */
 int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
                                                  int backward, int want_dx, int want_dw);
-int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
+/* Floats of the logits that a forward call leaves for the backward call, where both are given a buffer of them (NULL: none), in fp32: of up to dim / 4
+ * tokens, so that they are at most a quarter of the weight's bytes, and 2^26 logits.  The backward call then does not compute them again: the same bits.  0: never. */
+int64_t rdb_linear_cross_entropy_keeps(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw);
+int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
                                  int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace, int64_t workspace_bytes,
                                  void *stream);
-int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
                                  const int64_t *target, int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace,
                                  int64_t workspace_bytes, void *stream);
 

@@ -100,6 +100,7 @@ EXPORTS = [
     "rdb_causal_attention_fwd",
     "rdb_causal_attention_bwd",
     "rdb_linear_cross_entropy_workspace_bytes",
+    "rdb_linear_cross_entropy_keeps",
     "rdb_linear_cross_entropy_fwd",
     "rdb_linear_cross_entropy_bwd",
     "rdb_rotary",
@@ -298,8 +299,10 @@ def load() -> ctypes.CDLL:
     L.rdb_causal_attention_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, f32, vp]
     L.rdb_linear_cross_entropy_workspace_bytes.argtypes = [i64, i64, i64, ci, vp, i64, vp, i64, ci, ci, ci]
     L.rdb_linear_cross_entropy_workspace_bytes.restype = i64
-    L.rdb_linear_cross_entropy_fwd.argtypes = [vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
-    L.rdb_linear_cross_entropy_bwd.argtypes = [vp, vp, vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
+    L.rdb_linear_cross_entropy_keeps.argtypes = [i64, i64, i64, ci, i64]
+    L.rdb_linear_cross_entropy_keeps.restype = i64
+    L.rdb_linear_cross_entropy_fwd.argtypes = [vp, vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
+    L.rdb_linear_cross_entropy_bwd.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp, i64, ci, vp, i64, i64, i64, i64, ci, vp, i64, vp]
     rp = ctypes.POINTER(RotaryRows)
     L.rdb_rotary.argtypes = [rp, rp, ci, i64, i64, i64, vp, i64, vp, ci, i64, i64, ci, f32, ci, vp]
     for name in ("rdb_sq5_fill_2d", "rdb_sq5_fill_1d", "rdb_materialize_fwd", "rdb_materialize_bwd", "rdb_scale_bias_bwd",

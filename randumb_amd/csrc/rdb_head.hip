@@ -1,5 +1,5 @@
 // Softmax cross entropy of an output head, x . W^T over a large vocabulary, and its gradient, in pieces of the vocabulary: the logits are
-// never kept, and neither is their gradient.
+// never kept whole (but those of few tokens in fp32), and neither is their gradient.
 //
 //   lse[t] = log sum_v exp <x_t, w_v>,  nll[t] = lse[t] - <x_t, w_target[t]>,  loss = their mean, their sum, or nll itself
 //   G[t][v] = (exp(<x_t, w_v> - lse[t]) - [v == target[t]]) g_t,   dx = G . W,   dW = G^T . x
@@ -17,7 +17,8 @@
 //   head_dx_kernel          dx from its sums, back in the rows' own places
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
 // which are nearly all of the gradient, would all be off by the same rounding.
-// fp32: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between; ignored rows are rows of zeros of G there.
+// fp32: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between, which of few tokens stay for the
+// backward pass (rdb_linear_cross_entropy_keeps); ignored rows are rows of zeros of G there.
 //
 // Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 68 % of the time at
 // 1.7 GHz in the statistics and in the products alike (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
@@ -598,7 +599,8 @@ __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, c
 
 // ----------------------------------------------------------------------------------------------- fp32: rows of a piece of logits
 struct HeadRows {
-    float *logits;         // [tokens][n], n classes from v0 on; G in their place
+    float *logits;         // [tokens][n], n classes from v0 on
+    float *g;              // G, there or somewhere else
     float2 *state;         // [tokens]: maximum (times log2 e) and sum of the pieces so far
     float *picked;         // [tokens]: the target's logit
     float *stats;
@@ -657,7 +659,8 @@ __global__ __launch_bounds__(256) void head_rows_grad_kernel(HeadRows p)
 {
     const int64_t row = blockIdx.x, c = p.sum.target[row];
     const bool counts = c != p.sum.ignore, known = c >= 0 && c < p.classes;
-    float *l = p.logits + row * p.n;
+    const float *l = p.logits + row * p.n;
+    float *out = p.g + row * p.n;
     const float lse = p.stats[row], f = !counts ? 0.0f : !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[row] : p.scale.value();
     const int label = known ? (int)(c - p.v0) : -1, begin = (int)blockIdx.y * p.columns, end = min(p.n, begin + p.columns);
     if (counts)
@@ -665,10 +668,10 @@ __global__ __launch_bounds__(256) void head_rows_grad_kernel(HeadRows p)
         for (int i = begin + (int)threadIdx.x; i < end; i += 256) {
             float v = expf(l[i] - lse);
             if (i == label) v -= 1.0f;
-            l[i] = v * f;
+            out[i] = v * f;
         }
     else
-        for (int i = begin + (int)threadIdx.x; i < end; i += 256) l[i] = 0.0f;
+        for (int i = begin + (int)threadIdx.x; i < end; i += 256) out[i] = 0.0f;
     if (p.xc && blockIdx.y == 0)
         for (int i = threadIdx.x; i < p.dim; i += 256) p.xc[row * p.dim + i] = counts ? p.x[row * p.ldx + i] : 0.0f;
 }
@@ -1155,7 +1158,7 @@ static int head_dx_f32(const HeadCall &c, float *dx, const float *g, int64_t v0,
     head_add_kernel<<<(unsigned)std::min<int64_t>(cdiv(count, 1024), 4096), 256, 0, c.s>>>(dx, to, count);
     return check_launch("head_add_kernel");
 }
-static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduction)
+static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, float *kept, int reduction)
 {
     const HeadPlan &h = c.h;
     HeadRows p = head_rows(c);
@@ -1163,6 +1166,7 @@ static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduct
     p.picked = c.at<float>(h.picked);
     p.stats = stats;
     p.sum = head_sum_of(c, loss, stats, reduction);
+    if (kept) p.logits = kept;
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
         if (int rc = head_logits_f32(c, p.logits, v0, n)) return rc;
@@ -1179,11 +1183,13 @@ static int head_fwd_f32(const HeadCall &c, float *loss, float *stats, int reduct
     head_loss_kernel<<<1, 1024, 0, c.s>>>(p.sum);
     return check_launch("head_loss_kernel");
 }
-static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dloss, const float *stats, int reduction)
+static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dloss, const float *stats, const float *kept, int reduction)
 {
     const HeadPlan &h = c.h;
     HeadRows p = head_rows(c);
     p.stats = const_cast<float *>(stats);
+    p.g = p.logits;
+    if (kept) p.logits = const_cast<float *>(kept);
     p.scale = {dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
     p.dloss = reduction == HD_NONE ? dloss : nullptr;
     p.x = static_cast<const float *>(c.x);
@@ -1191,7 +1197,8 @@ static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dl
     p.dim = (int)h.dim;
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
-        if (int rc = head_logits_f32(c, p.logits, v0, n)) return rc;
+        if (!kept)
+            if (int rc = head_logits_f32(c, p.logits, v0, n)) return rc;
         p.n = (int)n;
         p.v0 = (int)v0;
         p.xc = dw && i == 0 ? c.at<float>(h.xc) : nullptr;
@@ -1199,9 +1206,9 @@ static int head_bwd_f32(const HeadCall &c, float *dx, float *dw, const float *dl
         head_rows_grad_kernel<<<dim3((unsigned)h.tokens, (unsigned)cdiv(n, p.columns)), 256, 0, c.s>>>(p);
         if (int rc = check_launch("head_rows_grad_kernel")) return rc;
         if (dx)
-            if (int rc = head_dx_f32(c, dx, p.logits, v0, n, i > 0)) return rc;
+            if (int rc = head_dx_f32(c, dx, p.g, v0, n, i > 0)) return rc;
         if (dw)
-            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.logits, n, 1, c.at<float>(h.xc), h.dim, 1, nullptr, n, h.dim, h.tokens, c.at<void>(h.product), h.product_bytes, c.s)) return rc;
+            if (int rc = rdb_product_f32(dw + v0 * h.dim, p.g, n, 1, c.at<float>(h.xc), h.dim, 1, nullptr, n, h.dim, h.tokens, c.at<void>(h.product), h.product_bytes, c.s)) return rc;
     }
     return RDB_OK;
 }
@@ -1237,7 +1244,16 @@ extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int6
     return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward != 0, want_dx != 0, want_dw != 0).total;
 }
 
-extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
+// A product less in a backward pass that few tokens leave bound by the weight: us a step, computed again | kept: 12 tokens x 2048 -> 47643 407 | 306, 69 x 2723 -> 55040 1107 | 862,
+// 259 x 3136 -> 96128 5000 | 3960.
+extern "C" int64_t rdb_linear_cross_entropy_keeps(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw)
+{
+    if (check_head("rdb_linear_cross_entropy_keeps", tokens, dim, classes, dtype, dim, ldw, 0)) return 0;
+    if (dtype != RDB_F32 || 4 * tokens > dim) return 0;
+    return head_plan(tokens, dim, classes, dtype, ldw, true, true, true, false, false).pieces == 1 ? tokens * classes : 0;
+}
+
+extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
                                             int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace, int64_t workspace_bytes,
                                             void *stream)
 {
@@ -1246,11 +1262,12 @@ extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, const voi
     if (!loss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
     const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, false, false, false);
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
+    if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
-    return dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, reduction) : head_fwd_bf16(c, loss, stats, reduction);
+    return dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, logits, reduction) : head_fwd_bf16(c, loss, stats, reduction);
 }
 
-extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
+extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
                                             const int64_t *target, int64_t tokens, int64_t dim, int64_t classes, int64_t ignore_index, int reduction, void *workspace,
                                             int64_t workspace_bytes, void *stream)
 {
@@ -1261,7 +1278,8 @@ extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dlo
     if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return set_error(RDB_E_ALIGN, "%s: dx and dw must be 16-byte aligned", who);
     const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, true, dx != nullptr, dw != nullptr);
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
+    if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
-    return dtype == RDB_F32 ? head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, reduction)
+    return dtype == RDB_F32 ? head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, logits, reduction)
                             : head_bwd_bf16(c, static_cast<bf16_t *>(dx), static_cast<bf16_t *>(dw), dloss, stats, reduction);
 }

@@ -1134,18 +1134,20 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const c10::OptionalDeviceGuard guard(x.device());
         const int64_t tokens = x.size(0), dim = x.size(1), classes = w.size(0);
         const auto f32 = x.options().dtype(at::kFloat);
-        Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32);
+        Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32), logits;
         if (tokens) {
             const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), 0, 0, 0);
             const Tensor ws = bytes(need, x);
-            check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), ld(x), w.data_ptr(), ld(w), code(x.scalar_type()),
+            if (const int64_t n = x0.requires_grad() || w0.requires_grad() ? rdb_linear_cross_entropy_keeps(tokens, dim, classes, code(x.scalar_type()), ld(w)) : 0)
+                logits = at::empty({n}, f32);
+            check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), static_cast<float *>(ptr(logits)), x.data_ptr(), ld(x), w.data_ptr(), ld(w), code(x.scalar_type()),
                                                target.data_ptr<int64_t>(), tokens, dim, classes, ignore, (int)reduction, ptr(ws), need, stream_of(x)),
                   "rdb_linear_cross_entropy_fwd");
         } else {
             loss.fill_(reduction == 1 ? NAN : 0.0f);
         }
-        ctx->save_for_backward({x0, w0, target, stats});
-        ctx->saved_data["m"] = std::vector<int64_t>{tokens, dim, classes, ignore, reduction};
+        ctx->save_for_backward({x0, w0, target, stats, logits});
+        ctx->saved_data["m"] = std::vector<int64_t>{tokens, dim, classes, ignore, reduction, logits.defined()};
         return loss;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads)
@@ -1158,13 +1160,15 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
     {
         const at::AutoGradMode no_grad(false);
         const auto saved = ctx->get_saved_variables();
-        const auto m = ctx->saved_data["m"].toIntVector();   // tokens, dim, classes, ignored label, reduction
+        const auto m = ctx->saved_data["m"].toIntVector();   // tokens, dim, classes, ignored label, reduction, logits kept
         constexpr const char *who = "linear_cross_entropy (backward)";
         const Tensor dloss = grad.to(at::kFloat).contiguous();
         const Tensor x = rows(restored(who, saved[0], dloss, {m[0], m[1]}), true), w = rows(restored(who, saved[1], dloss, {m[2], m[1]}));
         if (!readable(x.scalar_type()) || x.scalar_type() != w.scalar_type()) fail(PyExc_RuntimeError, std::string(who) + ": a saved tensor came back as something else");
         restored_values(who, saved[2], dloss, at::kLong, m[0]);
         restored_values(who, saved[3], dloss, at::kFloat, m[0] + 1);
+        if (m[5]) restored_values(who, saved[4], dloss, at::kFloat, m[0] * m[2]);
+        const bool kept = m[5] && rdb_linear_cross_entropy_keeps(m[0], m[1], m[2], code(x.scalar_type()), ld(w));   // not of a weight that came back with longer rows
         const c10::OptionalDeviceGuard guard(x.device());
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         Tensor dx, dw;
@@ -1173,7 +1177,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         if (m[0] && (want_x || want_w)) {
             const int64_t need = rdb_linear_cross_entropy_workspace_bytes(m[0], m[1], m[2], code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), 1, want_x, want_w);
             const Tensor ws = bytes(need, x);
-            check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), x.data_ptr(), ld(x), w.data_ptr(), ld(w),
+            check(rdb_linear_cross_entropy_bwd(ptr(dx), ptr(dw), dloss.data_ptr<float>(), saved[3].data_ptr<float>(), kept ? saved[4].data_ptr<float>() : nullptr, x.data_ptr(), ld(x), w.data_ptr(), ld(w),
                                                code(x.scalar_type()), saved[2].data_ptr<int64_t>(), m[0], m[1], m[2], m[3], (int)m[4], ptr(ws), need, stream_of(x)),
                   "rdb_linear_cross_entropy_bwd");
         }

@@ -101,8 +101,8 @@ class RT_GPTConfig:
     # True: the token embedding and the output head are random-backed too, as in the reference's model
     # (modded-nanogpt/gpt_models.py:303, 310); they then draw the first and the last (k, seed) of the generators
     random_embedding_and_head: bool = False
-    # True: the loss comes from the head's input and weight (or coefficients), on the GPU, without the logits ever being in memory, and without
-    # their rounding to bf16
+    # True: the loss comes from the head's input and weight (or coefficients), on the GPU, without the logits being in memory
+    # (ops.linear_cross_entropy), and without their rounding to bf16
     loss_without_logits: bool = False
     # further arguments of Rotary (interleaved, rotary_dim, base, scaling, factor, ...)
     rotary: Optional[dict] = None

@@ -893,7 +893,7 @@ def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torc
     with _on(dev):
         n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), _ld(x), _p(w), _ld(w), 0, 0, 0))
         ws = _workspace(n, dev)
-        rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
+        rc = L.rdb_linear_cross_entropy_fwd(_p(loss), _p(stats), None, _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0], ignore_index, reduction,
                                             _p(ws), n, _stream(dev))
     _lib.check(rc, "rdb_linear_cross_entropy_fwd")
     return loss, stats
@@ -915,7 +915,7 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
     with _on(dev):
         n = int(L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, w.shape[0], _DT[x.dtype], _p(x), _ld(x), _p(w), _ld(w), 1, want_dx, want_dw))
         ws = _workspace(n, dev)
-        rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
+        rc = L.rdb_linear_cross_entropy_bwd(_p(dx), _p(dw), _p(d), _p(stats), None, _p(x), _ld(x), _p(w), _ld(w), _DT[x.dtype], _p(t), tokens, dim, w.shape[0],
                                             ignore_index, reduction, _p(ws), n, _stream(dev))
     _lib.check(rc, "rdb_linear_cross_entropy_bwd")
     return dx, dw

@@ -9,7 +9,7 @@ Additive to the reference surface:
 * ``materialize_bwd`` takes an optional ``coef_rows``;
 * ``rten::linear_fwd`` / ``linear_bwd_dx`` / ``linear_bwd_dcoef``: the fused products that never write the
   weight (or its gradient) to memory;
-* :func:`linear_cross_entropy` and :func:`rotary`: the loss of a language model's output head, whose logits are never kept, and rotary
+* :func:`linear_cross_entropy` and :func:`rotary`: the loss of a language model's output head, formed in pieces of its logits, and rotary
   positions in the layouts and with the frequencies of such models.
 """
 from __future__ import annotations
@@ -540,10 +540,11 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
     """``F.cross_entropy(F.linear(x, weight).float(), target, ignore_index=..., reduction=...)`` for a large vocabulary, with its gradients and without
-    the logits: neither they nor their gradient are ever in memory beyond a piece of the vocabulary.
+    the logits: neither they nor their gradient are ever in memory beyond a piece of the vocabulary (fp32 of up to dim / 4 tokens keeps up to 256 MB of them from
+    the forward to the backward pass).
 
     ``x`` (..., dim) and ``weight`` (classes, dim): both bf16 or both fp32, on one GPU; ``target`` (...): int64 or int32.  The loss is fp32; logits are
-    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out of the work: what their rows hold does not matter.  The mean over no tokens is
+    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out, in bf16 before anything is multiplied: what their rows hold does not matter.  The mean over no tokens is
     NaN, with gradients of zero; a target outside the classes makes its token's loss and gradients NaN.  First derivatives only."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")

@@ -108,11 +108,11 @@ def test_the_library_refuses():
     assert size(8, 64, 100, _lib.RDB_BF16, one, 64, one, 64, 0, 0, 0) > 0
     assert size(8, 64, 100, 7, one, 64, one, 64, 0, 0, 0) == 0 and size(0, 64, 100, 1, one, 64, one, 64, 0, 0, 0) == 0
     assert size(1 << 20, 1 << 10, 100, 1, one, 1 << 10, one, 1 << 10, 0, 0, 0) == 0
-    fwd = lambda **k: L.rdb_linear_cross_entropy_fwd(*{**dict(loss=one, stats=one, x=one, ldx=64, w=one, ldw=64, dtype=1, target=one, tokens=8, dim=64, classes=100,  # noqa: E731
+    fwd = lambda **k: L.rdb_linear_cross_entropy_fwd(*{**dict(loss=one, stats=one, logits=None, x=one, ldx=64, w=one, ldw=64, dtype=1, target=one, tokens=8, dim=64, classes=100,  # noqa: E731
                                                              ignore=-100, reduction=1, ws=one, n=0, stream=None), **k}.values())
     assert fwd() == -6 and fwd(dtype=2) == -3 and fwd(tokens=0) == -2 and fwd(dim=0) == -2 and fwd(classes=0) == -2 and fwd(ldx=63) == -2 and fwd(ldw=63) == -2
     assert fwd(reduction=3) == -2 and fwd(loss=None) == -1 and fwd(ws=None, n=1 << 40) == -6 and fwd(ldw=1 << 20) == -5 and fwd(tokens=1 << 23) == -5
-    bwd = lambda **k: L.rdb_linear_cross_entropy_bwd(*{**dict(dx=one, dw=one, dloss=one, stats=one, x=one, ldx=64, w=one, ldw=64, dtype=1, target=one, tokens=8, dim=64,  # noqa: E731
+    bwd = lambda **k: L.rdb_linear_cross_entropy_bwd(*{**dict(dx=one, dw=one, dloss=one, stats=one, logits=None, x=one, ldx=64, w=one, ldw=64, dtype=1, target=one, tokens=8, dim=64,  # noqa: E731
                                                              classes=100, ignore=-100, reduction=1, ws=one, n=0, stream=None), **k}.values())
     assert bwd() == -6 and bwd(dx=None, dw=None) == 0 and bwd(dx=one + 2) == -4 and bwd(dloss=None) == -1 and bwd(reduction=-1) == -2
     rows = lambda heads=2: _lib.ctypes.byref(_lib.RotaryRows(one, one, heads, 64, 64, 16))  # noqa: E731
@@ -128,5 +128,15 @@ def test_more_logits_than_a_launch_has_threads_are_refused():
     sizes = ((1 << 21) - 1, 8, 1 << 30)
     for tokens, dim, classes in (sizes, (1 << 20, 8, 1 << 18)):
         assert L.rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, _lib.RDB_BF16, 4096, 8, 4096, 8, 0, 0, 0) == 0
-        assert L.rdb_linear_cross_entropy_fwd(4096, 4096, 4096, 8, 4096, 8, _lib.RDB_BF16, 4096, tokens, dim, classes, -100, 1, 4096, 1 << 62, None) == -5
+        assert L.rdb_linear_cross_entropy_fwd(4096, 4096, None, 4096, 8, 4096, 8, _lib.RDB_BF16, 4096, tokens, dim, classes, -100, 1, 4096, 1 << 62, None) == -5
     assert L.rdb_linear_cross_entropy_workspace_bytes((1 << 20) - 128, 8, 1 << 18, _lib.RDB_BF16, 4096, 8, 4096, 8, 0, 0, 0) > 0
+
+
+def test_logits_that_are_kept():
+    """fp32, few beside the weight and in one piece; others are refused."""
+    L = _lib.load()
+    keeps = lambda tokens, dim, classes, dtype=_lib.RDB_F32, ldw=0: L.rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw or dim)  # noqa: E731
+    assert keeps(16, 64, 1000) == 16000 and keeps(17, 64, 1000) == 0 and keeps(16, 64, 1000, _lib.RDB_BF16) == 0 and keeps(0, 64, 1000) == 0
+    assert keeps(512, 2048, 1 << 17) == 1 << 26 and keeps(512, 2048, 1 << 18) == 0 and keeps(16, 64, 100000, ldw=1 << 19) == 0
+    sizes = 4096, 64, 4096, 64, _lib.RDB_F32, 4096, 17, 64, 1000, -100, 1, 4096, 1 << 40, None
+    assert L.rdb_linear_cross_entropy_fwd(4096, 4096, 4096, *sizes) == -5 and L.rdb_linear_cross_entropy_bwd(4096, 4096, 4096, 4096, 4096, *sizes) == -5

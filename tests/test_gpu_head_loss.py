@@ -319,3 +319,18 @@ def test_few_tokens_in_fp32(tokens, dim, classes):
         for a, b in ((x, w), (wide_x[:, 1:dim + 1], wide_w[:, :dim])):
             loss, dloss, dx, dw = both(a, b, t, reduction)
             check(x, w, t, reduction, loss, dloss, dx, dw)
+
+
+@pytest.mark.parametrize("tokens,dim,classes", [(7, 64, 3000), (70, 333, 5001), (200, 1024, 2000)])
+def test_kept_logits_give_the_same_bits(tokens, dim, classes):
+    """The operators compute them again; a second backward pass through the same graph finds them as they were."""
+    x, w, t = inputs(tokens, dim, classes, torch.float32, tokens, 0.3)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    again, _ = torch.ops.rten.linear_cross_entropy_fwd(a, b, t, IGNORED, 1)
+    want = torch.autograd.grad(again, [a, b])
+    kept = ops.linear_cross_entropy(a, b, t, IGNORED)
+    assert torch.equal(kept, again)
+    for _ in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(kept, [a, b], retain_graph=True)))
+    one = torch.autograd.grad(ops.linear_cross_entropy(a, w, t, IGNORED), a)[0]
+    assert torch.equal(one, want[0])
