@@ -768,13 +768,13 @@ __global__ __launch_bounds__(256, 2) void head_few_dx_kernel(HeadFew p)
     __shared__ float sums[HS_T][128 + 4];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, d0 = (int)blockIdx.x * 128, d = d0 + r * 4;
     const int begin = (int)blockIdx.y * p.range, end = min(p.classes, begin + p.range), left = p.dim - d;
-    const float *w = p.w + (left > 0 ? d : 0), *x = p.x + (int64_t)min(r, p.tokens - 1) * p.ldx;   // columns behind the last are nobody's
+    const float *w = p.w + d, *x = p.x + (int64_t)min(r, p.tokens - 1) * p.ldx;   // columns behind the last are not read
     f32x16 acc[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = zero16();
     f32x4 a[2][4], b[2];
     auto load = [&](int i, int v) {
-        const bool whole = v + 8 <= end, columns = whole && p.dim % 4 == 0;
+        const bool whole = v + 8 <= end, columns = whole && left >= 4;
         v += g * 4;
 #pragma unroll
         for (int s = 0; s < 4; ++s) a[i][s] = head_load4(w + (int64_t)min(v + s, p.classes - 1) * p.ldw, v + s < end ? left : 0, columns);

@@ -334,3 +334,35 @@ def test_kept_logits_give_the_same_bits(tokens, dim, classes):
         assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(kept, [a, b], retain_graph=True)))
     one = torch.autograd.grad(ops.linear_cross_entropy(a, w, t, IGNORED), a)[0]
     assert torch.equal(one, want[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_few_tokens_in_a_graph(dtype):
+    """The forms for few tokens, logits that are kept among them: captured once, replayed with other inputs and eager calls in between; and on two streams at once."""
+    x, w, t = inputs(24, 256, 3001, dtype, 41, 0.2)
+    sx, sw, st, dloss = x.clone().requires_grad_(), w.clone().requires_grad_(), t.clone(), torch.tensor(0.5, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.linear_cross_entropy(sx, sw, st, IGNORED), [sx, sw], dloss)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = ops.linear_cross_entropy(sx, sw, st, IGNORED)
+        grads = torch.autograd.grad(loss, [sx, sw], dloss)
+    for seed in (42, 43, 44):
+        nx, nw, nt = inputs(24, 256, 3001, dtype, seed, 0.3 * (seed - 42))
+        with torch.no_grad():
+            sx.copy_(nx), sw.copy_(nw), st.copy_(nt)
+        eager = both(nx, nw, nt, "mean", dloss)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, eager[0]) and torch.equal(grads[0], eager[2]) and torch.equal(grads[1], eager[3])
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(4):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            got.append(both(nx, nw, nt, "mean", dloss))
+    torch.cuda.synchronize()
+    for other in got:
+        assert all(torch.equal(a, b) for a, b in zip(eager, other))
