@@ -1118,6 +1118,28 @@ class CausalAttention : public Function<CausalAttention> {
 };
 
 // ----------------------------------------------------------------------------------------------- ends of a language model
+// A leaf's gradient goes to its accumulator on the stream on which that was made, and a capture under way would take in that stream and could not end: the process would.  So
+// an accumulator that an older graph keeps alive, made on a stream outside of the capture, is refused.
+void no_leaves_outside_capture(const char *who, const Tensor &grad)
+{
+    const auto here = c10::hip::getCurrentHIPStream(grad.get_device());
+    auto capturing = [](hipStream_t s) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;   // the default stream never is
+    };
+    if (!capturing(here.stream())) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const auto &edge : node->next_edges()) {
+        if (!edge.function || edge.function->name() != "torch::autograd::AccumulateGrad") continue;
+        const auto there = edge.function->stream();   // its device is called by the other name that autograd has for it
+        if (!there || (there->id() == here.id() && there->device_index() == here.device_index())) continue;
+        if (!capturing(c10::hip::HIPStream(c10::Stream(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, there->device_index()), there->id())).stream()))
+            fail(PyExc_RuntimeError, std::string(who) + ": captured while an earlier graph of the same leaf, made on another stream, is alive: drop what holds it (a loss, an output), or "
+                                                        "make it on the capturing stream");
+    }
+}
+
 // loss of x (tokens, dim) against a weight (classes, dim) that never become logits; the argument checks are ops.linear_cross_entropy's
 class LinearCrossEntropy : public Function<LinearCrossEntropy> {
   public:
@@ -1162,6 +1184,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const auto saved = ctx->get_saved_variables();
         const auto m = ctx->saved_data["m"].toIntVector();   // tokens, dim, classes, ignored label, reduction, logits kept
         constexpr const char *who = "linear_cross_entropy (backward)";
+        no_leaves_outside_capture(who, grad);
         const Tensor dloss = grad.to(at::kFloat).contiguous();
         const Tensor x = rows(restored(who, saved[0], dloss, {m[0], m[1]}), true), w = rows(restored(who, saved[1], dloss, {m[2], m[1]}));
         if (!readable(x.scalar_type()) || x.scalar_type() != w.scalar_type()) fail(PyExc_RuntimeError, std::string(who) + ": a saved tensor came back as something else");
@@ -1218,6 +1241,7 @@ class Rotary : public Function<Rotary> {
         const Tensor &some = grads[0].defined() ? grads[0] : keys ? grads[1] : grads[0];
         if (!some.defined()) return variable_list(7);
         constexpr const char *who = "rotary (backward)";
+        no_leaves_outside_capture(who, some);
         restored_values(who, saved[0], some, at::kFloat, m[9]);
         const Tensor &pos = saved[1];
         if (m[10]) {

@@ -1,6 +1,9 @@
 """ops.linear_cross_entropy against its formula in 64 bits, value by value, with bounds that count the roundings: a logit is a sum of ``dim`` products in fp32, a value of the
 softmax is off by its logit's error, and a gradient is a sum of such values (in bf16: rounded once more each) times the other factor."""
 import math
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -366,3 +369,39 @@ def test_few_tokens_in_a_graph(dtype):
     torch.cuda.synchronize()
     for other in got:
         assert all(torch.equal(a, b) for a, b in zip(eager, other))
+
+
+CAPTURE = """
+import torch
+from randumb_amd import ops
+x, w, t = torch.randn(24, 64, device="cuda"), torch.randn(300, 64, device="cuda"), torch.randint(0, 300, (24,), device="cuda")
+q, freq = torch.randn(2, 5, 3, 8, device="cuda"), ops.rotary_frequencies(8, device="cuda")[0]
+for leaves, call in (([x, w], lambda: ops.linear_cross_entropy(x, w, t)), ([q], lambda: ops.rotary(q, None, freq)[0].square().sum())):
+    for leaf in leaves:
+        leaf.requires_grad_()
+    held = call()
+    want = torch.autograd.grad(held, leaves, retain_graph=True)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(call(), leaves)
+    except RuntimeError as e:
+        assert "an earlier graph of the same leaf" in str(e), e
+        print("refused", flush=True)
+    torch.cuda.synchronize()
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaves)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    print("captured", flush=True)
+"""
+
+
+def test_a_capture_beside_an_older_graph_of_the_same_leaves():
+    """Refused, where it would end the process; without the older graph it is captured.  In a process of its own."""
+    done = subprocess.run([sys.executable, "-c", CAPTURE], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.split() == ["refused", "captured"] * 2, (done.returncode, done.stdout, done.stderr[-2000:])
