@@ -75,6 +75,7 @@ class Rotary(nn.Module):
                 raise ValueError(f"Rotary: between 2 and {dim} values of a head, got {rotary_dim}")
             freq, self.scale = ops.rotary_frequencies(dim if rotary_dim is None else rotary_dim, base, **scaling)
             self.register_buffer("freq_bits", freq.view(torch.int32), persistent=False)   # as whole numbers: a module's change of type leaves them alone
+            self.register_buffer("no_turn", torch.zeros(dim // 2), persistent=False)      # frequencies of what is turned already
 
     def both(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None):
         """Queries and keys (or None) in one launch."""
@@ -134,8 +135,15 @@ class RT_CausalSelfAttention(nn.Module):
         qkv = self.c_qkv(x)
         ext = _fused(qkv)
         stock = getattr(self.rotary, "stock", True)   # somebody's own rotation is called with one side at a time
-        if ext is not None and stock and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
-            y = ext.causal_attention(qkv, self.rotary.inv_freq, self.n_head, _EPS)
+        # q and k that turn without becoming longer may do so before they are normalised as well as behind: the kernel that normalises them then has nothing to turn
+        turned = not stock and type(self.rotary) is Rotary and self.rotary.scale == 1.0
+        if ext is not None and (stock or turned) and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
+            if turned:
+                q, k, v = qkv.split(D, 2)
+                q, k = self.rotary.both(q.view(B, T, self.n_head, 64), k.view(B, T, self.n_head, 64))
+                y = ext.causal_attention(torch.cat((q.view(B, T, D), k.view(B, T, D), v), 2), self.rotary.no_turn, self.n_head, _EPS)
+            else:
+                y = ext.causal_attention(qkv, self.rotary.inv_freq, self.n_head, _EPS)
             if y is not None:
                 return self.c_proj(y)
         q, k, v = qkv.view(B, T, 3, self.n_head, D // self.n_head).unbind(2)

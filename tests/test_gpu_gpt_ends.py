@@ -93,6 +93,22 @@ def test_training_step_in_bf16(random_head):
             assert p.grad.dtype == torch.bfloat16 and rel(p.grad, q.grad) < 0.05, name
 
 
+@pytest.mark.parametrize("rotary", [{"interleaved": True}, {"rotary_dim": 32, "scaling": "linear", "factor": 4.0}, {"scaling": "parts", "factor": 4.0, "original_context": 512}])
+def test_attention_of_what_is_turned_already(monkeypatch, rotary):
+    """bf16: attention's own kernels behind the rotation (of the length that they were: the last one is not) against the stock operators, both by their distance from fp32: q and k
+    are rounded once more, every other rounding has its counterpart."""
+    idx, target = batch()
+    model, stock, exact = (make(torch.bfloat16, rotary=rotary) for _ in range(3))
+    exact = exact.float()
+    for m in (model, exact):
+        m(idx, target).backward()
+    monkeypatch.setattr(gpt, "_fused", lambda x: None)
+    stock(idx, target).backward()
+    for (name, p), (_, q), (_, e) in zip(*(m.named_parameters() for m in (model, stock, exact))):
+        if e.grad is not None:
+            assert rel(p.grad, e.grad) < 2 * rel(q.grad, e.grad) + 2.0**-8, name
+
+
 def test_types_devices_and_states():
     """The frequencies survive a change of the module's type, and neither they nor the identity are in its state."""
     model = make(torch.bfloat16, True, rotary={"rotary_dim": 20}, loss_without_logits=True)
