@@ -1585,7 +1585,7 @@ PyObject *py_rotary(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (interleaved < 0) throw BadArgument();
         if (q.dim() != 4 || !readable(q.scalar_type()) || (k && (k->dim() != 4 || k->scalar_type() != q.scalar_type() || k->size(0) != q.size(0) || k->size(1) != q.size(1) ||
                                                                   k->size(3) != q.size(3))) ||
-            f.dim() != 1 || f.scalar_type() != at::kFloat || 2 * f.numel() > q.size(3) ||
+            f.dim() != 1 || f.scalar_type() != at::kFloat || !f.numel() || f.numel() > 1024 || 2 * f.numel() > q.size(3) ||
             (pos && ((pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt) || pos->dim() < 1 || pos->dim() > 2 || pos->size(-1) != q.size(1) ||
                      (pos->dim() == 2 && pos->size(0) != 1 && pos->size(0) != q.size(0)))))
             fail(PyExc_ValueError, "rotary needs queries and keys (batch, time, heads, head_dim) of one type, fp32 frequencies and positions (time) or (batch, time)");

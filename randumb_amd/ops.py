@@ -593,14 +593,7 @@ def _rotary_backward(ctx, grads):
 _rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup_context)
 
 
-def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional[Tensor] = None, *, interleaved: bool = False, scale: float = 1.0):
-    """Queries (batch, time, heads, head_dim) and keys (batch, time, kv_heads, head_dim), or queries alone (``k`` None), turned by their positions, in one
-    launch; returns both.  Of every head the first ``2 * len(inv_freq)`` values are pairs, value i with the one half of them
-    on, or neighbours (``interleaved``): ``(a, b) -> (a cos + b sin, b cos - a sin)``, the direction of :class:`randumb_amd.gpt.Rotary`, with the angle
-    ``position * inv_freq[i]`` formed in 64 bits and cosine and sine times ``scale``; the rest passes through.
-
-    bf16 or fp32, any strides (unit inner ones are read in place), arithmetic in fp32, rounded once.  ``inv_freq``: fp32 (:func:`rotary_frequencies`).  ``positions``:
-    int64 or int32, (time,) or (batch, time), any integers; None: 0, 1, ...  Gradients of any order for q and k, none for the frequencies."""
+def _check_rotary(q, k, inv_freq, positions) -> None:
     if q.dtype not in (torch.float32, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
         raise TypeError(f"rotary: queries and keys both bfloat16 or both float32, got {q.dtype}" + ("" if k is None else f" and {k.dtype}"))
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
@@ -609,11 +602,25 @@ def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional
         raise ValueError(f"rotary: float32 frequencies, one for each pair of a head's {q.shape[3]} values (1024 at most), got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     if positions is not None and (positions.dtype not in (torch.int64, torch.int32) or positions.shape not in (q.shape[1:2], q.shape[:2], (1, q.shape[1]))):
         raise ValueError(f"rotary: positions int64 or int32 of shape (time,) or (batch, time), got {positions.dtype} {tuple(positions.shape)}")
-    scale = float(scale)
-    both = None
-    if not _tracing() and q.is_cuda:
-        both = (_lib._ext or _lib.extension()).rotary(q, k, inv_freq, positions, interleaved, scale)
+
+
+def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional[Tensor] = None, *, interleaved: bool = False, scale: float = 1.0):
+    """Queries (batch, time, heads, head_dim) and keys (batch, time, kv_heads, head_dim), or queries alone (``k`` None), turned by their positions, in one
+    launch; returns both.  Of every head the first ``2 * len(inv_freq)`` values are pairs, value i with the one half of them
+    on, or neighbours (``interleaved``): ``(a, b) -> (a cos + b sin, b cos - a sin)``, the direction of :class:`randumb_amd.gpt.Rotary`, with the angle
+    ``position * inv_freq[i]`` formed in 64 bits and cosine and sine times ``scale``; the rest passes through.
+
+    bf16 or fp32, any strides (unit inner ones are read in place), arithmetic in fp32, rounded once.  ``inv_freq``: fp32 (:func:`rotary_frequencies`).  ``positions``:
+    int64 or int32, (time,) or (batch, time), any integers; None: 0, 1, ...  Gradients of any order for q and k, none for the frequencies."""
+    scale, both = float(scale), None
+    if not _tracing() and isinstance(q, Tensor) and q.is_cuda:
+        try:   # which checks the same: 2 of the 9 us of a call go to saying what is wrong with it
+            both = (_lib._ext or _lib.extension()).rotary(q, k, inv_freq, positions, interleaved, scale)
+        except (TypeError, ValueError, RuntimeError):
+            _check_rotary(q, k, inv_freq, positions)
+            raise
     if both is None:
+        _check_rotary(q, k, inv_freq, positions)
         both = _rotary(q, k, inv_freq.detach(), positions, bool(interleaved), scale, False)
     return both[0], None if k is None else both[1]
 

@@ -168,3 +168,16 @@ def test_more_blocks_than_one_launch():
     out = ops.rotary(q, None, freq, pos)[0]
     for at in (slice(0, 40), slice((1 << 23) - 20, (1 << 23) + 20), slice((1 << 24) - 20, (1 << 24) + 5)):
         close(out[at], q[at], turned(q[at], freq, pos[at], False, 1.0), freq, False, 1.0)
+
+
+def test_refusals_on_the_gpu():
+    """The same errors as on the CPU, where the extension does not see the call."""
+    q, f = torch.randn(2, 3, 4, 8, device="cuda"), ops.rotary_frequencies(8, device="cuda")[0]
+    pos = torch.arange(3, device="cuda")
+    for error, args in [(TypeError, (q.half(), None, f)), (TypeError, (q, q.bfloat16(), f)), (ValueError, (q[0], None, f)), (ValueError, (q, q[:, :2], f)), (ValueError, (q, q[..., :4], f)),
+                        (ValueError, (q, None, f.double())), (ValueError, (q, None, f[:0])), (ValueError, (q, None, torch.cat([f, f]))), (ValueError, (q, None, f, pos.float())),
+                        (ValueError, (q, None, f, pos[:2])), (ValueError, (q, None, f, pos.expand(3, 3))), (ValueError, (q, None, f, pos[0]))]:
+        with pytest.raises(error, match="rotary: "):
+            ops.rotary(*args)
+    with pytest.raises(ValueError, match="1024 at most"):
+        ops.rotary(torch.randn(1, 1, 1, 2050, device="cuda"), None, torch.ones(1025, device="cuda"))
