@@ -555,15 +555,16 @@ int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const vo
 /* ------------------------------------------------------------------------------------------ ends of a language model
  * Softmax cross entropy of an output head in pieces of its logits: F.cross_entropy(F.linear(x, w), target) of modded-nanogpt/gpt_models.py's head and loss, x [tokens x dim]
  * and w [classes x dim] both of `dtype` (RDB_F32 or RDB_BF16) with unit inner stride, target int64.  Products, exponentials and sums in fp32 (bf16: on the matrix cores with fp32
- * sums; fp32: rdb_product_f32's).
+ * sums; fp32: at the accuracy of rdb_product_f32).
  *   reduction  0: loss[tokens] (0 where target == ignore_index); 1: loss[0], the mean over the other rows (NaN of none); 2: loss[0], their sum
  *   stats      tokens + 1 floats, for the backward call: log of every row's sum of exponentials, and (reductions 1 and 2) the number of rows that count
  * A target outside the classes makes its row's loss and gradients NaN.  Rows with target == ignore_index are not read.
  * Backward: dloss[tokens] for reduction 0, dloss[0] otherwise; dx [tokens x dim] and dw [classes x dim] contiguous, of `dtype`, overwritten,
  * 16-byte aligned, NULL where not wanted.  G = (softmax - onehot) is formed from the logits computed again, a piece of the vocabulary at
  * a time (bf16: rounded to bf16 without the factor that its rows share).  Sums in fixed orders: results are bitwise reproducible.
+ * fp32 of many tokens runs on the bf16 matrix cores in three planes, which take 1.5 times the weight's bytes of the workspace; an infinity in x or w is a NaN there.
  * The workspace's size depends on where x and w begin.  RDB_E_UNSUPPORTED: x of 2^29 values or more, 2^21 rows or more, ldw of 2^20 or more,
- * 2^38 bf16 logits or more in tiles of 128 x 256 (size query: 0). */
+ * 2^38 logits or more in tiles of 128 x 256 (size query: 0). */
 int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
                                                  int backward, int want_dx, int want_dw);
 /* Floats of the logits that a forward call leaves for the backward call, where both are given a buffer of them (NULL: none), in fp32: of up to dim / 4

@@ -73,6 +73,27 @@ template <int ROWS, int LAYOUT> struct DuoOperand {
     }
 };
 
+// The same of an fp32 matrix in three bf16 planes beside each other in its rows (h + m + l of fg_split3, `plane` values apart): the six products of the planes that make an fp32
+// one, one after the other, the small ones first.  SIDE 0: A, 1: B of (m m) (l h) (h l) (m h) (h m) (h h).  set() with the whole row, plane 0 first.
+template <int ROWS, int LAYOUT, int SIDE> struct DuoPlanes : DuoOperand<ROWS, LAYOUT> {
+    int stages;       // of a plane
+    uint32_t plane;   // bytes
+    __device__ __forceinline__ void set(const bf16_t *src, int64_t ld, int row0, int rows, int k, int plane_values)
+    {
+        DuoOperand<ROWS, LAYOUT>::set(src, ld, row0, rows, k);
+        // all of the last row is in the matrix
+        this->rsrc[2] = __builtin_amdgcn_readfirstlane((int)((LAYOUT == K_CONT ? (int64_t)max(rows, 0) * ld : (int64_t)max(k, 0) * ld) * 2));
+        stages = max(1, (k + DUO_K - 1) / DUO_K);
+        plane = (uint32_t)plane_values * 2u;
+    }
+    __device__ __forceinline__ uint32_t stage(int s) const
+    {
+        const int pair = s / stages;
+        const uint32_t at = DuoOperand<ROWS, LAYOUT>::stage(s - pair * stages), which = ((SIDE ? 0x121u : 0x49u) >> (2 * min(pair, 6))) & 3u;
+        return at + which * plane;
+    }
+};
+
 __device__ __forceinline__ uint32_t duo_lds_address(const bf16_t *p)
 {
     return __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const bf16_t __attribute__((address_space(3))) *)p);

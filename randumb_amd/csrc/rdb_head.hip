@@ -7,7 +7,7 @@
 // Rows whose target is the ignored label are left out before anything is multiplied (head_gather_kernel): they cost nothing, and what they hold, NaN
 // included, reaches no sum.  A target outside the classes makes its row NaN.
 //
-// bf16 (products on the tiles of rdb_duo.hpp, of few tokens on those of rdb_gemm.hpp):
+// On the tiles of rdb_duo.hpp (bf16; of few tokens on those of rdb_gemm.hpp; fp32 in three bf16 planes, where that is faster):
 //   head_gather_kernel      the rows that count, one after the other, in rows of a multiple of 8 values
 //   head_logits_duo_kernel  a tile of logits in the accumulators -> its maximum and its sum of exponentials for each token; or (backward), a piece of the
 //   head_logits_solo_kernel vocabulary's logits once more -> G, in bf16, for the next launch
@@ -17,7 +17,7 @@
 //   head_dx_kernel          dx from its sums, back in the rows' own places
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
 // which are nearly all of the gradient, would all be off by the same rounding.
-// fp32: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between, which of few tokens stay for the
+// fp32 otherwise: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between, which of few tokens stay for the
 // backward pass (rdb_linear_cross_entropy_keeps); ignored rows are rows of zeros of G there.
 //
 // Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 68 % of the time at
@@ -25,6 +25,7 @@
 // priority for the main loop all change nothing.  Measured there, us: statistics 540 - 640, by the card (1172 - 990 TFLOP/s; the library's product alone 656), backward 1700 (three
 // products, 1900 GFLOP), a step 2310; 8192 x 256 -> 50304 1030; 4096 x 4096 -> 65536 7080 (four products, 1240 TFLOP/s).
 #include "rdb_duo.hpp"
+#include "rdb_f32.hpp"
 #include <algorithm>
 
 namespace rdb {
@@ -38,8 +39,8 @@ enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
 
 // ----------------------------------------------------------------------------------------------- the rows that count
 struct HeadGather {
-    bf16_t *xc;              // [tokens][ldc]: the rows that count, in order, zeros behind their last values
-    const bf16_t *x;
+    bf16_t *xc;              // [tokens][ldc]: the rows that count, in order, zeros behind their last values; fp32: three planes of ldc / 3 (rdb_duo.hpp)
+    const void *x;
     int64_t ldx, ldc;
     const int64_t *target;
     int *pos;                // [tokens]: where a row went, -1: ignored
@@ -52,8 +53,34 @@ struct HeadGather {
     int64_t tokens, dim, classes, ignore;
     int rows;                // per block
 };
+__device__ __forceinline__ f32x4 head_load4(const float *p, int left, bool whole)
+{
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (whole) __builtin_memcpy(&v, p, 16);   // at any address
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) v[e] = p[e];
+    return v;
+}
+// 8 values, `left` of them there, into the planes
+__device__ __forceinline__ void head_split8(bf16_t *to, int plane, const float *from, int left)
+{
+    const f32x4 a = head_load4(from, left, left >= 4), b = head_load4(from + 4, left - 4, left >= 8);
+    u32x4 v[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t h, m, l;
+        fg_split3(e < 2 ? a[2 * e] : b[2 * e - 4], e < 2 ? a[2 * e + 1] : b[2 * e - 3], h, m, l);
+        v[0][e] = h;
+        v[1][e] = m;
+        v[2][e] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4 *>(to + i * plane) = v[i];
+}
 // Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.
-__device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
+template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
 {
     __shared__ int before_[4], place_[64];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
@@ -87,6 +114,15 @@ __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
         }
     }
     __syncthreads();
+    if constexpr (PLANES) {
+        const int plane = (int)(p.ldc / 3), chunks = plane / 8;
+        for (int i = t; i < mine * chunks; i += 256) {
+            const int row = i / chunks, col = (i - row * chunks) * 8, at = place_[row];
+            if (at >= 0) head_split8(p.xc + (int64_t)at * p.ldc + col, plane, static_cast<const float *>(p.x) + (r0 + row) * p.ldx + col, (int)p.dim - col);
+        }
+        return;
+    }
+    const bf16_t *x = static_cast<const bf16_t *>(p.x);
     // 8 values a lane, at any address; a ragged piece of the last row that there is, and rows of less than 8 values, one by one: 16 bytes would reach behind the last of them
     const int chunks = (int)(p.ldc / 8), dim = (int)p.dim, total = mine * chunks, whole = dim < 8 ? 0 : dim % 8 && r0 + mine == p.tokens ? total - 1 : total;
     for (int i0 = t; i0 < whole; i0 += 1024) {
@@ -95,7 +131,7 @@ __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int i = min(i0 + q * 256, whole - 1), row = i / chunks, col = (i - row * chunks) * 8, at = place_[row], left = dim - col;
-            __builtin_memcpy(&v[q], p.x + (r0 + row) * p.ldx + col, 16);
+            __builtin_memcpy(&v[q], x + (r0 + row) * p.ldx + col, 16);
             to[q] = at < 0 || i0 + q * 256 >= whole ? nullptr : p.xc + (int64_t)at * p.ldc + col;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[q][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
@@ -106,7 +142,7 @@ __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
     }
     for (int i = whole * 8 + t; i < total * 8; i += 256) {
         const int row = i / 8 / chunks, col = i - row * chunks * 8, at = place_[row];
-        if (at >= 0) p.xc[(int64_t)at * p.ldc + col] = col < dim ? p.x[(r0 + row) * p.ldx + col] : (bf16_t)0;
+        if (at >= 0) p.xc[(int64_t)at * p.ldc + col] = col < dim ? x[(r0 + row) * p.ldx + col] : (bf16_t)0;
     }
 }
 
@@ -114,14 +150,14 @@ __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
 // and writes them to a multiple of 16 bytes.  per_block: a multiple of 8, at most 8192 values; out of padded rows it reads up to 14 bytes behind the last of them.
 struct HeadRepack {
     bf16_t *dst;
-    const bf16_t *src;
+    const void *src;
     int64_t ld, rows;   // of src
     int cols, per_block, blocks;
 };
 template <bool PAD> __device__ __forceinline__ void head_repack_rows(const HeadRepack &p, int block)
 {
     const int64_t r0 = (int64_t)block * p.per_block, lds = p.ld;
-    const bf16_t *__restrict__ src = p.src;
+    const bf16_t *__restrict__ src = static_cast<const bf16_t *>(p.src);
     bf16_t *__restrict__ dst = p.dst;
     const int cols = p.cols, mine = p.rows - r0 < p.per_block ? (int)(p.rows - r0) : p.per_block, out_cols = PAD ? (cols + 7) & ~7 : cols, total = mine * out_cols;
     src += r0 * lds;
@@ -157,10 +193,22 @@ template <bool PAD> __device__ __forceinline__ void head_repack_rows(const HeadR
     }
 }
 // The rows that count and, where it needs one, the weight's copy, in one launch (three launches less with dW's, 1025 x 999 -> 10001: a step 136 -> 126.5 us).
-__global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p, HeadRepack w, int gathering)
+// PLANES: fp32, both into planes (50304 x 768: 60 us, 6.4 TB/s).
+template <bool PLANES> __global__ __launch_bounds__(256) void head_gather_kernel(HeadGather p, HeadRepack w, int gathering)
 {
-    if ((int)blockIdx.x < gathering) head_gather_rows(p, (int)blockIdx.x);
-    else head_repack_rows<true>(w, (int)blockIdx.x - gathering);
+    if ((int)blockIdx.x < gathering) return head_gather_rows<PLANES>(p, (int)blockIdx.x);
+    const int block = (int)blockIdx.x - gathering;
+    if constexpr (!PLANES) {
+        head_repack_rows<true>(w, block);
+    } else {
+        const int64_t r0 = (int64_t)block * w.per_block;
+        const int mine = w.rows - r0 < w.per_block ? (int)(w.rows - r0) : w.per_block, chunks = (w.cols + 7) / 8;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < mine * chunks; i += 256) {
+            const int row = i / chunks, col = (i - row * chunks) * 8;
+            head_split8(w.dst + (r0 + row) * chunks * 24 + col, chunks * 8, static_cast<const float *>(w.src) + (r0 + row) * w.ld + col, w.cols - col);
+        }
+    }
 }
 
 // ----------------------------------------------------------------------------------------------- logits, in the accumulators
@@ -176,6 +224,7 @@ struct HeadLogits {
     int64_t tokens;
     bf16_t *g;            // gradient: [tokens][ldg], class v0 first
     int64_t ldg;
+    int plane, plane_g;   // fp32: values from plane to plane of x and w, of g
     const float *lse2, *factor;
     const int *label;
 };
@@ -225,8 +274,8 @@ __device__ __forceinline__ void head_leave_stats(const f32x16 (&acc)[MI][NI], co
     }
 }
 
-// G of the tile, through LDS into whole rows; classes past the last one are zeros
-template <int MI, int NI>
+// G of the tile, through LDS into whole rows; classes past the last one are zeros.  PLANES: one plane after the other
+template <int MI, int NI, bool PLANES>
 __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *__restrict__ lds, const HeadLogits &p, int tv, int tok0, int count, int t)
 {
     constexpr int HALF = MI * 32, N = MI * 16, BM = MI * 64, BN = NI * 64, LD = BM + 8;
@@ -237,6 +286,23 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *_
         const int b = wn * NI * 32 + ni * 32 + r, tok = min(tok0 + b, count - 1);
         const float l = p.lse2[tok], f = p.factor[tok];
         const int rel = p.label[tok] - first;
+        if constexpr (PLANES) {   // in place
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i >> 4][ni][i & 15] = __builtin_amdgcn_exp2f(fmaf(acc[i >> 4][ni][i & 15], HD_LOG2E, -l));
+            if (__any((unsigned)rel < (unsigned)HALF)) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i >> 4][ni][i & 15] -= (i >> 4) * 32 + head_row(i & 15, g) == rel ? 1.0f : 0.0f;
+            }
+            if (left < HALF) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if ((i >> 4) * 32 + head_row(i & 15, g) >= left) acc[i >> 4][ni][i & 15] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i >> 4][ni][i & 15] *= f;
+            __builtin_amdgcn_sched_barrier(0);
+            continue;
+        }
         float v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(acc[i >> 4][ni][i & 15], HD_LOG2E, -l));
@@ -255,14 +321,34 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *_
             store4<bf16_t>(lds + b * LD + wm * HALF + (q >> 2) * 32 + 8 * (q & 3) + 4 * g, v[q * 4] * f, v[q * 4 + 1] * f, v[q * 4 + 2] * f, v[q * 4 + 3] * f);
         __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
-    constexpr int LPR = BM / 8, RPP = 256 / LPR;   // lanes a row, rows at once
-    bf16_t *out = p.g + (int64_t)tok0 * p.ldg + (int64_t)tv * BM;
-    const int a = (t % LPR) * 8;
-#pragma unroll 8
-    for (int q = 0; q < BN / RPP; ++q) {
-        const int b = q * RPP + t / LPR;
-        if (tok0 + b < count) *reinterpret_cast<f32x4 *>(out + (int64_t)b * p.ldg + a) = *reinterpret_cast<const f32x4 *>(lds + b * LD + a);
+#pragma unroll 1
+    for (int plane = 0; plane < (PLANES ? 3 : 1); ++plane) {
+        if constexpr (PLANES) {
+            if (plane) __syncthreads();   // the one before is out of LDS
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                for (int q = 0; q < MI * 4; ++q) {
+                    f32x16 &c = acc[q >> 2][ni];
+                    const int j = (q & 3) * 4;
+                    const uint32_t lo = f32x2_to_bf16x2(c[j], c[j + 1]), hi = f32x2_to_bf16x2(c[j + 2], c[j + 3]);
+                    *reinterpret_cast<uint2 *>(lds + (wn * NI * 32 + ni * 32 + r) * LD + wm * HALF + (q >> 2) * 32 + 8 * (q & 3) + 4 * g) = uint2{lo, hi};
+                    c[j] -= __uint_as_float(lo << 16);
+                    c[j + 1] -= __uint_as_float(lo & 0xffff0000u);
+                    c[j + 2] -= __uint_as_float(hi << 16);
+                    c[j + 3] -= __uint_as_float(hi & 0xffff0000u);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+        __syncthreads();
+        constexpr int LPR = BM / 8, RPP = 256 / LPR;   // lanes a row, rows at once
+        bf16_t *out = p.g + (int64_t)tok0 * p.ldg + (int64_t)tv * BM + plane * p.plane_g;
+        const int a = (t % LPR) * 8;
+#pragma unroll PLANES ? 2 : 8
+        for (int q = 0; q < BN / RPP; ++q) {
+            const int b = q * RPP + t / LPR;
+            if (tok0 + b < count) *reinterpret_cast<f32x4 *>(out + (int64_t)b * p.ldg + a) = *reinterpret_cast<const f32x4 *>(lds + b * LD + a);
+        }
     }
 }
 
@@ -293,7 +379,7 @@ template <bool GRAD, int HF_V> __global__ __launch_bounds__(256, 2) void head_lo
         for (int mi = 0; mi < MI; ++mi) acc[mi][0] = zero16();
         gemm_mainloop<HF_V, HF_T, 64, AHEAD, AHEAD>(acc, lds, pa, pb, 0, (p.dim + 63) / 64);
         if constexpr (GRAD) {
-            head_leave_grad<MI, 1>(acc, lds, p, tv, 0, count, t);
+            head_leave_grad<MI, 1, false>(acc, lds, p, tv, 0, count, t);
             __syncthreads();
         } else {
             float m2, s2;
@@ -317,31 +403,40 @@ static int head_few_tile(int64_t classes) { return cdiv(classes, 128) >= num_com
 static int head_few_blocks(int64_t classes) { return (int)std::min<int64_t>(cdiv(classes, head_few_tile(classes)), 2 * num_compute_units()); }
 
 // The same on two blocks a compute unit, a tile of 256 classes x 128 tokens each.  A die's 64 tiles at a time: 8 of the weight x 8 of the tokens.
-template <bool GRAD, bool SOLO> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
+template <bool GRAD, bool SOLO, bool PLANES> __device__ __forceinline__ void head_logits_tile(const HeadLogits &p, bf16_t *lds, int count, int block)
 {
     const int tiles_t = (count + HD_TOK - 1) / HD_TOK, total = p.tiles_v * tiles_t, per_die = (total + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
     if ((block >> 3) >= per_die || w >= total) return;
     const int per_group = 8 * p.tiles_v, group = w / per_group, in_group = w - group * per_group, size = min(8, tiles_t - group * 8);
     const int tv = in_group / size, tok0 = (group * 8 + in_group - tv * size) * HD_TOK, row = p.v0 + tv * HD_TILE;
-    DuoOperand<DUO_A, K_CONT> pa;
-    DuoOperand<DUO_B, K_CONT> pb;
-    pa.set(p.w + (int64_t)row * p.ldw, p.ldw, 0, min(HD_TILE, p.classes - row), p.dim);
-    pb.set(p.x + (int64_t)tok0 * p.ldx, p.ldx, 0, min(HD_TOK, count - tok0), p.dim);
     f32x16 acc[DUO_MI][DUO_NI];
     duo_zero(acc);
-    duo_mainloop<SOLO>(acc, lds, pa, pb, (p.dim + DUO_K - 1) / DUO_K);
-    if constexpr (GRAD) head_leave_grad<DUO_MI, DUO_NI>(acc, lds, p, tv, tok0, count, (int)threadIdx.x);
+    const int stages = (p.dim + DUO_K - 1) / DUO_K;
+    if constexpr (PLANES) {
+        DuoPlanes<DUO_A, K_CONT, 0> pa;
+        DuoPlanes<DUO_B, K_CONT, 1> pb;
+        pa.set(p.w + (int64_t)row * p.ldw, p.ldw, 0, min(HD_TILE, p.classes - row), p.dim, p.plane);
+        pb.set(p.x + (int64_t)tok0 * p.ldx, p.ldx, 0, min(HD_TOK, count - tok0), p.dim, p.plane);
+        duo_mainloop<SOLO>(acc, lds, pa, pb, 6 * stages);
+    } else {
+        DuoOperand<DUO_A, K_CONT> pa;
+        DuoOperand<DUO_B, K_CONT> pb;
+        pa.set(p.w + (int64_t)row * p.ldw, p.ldw, 0, min(HD_TILE, p.classes - row), p.dim);
+        pb.set(p.x + (int64_t)tok0 * p.ldx, p.ldx, 0, min(HD_TOK, count - tok0), p.dim);
+        duo_mainloop<SOLO>(acc, lds, pa, pb, stages);
+    }
+    if constexpr (GRAD) head_leave_grad<DUO_MI, DUO_NI, PLANES>(acc, lds, p, tv, tok0, count, (int)threadIdx.x);
     else head_leave_stats<DUO_MI, DUO_NI>(acc, p, tv, tok0, count, (int)threadIdx.x);
 }
-template <bool GRAD> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
+template <bool GRAD, bool PLANES> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
-    head_logits_tile<GRAD, false>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
+    head_logits_tile<GRAD, false, PLANES>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
 }
-template <bool GRAD> __global__ __launch_bounds__(256, 1) void head_logits_solo_kernel(HeadLogits p)
+template <bool GRAD, bool PLANES> __global__ __launch_bounds__(256, 1) void head_logits_solo_kernel(HeadLogits p)
 {
     __shared__ __align__(16) bf16_t lds[SOLO_LDS];
-    head_logits_tile<GRAD, true>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
+    head_logits_tile<GRAD, true, PLANES>(p, lds, p.count ? *p.count : (int)p.tokens, (int)blockIdx.x);
 }
 
 // ----------------------------------------------------------------------------------------------- loss
@@ -411,13 +506,13 @@ struct HeadMerge {
     float *stats;          // [tokens]: lse, 0 in ignored rows
     const float2 *part;    // [parts][tokens], by place
     const int *pos;        // NULL: every row in its place
-    const bf16_t *x, *w;
+    const void *x, *w;     // bf16: as the products have them, x by place; fp32: the caller's own
     int64_t ldx, ldw, classes;
-    int parts, dim;        // dim: a multiple of 8, zeros behind the last value
+    int parts, dim;        // bf16: a multiple of 8, zeros behind the last value
     HeadSum sum;
 };
 // LANES lanes a token: many where the tokens are few and their parts a chain of loads.
-template <int LANES> __global__ __launch_bounds__(1024) void head_merge_kernel(HeadMerge p)
+template <int LANES, bool F32> __global__ __launch_bounds__(1024) void head_merge_kernel(HeadMerge p)
 {
     constexpr int TOK = 1024 / LANES;
     __shared__ float ms_[TOK][LANES + 1], ss_[TOK][LANES + 1];
@@ -443,12 +538,18 @@ template <int LANES> __global__ __launch_bounds__(1024) void head_merge_kernel(H
     const int64_t c = at < 0 ? 0 : p.sum.target[row];
     const bool known = c >= 0 && c < p.classes;
     if (at >= 0 && known) {
-        const bf16_t *x = p.x + (int64_t)at * p.ldx, *w = p.w + c * p.ldw;
+        if constexpr (F32) {
+            const float *x = static_cast<const float *>(p.x) + row * p.ldx, *w = static_cast<const float *>(p.w) + c * p.ldw;
+#pragma unroll 4
+            for (int i = lane; i < p.dim; i += LANES) d = fmaf(x[i], w[i], d);
+        } else {
+            const bf16_t *x = static_cast<const bf16_t *>(p.x) + (int64_t)at * p.ldx, *w = static_cast<const bf16_t *>(p.w) + c * p.ldw;
 #pragma unroll 2
-        for (int i = lane * 8; i < p.dim; i += LANES * 8) {
-            const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
+            for (int i = lane * 8; i < p.dim; i += LANES * 8) {
+                const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
+                for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
+            }
         }
     }
 #pragma unroll
@@ -480,15 +581,16 @@ struct HeadProducts {
     int64_t lddx, dx_stride, tokens;
     bool add;                  // to the sums that are there
     int splits, split_v;       // a split's classes, a multiple of 64
-    bf16_t *dw;                // the piece's first row of [classes][lddw], or NULL
+    void *dw;                  // the piece's first row of [classes][lddw], or NULL
+    int plane, plane_g;        // fp32: as in HeadLogits
     int64_t lddw;
     HeadScale scale;
     int tiles_d, tiles_v;
     int blocks_dw, blocks_dx;   // of the launch, multiples of 8; the others are the next piece's logits
 };
-// D[a][b] to out[a * ld + b], times a factor (bf16) or added to what is there (fp32): each wave passes 32 rows x its 64 columns at a time through LDS, so that a lane
-// stores 16 bytes of a row
-template <typename E, bool ADD>
+// D[a][b] to out[a * ld + b], times a factor (KEEP: fp32 sums, which the next launch adds to or finds, as they are; ADD: added to what is there): each wave passes 32 rows x
+// its 64 columns at a time through LDS, so that a lane stores 16 bytes of a row
+template <typename E, bool KEEP, bool ADD>
 __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], bf16_t *__restrict__ lds, E *__restrict__ out, int64_t ld, int na, int b0, int nb, float scale, int t)
 {
     constexpr int COLS = DUO_NI * 32, LDP = COLS + 4, PER = 16 / (int)sizeof(E), LPR = COLS / PER, RPP = 64 / LPR;
@@ -520,7 +622,16 @@ __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], b
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += o[e];
                 }
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rs, (int)off, 0, 0);
+                if constexpr (KEEP) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rs, (int)off, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] *= scale;
+                    if (b + 4 <= nb) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rs, (int)off, 0, 2);
+                    else   // the last values of a row
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v[e]), rs, a < na && b + e < nb ? (int)(off + 4u * e) : (int)HD_OOB, 0, 0);
+                }
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -529,12 +640,12 @@ __device__ __forceinline__ void head_store_rows(f32x16 (&acc)[DUO_MI][DUO_NI], b
 
 // dW's tiles (256 classes x 128 columns), dx's (256 tokens x 128 columns, a range of the piece's classes), and the next piece's logits: short tiles that fill the
 // compute units that have no more of the long ones.
-template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kernel(HeadProducts p, HeadLogits next)
+template <bool ADD, bool PLANES> __global__ __launch_bounds__(256, 2) void head_products_kernel(HeadProducts p, HeadLogits next)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];
     const int count = *p.count;
     int block = (int)blockIdx.x;
-    if (block >= p.blocks_dw + p.blocks_dx) return head_logits_tile<true, false>(next, lds, count, block - p.blocks_dw - p.blocks_dx);
+    if (block >= p.blocks_dw + p.blocks_dx) return head_logits_tile<true, false, PLANES>(next, lds, count, block - p.blocks_dw - p.blocks_dx);
     const bool dw = block < p.blocks_dw;
     if (!dw) block -= p.blocks_dw;
     const int tiles_t = (count + HD_TILE - 1) / HD_TILE, n = (dw ? p.tiles_v : p.splits * tiles_t) * p.tiles_d, per_die = (n + 7) >> 3, w = (block & 7) * per_die + (block >> 3);
@@ -544,26 +655,44 @@ template <bool ADD> __global__ __launch_bounds__(256, 2) void head_products_kern
     const int td = w % p.tiles_d, b0 = td * DUO_B;
     if (dw) {
         const int tv = w / p.tiles_d;
-        DuoOperand<DUO_A, M_CONT> pa;   // G: rows = classes, contraction = tokens
-        DuoOperand<DUO_B, M_CONT> pb;   // x: rows = its columns
-        pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
-        pb.set(p.x, p.ldx, b0, p.dim, count);
-        duo_mainloop<false>(acc, lds, pa, pb, (count + DUO_K - 1) / DUO_K);   // no rows: zeros
-        head_store_rows<bf16_t, false>(acc, lds, p.dw + (int64_t)tv * HD_TILE * p.lddw, p.lddw, min(HD_TILE, p.rows_v - tv * HD_TILE), b0, p.dim, p.scale.value(), (int)threadIdx.x);
+        const int stages = (count + DUO_K - 1) / DUO_K, rows = min(HD_TILE, p.rows_v - tv * HD_TILE);   // no rows: zeros
+        if constexpr (PLANES) {
+            DuoPlanes<DUO_A, M_CONT, 0> pa;   // G: rows = classes, contraction = tokens
+            DuoPlanes<DUO_B, M_CONT, 1> pb;   // x: rows = its columns
+            pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count, p.plane_g);
+            pb.set(p.x, p.ldx, b0, (int)p.ldx, count, p.plane);
+            duo_mainloop<false>(acc, lds, pa, pb, 6 * stages);
+            head_store_rows<float, false, false>(acc, lds, static_cast<float *>(p.dw) + (int64_t)tv * HD_TILE * p.lddw, p.lddw, rows, b0, (int)p.lddw, p.scale.value(), (int)threadIdx.x);
+        } else {
+            DuoOperand<DUO_A, M_CONT> pa;
+            DuoOperand<DUO_B, M_CONT> pb;
+            pa.set(p.g, p.ldg, tv * HD_TILE, (int)p.ldg, count);
+            pb.set(p.x, p.ldx, b0, p.dim, count);
+            duo_mainloop<false>(acc, lds, pa, pb, stages);
+            head_store_rows<bf16_t, false, false>(acc, lds, static_cast<bf16_t *>(p.dw) + (int64_t)tv * HD_TILE * p.lddw, p.lddw, rows, b0, p.dim, p.scale.value(), (int)threadIdx.x);
+        }
     } else {
         const int tt = w / p.tiles_d % tiles_t, s = w / p.tiles_d / tiles_t, v0 = s * p.split_v, vs = min(p.split_v, p.rows_v - v0), tok = tt * HD_TILE;
-        const int toks = min(HD_TILE, count - tok);
-        DuoOperand<DUO_A, K_CONT> pa;   // G: rows = tokens, contraction = classes
-        DuoOperand<DUO_B, M_CONT> pb;   // W: rows = its columns
-        pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7);
-        pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
-        duo_mainloop<false>(acc, lds, pa, pb, (vs + DUO_K - 1) / DUO_K);
-        head_store_rows<float, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, (int)threadIdx.x);
+        const int toks = min(HD_TILE, count - tok), stages = (vs + DUO_K - 1) / DUO_K;
+        if constexpr (PLANES) {
+            DuoPlanes<DUO_A, K_CONT, 0> pa;   // G: rows = tokens, contraction = classes
+            DuoPlanes<DUO_B, M_CONT, 1> pb;   // W: rows = its columns
+            pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7, p.plane_g);
+            pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, (int)p.ldw, vs, p.plane);
+            duo_mainloop<false>(acc, lds, pa, pb, 6 * stages);
+        } else {
+            DuoOperand<DUO_A, K_CONT> pa;
+            DuoOperand<DUO_B, M_CONT> pb;
+            pa.set(p.g + (int64_t)tok * p.ldg + v0, p.ldg, 0, toks, (vs + 7) & ~7);
+            pb.set(p.w + (int64_t)v0 * p.ldw, p.ldw, b0, p.dim, vs);
+            duo_mainloop<false>(acc, lds, pa, pb, stages);
+        }
+        head_store_rows<float, true, ADD>(acc, lds, p.dx + s * p.dx_stride + (int64_t)tok * p.lddx, p.lddx, toks, b0, p.dim, 1.0f, (int)threadIdx.x);
     }
 }
 
 // dx[row] = factor * the sums of its place over the splits, rounded once; zeros in ignored rows.  The blocks behind those bring dW into rows without gaps.
-__global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, const float *__restrict__ sums, const int *__restrict__ pos, int64_t tokens, int dim,
+template <typename E> __global__ __launch_bounds__(256) void head_dx_kernel(E *__restrict__ dx, const float *__restrict__ sums, const int *__restrict__ pos, int64_t tokens, int dim,
                                                       int64_t ld, int64_t stride, int splits, HeadScale scale, HeadRepack dw)
 {
     const int summing = (int)gridDim.x - dw.blocks;
@@ -571,7 +700,7 @@ __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, c
     const float f = scale.value();
     const int chunks = (int)(ld / 4);
     const int64_t n = tokens * chunks;
-    const bool whole = dim % 4 == 0;   // rows of dx begin on 8 bytes then
+    const bool whole = dim % 4 == 0;   // rows of dx begin on pieces of 4 values then
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)summing * 256) {
         const int64_t row = i / chunks;
         const int c = (int)(i - row * chunks) * 4, at = pos[row];
@@ -586,13 +715,18 @@ __global__ __launch_bounds__(256) void head_dx_kernel(bf16_t *__restrict__ dx, c
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= f;
         }
-        bf16_t *out = dx + row * dim + c;
+        E *out = dx + row * dim + c;
         if (whole) {
-            if (c < dim) *reinterpret_cast<uint2 *>(out) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+            if (c >= dim) continue;
+            if constexpr (sizeof(E) == 4) *reinterpret_cast<f32x4 *>(out) = v;
+            else *reinterpret_cast<uint2 *>(out) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < dim) out[e] = f32_to_bf16(v[e]);
+                if (c + e < dim) {
+                    if constexpr (sizeof(E) == 4) out[e] = v[e];
+                    else out[e] = f32_to_bf16(v[e]);
+                }
         }
     }
 }
@@ -691,16 +825,6 @@ struct HeadFew {
     int tokens, dim, classes;
     int range;             // dx: classes of a range, a multiple of 32
 };
-__device__ __forceinline__ f32x4 head_load4(const float *p, int left, bool whole)
-{
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (whole) __builtin_memcpy(&v, p, 16);   // at any address
-    else
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) v[e] = p[e];
-    return v;
-}
 // The waves' sums one after the other: deterministic.  COLS values a token.
 template <int COLS, typename F> __device__ __forceinline__ void head_add_waves(float (&sums)[HS_T][COLS + 4], int wave, F value)
 {
@@ -823,13 +947,31 @@ __global__ __launch_bounds__(256) void head_few_sum_kernel(float *__restrict__ o
 // 768 columns 2319, 2319, 2329, 2322, 2449; 4096 tokens x 4096 -> 65536 7076, 7082, 7090, 7138, 7134.
 constexpr int64_t HD_PIECE_BYTES = 128ll << 20, HD_PIECE_MOST = 512ll << 20;
 constexpr int HD_TILE_COST = 8;   // of a tile's first operands and its stores
-static int64_t head_piece_bytes(int64_t tokens, int64_t dim)
+// planes: 1, or 3 of fp32, with six products of them
+static int64_t head_piece_bytes(int64_t tokens, int64_t dim, int64_t planes)
 {
-    const int64_t td = cdiv(dim, DUO_B), longest = cdiv(tokens, DUO_K) + HD_TILE_COST;
-    const int64_t of_256 = td * longest + cdiv(tokens, HD_TILE) * td * (HD_TILE / DUO_K) + cdiv(tokens, HD_TOK) * (cdiv(dim, DUO_K) + HD_TILE_COST);   // work of 256 classes
+    const int64_t products = planes == 1 ? 1 : 6, td = cdiv(dim, DUO_B), longest = products * cdiv(tokens, DUO_K) + HD_TILE_COST;
+    const int64_t of_256 = td * longest + cdiv(tokens, HD_TILE) * td * products * (HD_TILE / DUO_K) + cdiv(tokens, HD_TOK) * (products * cdiv(dim, DUO_K) + HD_TILE_COST);   // work of 256 classes
     int64_t bytes = HD_PIECE_BYTES;
-    while (bytes < HD_PIECE_MOST && bytes / (2 * HD_TILE * tokens) * of_256 < 2 * longest * 2 * num_compute_units()) bytes *= 2;
+    while (bytes < HD_PIECE_MOST && bytes / (2 * planes * HD_TILE * tokens) * of_256 < 2 * longest * 2 * num_compute_units()) bytes *= 2;
     return bytes;
+}
+
+// The logits of few tokens beside the weight are kept for the backward call.
+static bool head_keepable(int64_t tokens, int64_t dim, int64_t classes) { return 4 * tokens <= dim && tokens * classes <= (1ll << 26); }
+// fp32 on the tiles of the bf16 products, x, W and G in three planes each and six products of them, 1.1 - 1.25 PFLOP/s of bf16, where the offsets allow it and there are tiles enough:
+// in the logits two a compute unit, in dW (which contracts all tokens) three to four units in a piece, of not so few tokens that most of a tile of dx is for none.  Otherwise the
+// products of rdb_f32.hip, with smaller tiles and long contractions in ranges.  us, those | planes, forward: 2048 x 768 -> 50304 915 | 808, 8192 x 768 -> 50304 3554 | 2906, 3135 x 64 -> 5696
+// 44 | 29, 1000 x 512 -> 8000 64 | 62, 1024 x 2048 -> 8000 193 | 205, 2000 x 256 -> 2000 32 | 38; a step: 2048 x 768 -> 50304 3730 | 3420, 8192 x 768 -> 50304 16240 | 13380, 768 x 512 ->
+// 20000 491 | 412, 700 x 768 -> 30000 876 | 893, 400 x 512 -> 60000 769 | 917, 1024 x 1024 -> 4000 237 | 295, 8192 x 128 -> 30000 2382 | 3893.  Rows that are ignored cost nothing in planes:
+// 645 x 320 -> 103808 with half of them 1489 | 991.
+static bool head_in_planes(int64_t tokens, int64_t dim, int64_t classes, bool backward)
+{
+    const int64_t row = 3 * (dim + 7);
+    if (tokens <= HS_T || tokens > (1ll << 20) || head_keepable(tokens, dim, classes) || row >= (1ll << 20) || row * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29)) return false;
+    const int64_t units = num_compute_units();
+    if (!backward) return cdiv(classes, HD_TILE) * cdiv(tokens, HD_TOK) >= 2 * units;
+    return tokens >= 576 && std::min(classes, HD_PIECE_MOST / (6 * tokens)) / HD_TILE * cdiv(dim, DUO_B) >= units / 4 * 3;
 }
 
 struct HeadPlan {
@@ -837,6 +979,8 @@ struct HeadPlan {
     int dtype;
     bool backward, want_dx, want_dw, pack_w, pad_dw;
     bool direct;               // few tokens, forward: x as it is, ignored rows and all
+    bool tiles;                // on the tiles of rdb_duo.hpp (few: rdb_gemm.hpp)
+    int64_t planes;            // of an operand there: 1, or 3 (fp32)
     int64_t dp, vp;            // columns of the copies; classes of a piece
     int pieces, splits;
     bool few;                  // one tile of few tokens
@@ -859,21 +1003,24 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.backward = backward;
     h.want_dx = want_dx;
     h.want_dw = want_dw;
-    const bool f32 = dtype == RDB_F32;
-    const int64_t es = f32 ? 4 : 2;
+    h.planes = dtype == RDB_F32 && head_in_planes(tokens, dim, classes, backward) ? 3 : 1;
+    h.tiles = dtype != RDB_F32 || h.planes > 1;
+    const bool f32 = !h.tiles;
     h.dp = f32 ? dim : (dim + 7) / 8 * 8;
-    h.pack_w = !f32 && pack_w;
-    h.pad_dw = !f32 && h.dp != dim;
-    int64_t cols = (f32 ? 2 * HD_PIECE_BYTES : head_piece_bytes(tokens, dim)) / (es * tokens) / HD_TILE * HD_TILE;
-    // 32-bit offsets within a piece of the weight, and of dW
-    const int64_t far = std::max(h.dp, h.pack_w ? h.dp : ldw);
+    h.pack_w = h.tiles && (pack_w || h.planes > 1);
+    h.pad_dw = dtype != RDB_F32 && h.dp != dim;
+    const int64_t es = f32 ? 4 : 2 * h.planes;   // bytes of a value of G
+    int64_t cols = (f32 ? 2 * HD_PIECE_BYTES : head_piece_bytes(tokens, dim, h.planes)) / (es * tokens) / HD_TILE * HD_TILE;
+    // 32-bit offsets within a piece of the weight, of dW, and of G with 128 tokens more
+    const int64_t far = h.pack_w ? h.planes * h.dp : std::max(h.dp, ldw);
     cols = std::min<int64_t>(cols, (f32 ? (1ll << 29) - 1 : 1ll << 28) / std::max(f32 ? tokens : 0, far) / HD_TILE * HD_TILE);
+    if (h.tiles) cols = std::min<int64_t>(cols, (1ll << 23) / h.planes / HD_TILE * HD_TILE);
     cols = std::max<int64_t>(cols, HD_TILE);
     h.pieces = (int)cdiv(classes, cols);
     h.vp = cdiv(cdiv(classes, h.pieces), HD_TILE) * HD_TILE;
     if (f32 && h.pieces == 1) h.vp = classes;
     h.pieces = (int)cdiv(classes, h.vp);
-    h.few = tokens <= HD_FEW;
+    h.few = tokens <= HD_FEW && h.planes == 1;
     if (f32 && tokens <= HS_T) {   // ranges of dx: four blocks a compute unit, at least 128 classes each, sums of at most an eighth of the weight's bytes
         const int64_t most = std::min(4 * num_compute_units() / cdiv(dim, 128), std::min(h.vp / 128, h.vp / (8 * tokens)));
         h.range = cdiv(cdiv(h.vp, std::max<int64_t>(1, most)), 32) * 32;
@@ -892,11 +1039,11 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         at += (bytes + 255) / 256 * 256;
         return o;
     };
-    h.direct = !f32 && !backward && tokens <= HD_FEW && wide_x;
+    h.direct = dtype != RDB_F32 && !backward && tokens <= HD_FEW && wide_x;
     if (f32 ? want_dw : !h.direct) h.xc = room(tokens * h.dp * es);
     if (!f32 && !h.direct) h.pos = room(tokens * 4);
     h.count = room(8);
-    if (h.pack_w) h.wc = room(classes * h.dp * 2);
+    if (h.pack_w) h.wc = room(classes * h.dp * 2 * h.planes);
     if (!backward) {
         h.nll = room(tokens * 4);
         if (f32) {
@@ -943,7 +1090,7 @@ struct HeadCall {
 };
 static bool head_aligned(const void *p, int64_t ld, int es) { return !((uintptr_t)p & 15) && ld * es % 16 == 0; }
 
-static HeadRepack head_repack(bf16_t *dst, const bf16_t *src, int64_t ld, int64_t rows, int64_t cols)
+static HeadRepack head_repack(bf16_t *dst, const void *src, int64_t ld, int64_t rows, int64_t cols)
 {
     const int64_t per_block = std::max<int64_t>(1, 1024 / cols) * 8;   // four pieces a lane
     return {dst, src, ld, rows, (int)cols, (int)per_block, (int)cdiv(rows, per_block)};
@@ -958,15 +1105,15 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
     *w = static_cast<const bf16_t *>(c.w);
     *ldw = c.ldw;
     if (h.pack_w) {
-        r = head_repack(c.at<bf16_t>(h.wc), *w, c.ldw, h.classes, h.dim);
+        r = head_repack(c.at<bf16_t>(h.wc), c.w, c.ldw, h.classes, h.dim);
         *w = r.dst;
-        *ldw = h.dp;
+        *ldw = h.planes * h.dp;
     }
     if (!h.direct) {
         p.xc = c.at<bf16_t>(h.xc);
-        p.x = static_cast<const bf16_t *>(c.x);
+        p.x = c.x;
         p.ldx = c.ldx;
-        p.ldc = h.dp;
+        p.ldc = h.planes * h.dp;
         p.target = c.target;
         p.pos = c.at<int>(h.pos);
         p.count = c.at<int>(h.count);
@@ -985,7 +1132,8 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
         gathering = cdiv(h.tokens, p.rows);
     }
     if (!gathering && !r.blocks) return RDB_OK;
-    head_gather_kernel<<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
+    if (h.planes > 1) head_gather_kernel<true><<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
+    else head_gather_kernel<false><<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
     return check_launch("head_gather_kernel");
 }
 
@@ -1002,11 +1150,15 @@ template <bool GRAD> static int head_logits(HeadLogits &p, int64_t classes, bool
         return check_launch(GRAD ? "head_logits_few_kernel<gradient>" : "head_logits_few_kernel");
     }
     const int64_t tiles = p.tiles_v * cdiv(p.tokens, HD_TOK);
-    if (tiles <= num_compute_units() && p.dim >= HD_SOLO_DIM) {
-        head_logits_solo_kernel<GRAD><<<(unsigned)((tiles + 7) / 8 * 8), 256, 0, s>>>(p);
+    const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8);
+    const bool planes = p.plane != 0;
+    if (tiles <= num_compute_units() && (planes ? 6 : 1) * p.dim >= HD_SOLO_DIM) {
+        if (planes) head_logits_solo_kernel<GRAD, true><<<blocks, 256, 0, s>>>(p);
+        else head_logits_solo_kernel<GRAD, false><<<blocks, 256, 0, s>>>(p);
         return check_launch(GRAD ? "head_logits_solo_kernel<gradient>" : "head_logits_solo_kernel");
     }
-    head_logits_duo_kernel<GRAD><<<(unsigned)((tiles + 7) / 8 * 8), 256, 0, s>>>(p);
+    if (planes) head_logits_duo_kernel<GRAD, true><<<blocks, 256, 0, s>>>(p);
+    else head_logits_duo_kernel<GRAD, false><<<blocks, 256, 0, s>>>(p);
     return check_launch(GRAD ? "head_logits_duo_kernel<gradient>" : "head_logits_duo_kernel");
 }
 
@@ -1016,7 +1168,7 @@ static HeadSum head_sum_of(const HeadCall &c, float *loss, float *stats, int red
     return {reduction == HD_NONE ? nullptr : loss, stats + h.tokens, reduction == HD_NONE ? loss : c.at<float>(h.nll), c.at<unsigned int>(h.count) + 1, c.target, h.tokens, c.ignore,
             reduction == HD_MEAN};
 }
-static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduction)
+static int head_fwd_tiles(const HeadCall &c, float *loss, float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
     const bf16_t *w;
@@ -1024,9 +1176,10 @@ static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduc
     if (int rc = head_gather(c, nullptr, nullptr, &w, &ldw)) return rc;
     HeadLogits p = {};
     p.x = h.direct ? static_cast<const bf16_t *>(c.x) : c.at<bf16_t>(h.xc);
-    p.ldx = h.direct ? c.ldx : h.dp;
+    p.ldx = h.direct ? c.ldx : h.planes * h.dp;
     p.w = w;
     p.ldw = ldw;
+    p.plane = h.planes > 1 ? (int)h.dp : 0;
     p.count = h.direct ? nullptr : c.at<int>(h.count);
     p.cleared = h.direct ? c.at<unsigned int>(h.count) + 1 : nullptr;
     p.dim = (int)h.dp;
@@ -1034,36 +1187,49 @@ static int head_fwd_bf16(const HeadCall &c, float *loss, float *stats, int reduc
     p.part = c.at<float2>(h.part);
     p.tokens = h.tokens;
     if (int rc = head_logits<false>(p, h.classes, h.few, c.s)) return rc;
-    const HeadMerge m = {stats, p.part, h.direct ? nullptr : c.at<int>(h.pos), p.x, w, p.ldx, ldw, h.classes, h.parts, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
+    const int *pos = h.direct ? nullptr : c.at<int>(h.pos);
     // 16 lanes a token from as many tokens on as give every other compute unit a block of 64
-    if (h.tokens >= 8192) head_merge_kernel<16><<<(unsigned)cdiv(h.tokens, 64), 1024, 0, c.s>>>(m);
-    else head_merge_kernel<64><<<(unsigned)cdiv(h.tokens, 16), 1024, 0, c.s>>>(m);
+    const bool many = h.tokens >= 8192;
+    const unsigned blocks = (unsigned)cdiv(h.tokens, many ? 64 : 16);
+    if (h.planes > 1) {
+        const HeadMerge m = {stats, p.part, pos, c.x, c.w, c.ldx, c.ldw, h.classes, h.parts, (int)h.dim, head_sum_of(c, loss, stats, reduction)};
+        if (many) head_merge_kernel<16, true><<<blocks, 1024, 0, c.s>>>(m);
+        else head_merge_kernel<64, true><<<blocks, 1024, 0, c.s>>>(m);
+    } else {
+        const HeadMerge m = {stats, p.part, pos, p.x, w, p.ldx, ldw, h.classes, h.parts, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
+        if (many) head_merge_kernel<16, false><<<blocks, 1024, 0, c.s>>>(m);
+        else head_merge_kernel<64, false><<<blocks, 1024, 0, c.s>>>(m);
+    }
     return check_launch("head_merge_kernel");
 }
-static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float *dloss, const float *stats, int reduction)
+template <typename E> static int head_bwd_tiles(const HeadCall &c, E *dx, E *dw, const float *dloss, const float *stats, int reduction)
 {
     const HeadPlan &h = c.h;
     const bf16_t *w;
     int64_t ldw;
     if (int rc = head_gather(c, stats, reduction == HD_NONE ? dloss : nullptr, &w, &ldw)) return rc;
     const HeadScale scale = {reduction == HD_NONE ? nullptr : dloss, reduction == HD_MEAN ? stats + h.tokens : nullptr};
-    bf16_t *dwc = h.pad_dw && dw ? c.at<bf16_t>(h.dw) : dw;
+    constexpr bool PLANES = sizeof(E) == 4;
+    E *dwc = h.pad_dw && dw ? c.at<E>(h.dw) : dw;
+    const int64_t lddw = PLANES ? h.dim : h.dp;
     const int *count = c.at<int>(h.count);
     auto piece = [&](int i) {
         HeadLogits p = {};
         const int64_t v0 = i * h.vp;
         p.x = c.at<bf16_t>(h.xc);
-        p.ldx = h.dp;
+        p.ldx = h.planes * h.dp;
         p.w = w;
         p.ldw = ldw;
+        p.plane = PLANES ? (int)h.dp : 0;
+        p.plane_g = (int)h.vp;
         p.count = count;
         p.dim = (int)h.dp;
         p.classes = (int)h.classes;
         p.v0 = (int)v0;
         p.tiles_v = (int)cdiv(std::min(h.vp, h.classes - v0), HD_TILE);
         p.tokens = h.tokens;
-        p.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp;
-        p.ldg = h.vp;
+        p.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp * h.planes;
+        p.ldg = h.planes * h.vp;
         p.lse2 = c.at<float>(h.lse2);
         p.factor = c.at<float>(h.factor);
         p.label = c.at<int>(h.label);
@@ -1075,10 +1241,12 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
     for (int i = 0; i < h.pieces; ++i) {
         const int64_t v0 = i * h.vp, n = std::min(h.vp, h.classes - v0);
         HeadProducts q = {};
-        q.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp;
-        q.ldg = h.vp;
+        q.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp * h.planes;
+        q.ldg = h.planes * h.vp;
         q.x = c.at<bf16_t>(h.xc);
-        q.ldx = h.dp;
+        q.ldx = h.planes * h.dp;
+        q.plane = (int)h.dp;
+        q.plane_g = (int)h.vp;
         q.w = w + v0 * ldw;
         q.ldw = ldw;
         q.count = count;
@@ -1097,8 +1265,8 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
             q.blocks_dx = blocks_of(q.splits * cdiv(h.tokens, HD_TILE) * q.tiles_d);
         }
         if (dw) {
-            q.dw = dwc + v0 * h.dp;
-            q.lddw = h.dp;
+            q.dw = dwc + v0 * lddw;
+            q.lddw = lddw;
             q.blocks_dw = blocks_of((int64_t)q.tiles_v * q.tiles_d);
         }
         HeadLogits next = {};
@@ -1107,15 +1275,16 @@ static int head_bwd_bf16(const HeadCall &c, bf16_t *dx, bf16_t *dw, const float 
             next = piece(i + 1);
             blocks += blocks_of(next.tiles_v * cdiv(h.tokens, HD_TOK));
         }
-        if (i > 0) head_products_kernel<true><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
-        else head_products_kernel<false><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
+        if (i > 0) head_products_kernel<true, PLANES><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
+        else head_products_kernel<false, PLANES><<<(unsigned)blocks, 256, 0, c.s>>>(q, next);
         if (int rc = check_launch("head_products_kernel")) return rc;
     }
     HeadRepack r = {};
-    if (dw && h.pad_dw) r = head_repack(dw, dwc, h.dp, h.classes, h.dim);
+    if constexpr (!PLANES)
+        if (dw && h.pad_dw) r = head_repack(dw, dwc, h.dp, h.classes, h.dim);
     const int64_t summing = dx ? std::min<int64_t>(cdiv(h.tokens * h.dp / 4, 256), 8192) : 0;
     if (!summing && !r.blocks) return RDB_OK;
-    head_dx_kernel<<<(unsigned)(summing + r.blocks), 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale, r);
+    head_dx_kernel<E><<<(unsigned)(summing + r.blocks), 256, 0, c.s>>>(dx, c.at<float>(h.dx), c.at<int>(h.pos), h.tokens, (int)h.dim, h.dp, h.tokens * h.dp, h.splits, scale, r);
     return check_launch("head_dx_kernel");
 }
 
@@ -1222,8 +1391,8 @@ static int check_head(const char *who, int64_t tokens, int64_t dim, int64_t clas
     // 32-bit offsets within an operand: x in rows of a multiple of 8 values, a tile of W's rows, a piece of G
     if ((dim + 7) / 8 * 8 * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29) || tokens >= (1ll << 21) || ldw >= (1ll << 20))
         return set_error(RDB_E_UNSUPPORTED, "%s: x of less than 2^29 values and 2^21 rows, rows of w less than 2^20 apart", who);
-    if (dtype == RDB_BF16 && cdiv(classes, HD_TILE) * cdiv(tokens, HD_TOK) >= (1ll << 23))   // a launch has less than 2^32 threads
-        return set_error(RDB_E_UNSUPPORTED, "%s: less than 2^38 logits in bf16", who);
+    if (cdiv(classes, HD_TILE) * cdiv(tokens, HD_TOK) >= (1ll << 23))   // a launch has less than 2^32 threads
+        return set_error(RDB_E_UNSUPPORTED, "%s: less than 2^38 logits", who);
     return RDB_OK;
 }
 
@@ -1249,7 +1418,7 @@ extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int6
 extern "C" int64_t rdb_linear_cross_entropy_keeps(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw)
 {
     if (check_head("rdb_linear_cross_entropy_keeps", tokens, dim, classes, dtype, dim, ldw, 0)) return 0;
-    if (dtype != RDB_F32 || 4 * tokens > dim) return 0;
+    if (dtype != RDB_F32 || !head_keepable(tokens, dim, classes)) return 0;
     return head_plan(tokens, dim, classes, dtype, ldw, true, true, true, false, false).pieces == 1 ? tokens * classes : 0;
 }
 
@@ -1264,7 +1433,7 @@ extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *lo
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
-    return dtype == RDB_F32 ? head_fwd_f32(c, loss, stats, logits, reduction) : head_fwd_bf16(c, loss, stats, reduction);
+    return h.tiles ? head_fwd_tiles(c, loss, stats, reduction) : head_fwd_f32(c, loss, stats, logits, reduction);
 }
 
 extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dloss, const float *stats, const float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype,
@@ -1280,6 +1449,7 @@ extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dlo
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
-    return dtype == RDB_F32 ? head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, logits, reduction)
-                            : head_bwd_bf16(c, static_cast<bf16_t *>(dx), static_cast<bf16_t *>(dw), dloss, stats, reduction);
+    if (!h.tiles) return head_bwd_f32(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, logits, reduction);
+    return dtype == RDB_F32 ? head_bwd_tiles(c, static_cast<float *>(dx), static_cast<float *>(dw), dloss, stats, reduction)
+                            : head_bwd_tiles(c, static_cast<bf16_t *>(dx), static_cast<bf16_t *>(dw), dloss, stats, reduction);
 }

@@ -405,3 +405,30 @@ def test_a_capture_beside_an_older_graph_of_the_same_leaves():
     """Refused, where it would end the process; without the older graph it is captured.  In a process of its own."""
     done = subprocess.run([sys.executable, "-c", CAPTURE], cwd=pathlib.Path(__file__).parents[1], capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and done.stdout.split() == ["refused", "captured"] * 2, (done.returncode, done.stdout, done.stderr[-2000:])
+
+
+@pytest.mark.parametrize("tokens,dim,classes", [(611, 333, 33001), (640, 520, 12000), (577, 1001, 6400), (2050, 260, 50001), (1300, 40, 12001), (4100, 64, 4300)])
+def test_fp32_in_planes(tokens, dim, classes):
+    """On the tiles of the bf16 products, one piece and several, the last two going forward only; from rows with gaps, with rows that hold anything left out; the same bits every time
+    and for one gradient alone."""
+    print(f"case head loss in planes {tokens} x {dim} -> {classes}", flush=True)
+    for reduction, ignored in (("mean", 0.0), ("none", 0.4)):
+        x, w, t = inputs(tokens, dim, classes, torch.float32, tokens, ignored)
+        got = both(x, w, t, reduction)
+        check(x, w, t, reduction, got[0], got[1], got[2], got[3])
+        wide_x, wide_w = torch.full((tokens, dim + 5), math.nan, device="cuda"), torch.full((classes, dim + 2), math.nan, device="cuda")
+        wide_x[:, 3:3 + dim], wide_w[:, 1:1 + dim] = x, w
+        wide_x[t == IGNORED] = math.inf
+        for a, b in zip(got, both(wide_x[:, 3:3 + dim], wide_w[:, 1:1 + dim], t, reduction, got[1])):
+            assert torch.equal(a, b)
+    for leaf, at in ((0, 2), (1, 3)):
+        leaves = [x.detach(), w.detach()]
+        leaves[leaf].requires_grad_()
+        assert torch.equal(torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, IGNORED, "none"), leaves[leaf], got[1])[0], got[at])
+        leaves[leaf].requires_grad_(False)
+    u = t.clone()
+    u[5], u[9] = classes, -1
+    loss, _, dx, dw = both(x, w, u, "none")
+    assert bool(loss[[5, 9]].isnan().all()) and int(loss.isnan().sum()) == 2 and int(dx.isnan().any(1).sum()) == 2
+    nothing = both(x, w, torch.full_like(t, IGNORED), "sum")
+    assert float(nothing[0]) == 0.0 and not bool(nothing[2].any()) and not bool(nothing[3].any())
