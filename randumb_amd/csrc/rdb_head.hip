@@ -31,6 +31,7 @@
 namespace rdb {
 
 int num_compute_units();
+int f32_split_mode();
 
 constexpr int HD_TILE = 256, HD_TOK = DUO_B;
 constexpr uint32_t HD_OOB = 0xfffffff0u;   // outside a buffer of any size up to 2^32 - 16 bytes
@@ -964,11 +965,11 @@ static bool head_keepable(int64_t tokens, int64_t dim, int64_t classes) { return
 // products of rdb_f32.hip, with smaller tiles and long contractions in ranges.  us, those | planes, forward: 2048 x 768 -> 50304 915 | 808, 8192 x 768 -> 50304 3554 | 2906, 3135 x 64 -> 5696
 // 44 | 29, 1000 x 512 -> 8000 64 | 62, 1024 x 2048 -> 8000 193 | 205, 2000 x 256 -> 2000 32 | 38; a step: 2048 x 768 -> 50304 3730 | 3420, 8192 x 768 -> 50304 16240 | 13380, 768 x 512 ->
 // 20000 491 | 412, 700 x 768 -> 30000 876 | 893, 400 x 512 -> 60000 769 | 917, 1024 x 1024 -> 4000 237 | 295, 8192 x 128 -> 30000 2382 | 3893.  Rows that are ignored cost nothing in planes:
-// 645 x 320 -> 103808 with half of them 1489 | 991.
+// 645 x 320 -> 103808 with half of them 1489 | 991.  Not where fp32 matrix instructions are asked for (rdb_set_f32_split).
 static bool head_in_planes(int64_t tokens, int64_t dim, int64_t classes, bool backward)
 {
     const int64_t row = 3 * (dim + 7);
-    if (tokens <= HS_T || tokens > (1ll << 20) || head_keepable(tokens, dim, classes) || row >= (1ll << 20) || row * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29)) return false;
+    if (!f32_split_mode() || tokens <= HS_T || tokens > (1ll << 20) || head_keepable(tokens, dim, classes) || row >= (1ll << 20) || row * std::max<int64_t>(tokens, HD_TILE) >= (1ll << 29)) return false;
     const int64_t units = num_compute_units();
     if (!backward) return cdiv(classes, HD_TILE) * cdiv(tokens, HD_TOK) >= 2 * units;
     return tokens >= 576 && std::min(classes, HD_PIECE_MOST / (6 * tokens)) / HD_TILE * cdiv(dim, DUO_B) >= units / 4 * 3;

@@ -544,7 +544,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     the forward to the backward pass).
 
     ``x`` (..., dim) and ``weight`` (classes, dim): both bf16 or both fp32, on one GPU; ``target`` (...): int64 or int32.  The loss is fp32; logits are
-    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out, in bf16 before anything is multiplied: what their rows hold does not matter.  The mean over no tokens is
+    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out (in bf16, and in fp32 of many tokens, before anything is multiplied): what their rows hold does not matter.  The mean over no tokens is
     NaN, with gradients of zero; a target outside the classes makes its token's loss and gradients NaN.  First derivatives only."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")

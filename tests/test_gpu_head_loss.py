@@ -9,7 +9,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from randumb_amd import ops
+from randumb_amd import hip, ops
 
 pytestmark = pytest.mark.gpu
 IGNORED = -100
@@ -432,3 +432,18 @@ def test_fp32_in_planes(tokens, dim, classes):
     assert bool(loss[[5, 9]].isnan().all()) and int(loss.isnan().sum()) == 2 and int(dx.isnan().any(1).sum()) == 2
     nothing = both(x, w, torch.full_like(t, IGNORED), "sum")
     assert float(nothing[0]) == 0.0 and not bool(nothing[2].any()) and not bool(nothing[3].any())
+
+
+def test_fp32_matrix_instructions_where_they_are_asked_for():
+    """The switch of the fp32 products reaches the head's, too."""
+    x, w, t = inputs(640, 520, 12000, torch.float32, 7, 0.1)
+    planes = both(x, w, t, "mean")
+    before = hip.set_f32_split(0)
+    try:
+        got = both(x, w, t, "mean")
+    finally:
+        hip.set_f32_split(before)
+    check(x, w, t, "mean", got[0], got[1], got[2], got[3])
+    assert not torch.equal(got[3], planes[3])
+    for a, b in zip(planes, both(x, w, t, "mean")):
+        assert torch.equal(a, b)
