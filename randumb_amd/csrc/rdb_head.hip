@@ -64,6 +64,34 @@ __device__ __forceinline__ f32x4 head_load4(const float *p, int left, bool whole
             if (e < left) v[e] = p[e];
     return v;
 }
+// fg_split3 with products that nobody runs again.  An infinity is (0, 0, infinity): of its six products only that with the other side's first plane is not of zeros, so it is what an
+// infinity's is, inf by what is finite and not zero, NaN by zero.  A finite value that would round to an infinity has its first part cut off.  Two comparisons where there is none.
+__device__ __forceinline__ void head_split3(float v0, float v1, uint32_t &h, uint32_t &m, uint32_t &l)
+{
+    constexpr float ROUNDS_UP = 0x1.ffp127f;   // half a step past the largest bf16
+    fg_split3(v0, v1, h, m, l);
+    if (fabsf(v0) < ROUNDS_UP && fabsf(v1) < ROUNDS_UP) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float v = e ? v1 : v0;
+        if (!(fabsf(v) >= ROUNDS_UP)) continue;   // a NaN stays one in the first part
+        const int s = 16 * e;
+        const uint32_t keep = 0xffffu << (16 - s), bits = __float_as_uint(v);
+        uint32_t part[3] = {0u, 0u, bits >> 16};
+        if (__builtin_isfinite(v)) {
+            part[0] = bits >> 16;
+            float r = v - __uint_as_float(bits & 0xffff0000u);
+#pragma unroll
+            for (int i = 1; i < 3; ++i) {
+                part[i] = f32_to_bf16(r);
+                r -= __uint_as_float(part[i] << 16);
+            }
+        }
+        h = (h & keep) | part[0] << s;
+        m = (m & keep) | part[1] << s;
+        l = (l & keep) | part[2] << s;
+    }
+}
 // 8 values, `left` of them there, into the planes
 __device__ __forceinline__ void head_split8(bf16_t *to, int plane, const float *from, int left)
 {
@@ -72,7 +100,7 @@ __device__ __forceinline__ void head_split8(bf16_t *to, int plane, const float *
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         uint32_t h, m, l;
-        fg_split3(e < 2 ? a[2 * e] : b[2 * e - 4], e < 2 ? a[2 * e + 1] : b[2 * e - 3], h, m, l);
+        head_split3(e < 2 ? a[2 * e] : b[2 * e - 4], e < 2 ? a[2 * e + 1] : b[2 * e - 3], h, m, l);
         v[0][e] = h;
         v[1][e] = m;
         v[2][e] = l;
