@@ -9,10 +9,10 @@
 //
 // On the tiles of rdb_duo.hpp (bf16; of few tokens on those of rdb_gemm.hpp; fp32 in three bf16 planes, where that is faster):
 //   head_gather_kernel      the rows that count, one after the other, in rows of a multiple of 8 values
-//   head_logits_duo_kernel  a tile of logits in the accumulators -> its maximum and its sum of exponentials for each token; or (backward), a piece of the
-//   head_logits_solo_kernel vocabulary's logits once more -> G, in bf16, for the next launch
+//   head_logits_duo_kernel  a tile of logits in the accumulators -> its maximum and its sum of exponentials for each token, and the target's logit; or (backward), a piece
+//   head_logits_solo_kernel of the vocabulary's logits once more -> G, in bf16, for the next launch
 //   head_logits_few_kernel  (all tokens in one tile)
-//   head_merge_kernel       the tiles of a token together, the target's logit, nll; the last block adds up the tokens
+//   head_merge_kernel       the tiles of a token together, nll; the last block adds up the tokens
 //   head_products_kernel    dx += G . W and dW = G^T . x of the piece, and the next piece's G, one list of tiles
 //   head_dx_kernel          dx from its sums, back in the rows' own places
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
@@ -46,9 +46,8 @@ struct HeadGather {
     const int64_t *target;
     int *pos;                // [tokens]: where a row went, -1: ignored
     int *count;              // rows that count; behind it the counter of head_merge_kernel's blocks, cleared
-    // backward, by place: log2 of the row's sum, target (-1: none of the classes), its own factor of G
-    float *lse2, *factor;
-    int *label;
+    int *label;              // by place: target (-1: none of the classes)
+    float *lse2, *factor;    // backward, by place, or NULL: log2 of the row's sum, its own factor of G
     const float *stats;      // lse by row
     const float *dloss;      // [tokens], or NULL: 1
     int64_t tokens, dim, classes, ignore;
@@ -130,11 +129,13 @@ template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const He
         place_[lane] = counts ? at : -1;
         if (lane < mine) {
             p.pos[r0 + lane] = counts ? at : -1;
-            if (p.lse2 && counts) {
+            if (counts) {
                 const bool known = c >= 0 && c < p.classes;
-                p.lse2[at] = p.stats[r0 + lane] * HD_LOG2E;
                 p.label[at] = known ? (int)c : -1;
-                p.factor[at] = !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
+                if (p.lse2) {
+                    p.lse2[at] = p.stats[r0 + lane] * HD_LOG2E;
+                    p.factor[at] = !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
+                }
             }
         }
         if (lane == 0 && r0 + mine == p.tokens) {
@@ -250,12 +251,14 @@ struct HeadLogits {
     int dim, classes, v0;     // classes v0 .. v0 + tiles_v * 256 of this launch
     int tiles_v;
     float2 *part;         // stats: [2 * tiles_v][tokens]: maximum (times log2 e) and sum
+    float *picked;        // stats, by place: the target's logit, from the tile that has it
     int64_t tokens;
     bf16_t *g;            // gradient: [tokens][ldg], class v0 first
     int64_t ldg;
     int plane, plane_g;   // fp32: values from plane to plane of x and w, of g
     const float *lse2, *factor;
     const int *label;
+    const int64_t *target;   // few tokens as they are (count NULL): their targets, instead of labels
 };
 __device__ __forceinline__ int head_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
 
@@ -288,6 +291,24 @@ __device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2
     s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
     m = top;
 }
+// The logit of class `rel` of a wave's, where it has it, of its ni-th 32 tokens.  It has to be the one that is in the sum: from a sum of products in another order nll of a token
+// whose own class has nearly all of the probability would be rounding of either sign.
+template <int MI, int NI> __device__ __forceinline__ void head_pick(const f32x16 (&acc)[MI][NI], int ni, int rel, int g, float *to)
+{
+    if (!__any((unsigned)rel < (unsigned)(MI * 32))) return;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MI * 16; ++i)
+        if ((i >> 4) * 32 + head_row(i & 15, g) == rel) v = acc[i >> 4][ni][i & 15];
+    if ((unsigned)rel < (unsigned)(MI * 32) && ((rel >> 2) & 1) == g) *to = v;
+}
+// nll from what the maximum is above the target's logit (times log2 e) and the sum: what rounding a maximum that is held times log2 e has put into the sum, the same rounding in
+// `above` takes out again.  A sum has its target's own part, so that what is below zero is rounding.
+__device__ __forceinline__ float head_nll(float above, float s)
+{
+    const float v = above + log2f(s);
+    return v < 0.0f ? 0.0f : v * HD_LN2;
+}
 // ... for each of the wave's tokens; each wave leaves its half of the classes' own
 template <int MI, int NI>
 __device__ __forceinline__ void head_leave_stats(const f32x16 (&acc)[MI][NI], const HeadLogits &p, int tv, int tok0, int count, int t)
@@ -295,9 +316,11 @@ __device__ __forceinline__ void head_leave_stats(const f32x16 (&acc)[MI][NI], co
     const int wave = t >> 6, lane = t & 63, r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
+        const int tok = tok0 + wn * NI * 32 + ni * 32 + r, first = p.v0 + (tv * 2 + wm) * MI * 32;
+        head_pick(acc, ni, tok < count ? p.label[tok] - first : -1, g, p.picked + tok);
+        __builtin_amdgcn_sched_barrier(0);
         float m, s;
-        head_stats(acc, ni, p.classes - (p.v0 + (tv * 2 + wm) * MI * 32), g, m, s);
-        const int tok = tok0 + wn * NI * 32 + ni * 32 + r;
+        head_stats(acc, ni, p.classes - first, g, m, s);
         if (g == 0 && tok < count) p.part[(int64_t)(tv * 2 + wm) * p.tokens + tok] = float2{m, s};
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -397,8 +420,13 @@ template <bool GRAD, int HF_V> __global__ __launch_bounds__(256, 2) void head_lo
     if (p.cleared && blockIdx.x == 0 && threadIdx.x == 0) *p.cleared = 0u;
     const int count = p.count ? *p.count : (int)p.tokens;
     if (count <= 0) return;
-    const int t = threadIdx.x, lane = t & 63, r = lane & 31, g = lane >> 5, wm = t >> 7, wn = (t >> 6) & 1;
+    const int t = threadIdx.x, lane = t & 63, r = lane & 31, g = lane >> 5, wm = t >> 7, wn = (t >> 6) & 1, tok = wn * 32 + r;
     float m = -INFINITY, s = 0.0f;
+    int label = -1;
+    if (!GRAD && tok < count) {
+        const int64_t c = p.target ? p.target[tok] : p.label[tok];
+        label = c >= 0 && c < p.classes ? (int)c : -1;
+    }
     for (int tv = (int)blockIdx.x; tv < p.tiles_v; tv += (int)gridDim.x) {
         const int row = p.v0 + tv * HF_V, rows = min(HF_V, p.classes - row);
         PA pa = {p.w + (int64_t)row * p.ldw, p.ldw, 0, rows, p.dim, (int64_t)(rows - 1) * p.ldw + p.dim};
@@ -411,6 +439,7 @@ template <bool GRAD, int HF_V> __global__ __launch_bounds__(256, 2) void head_lo
             head_leave_grad<MI, 1, false>(acc, lds, p, tv, 0, count, t);
             __syncthreads();
         } else {
+            head_pick(acc, 0, label - (row + wm * MI * 32), g, p.picked + tok);
             float m2, s2;
             head_stats(acc, 0, p.classes - (row + wm * MI * 32), g, m2, s2);
             head_join(m, s, m2, s2);
@@ -424,7 +453,7 @@ template <bool GRAD, int HF_V> __global__ __launch_bounds__(256, 2) void head_lo
         __syncthreads();
         if (wm == 0 && g == 0) {
             head_join(m, s, ms_[0][wn][r], ms_[1][wn][r]);
-            if (wn * 32 + r < count) p.part[(int64_t)blockIdx.x * p.tokens + wn * 32 + r] = float2{m, s};
+            if (tok < count) p.part[(int64_t)blockIdx.x * p.tokens + tok] = float2{m, s};
         }
     }
 }
@@ -534,14 +563,14 @@ template <int THREADS> __device__ __forceinline__ void head_sum(const HeadSum &p
 struct HeadMerge {
     float *stats;          // [tokens]: lse, 0 in ignored rows
     const float2 *part;    // [parts][tokens], by place
+    const float *picked;   // by place
     const int *pos;        // NULL: every row in its place
-    const void *x, *w;     // bf16: as the products have them, x by place; fp32: the caller's own
-    int64_t ldx, ldw, classes;
-    int parts, dim;        // bf16: a multiple of 8, zeros behind the last value
+    int64_t classes;
+    int parts;
     HeadSum sum;
 };
 // LANES lanes a token: many where the tokens are few and their parts a chain of loads.
-template <int LANES, bool F32> __global__ __launch_bounds__(1024) void head_merge_kernel(HeadMerge p)
+template <int LANES> __global__ __launch_bounds__(1024) void head_merge_kernel(HeadMerge p)
 {
     constexpr int TOK = 1024 / LANES;
     __shared__ float ms_[TOK][LANES + 1], ss_[TOK][LANES + 1];
@@ -563,33 +592,15 @@ template <int LANES, bool F32> __global__ __launch_bounds__(1024) void head_merg
     __syncthreads();
     const int tok = t / LANES, lane = t % LANES, at = place(r0 + tok);
     const int64_t row = r0 + tok;
-    float m = ms_[tok][lane], s = ss_[tok][lane], d = 0.0f;
+    float m = ms_[tok][lane], s = ss_[tok][lane];
     const int64_t c = at < 0 ? 0 : p.sum.target[row];
     const bool known = c >= 0 && c < p.classes;
-    if (at >= 0 && known) {
-        if constexpr (F32) {
-            const float *x = static_cast<const float *>(p.x) + row * p.ldx, *w = static_cast<const float *>(p.w) + c * p.ldw;
-#pragma unroll 4
-            for (int i = lane; i < p.dim; i += LANES) d = fmaf(x[i], w[i], d);
-        } else {
-            const bf16_t *x = static_cast<const bf16_t *>(p.x) + (int64_t)at * p.ldx, *w = static_cast<const bf16_t *>(p.w) + c * p.ldw;
-#pragma unroll 2
-            for (int i = lane * 8; i < p.dim; i += LANES * 8) {
-                const u32x4 a = *reinterpret_cast<const u32x4 *>(x + i), b = *reinterpret_cast<const u32x4 *>(w + i);
+    const float picked = at >= 0 && known && lane == 0 ? p.picked[at] : 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d = fmaf(lo_f32(a[e]), lo_f32(b[e]), fmaf(hi_f32(a[e]), hi_f32(b[e]), d));
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) {
-        head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
-        d += __shfl_xor(d, o, 64);
-    }
+    for (int o = 1; o < LANES; o <<= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
     if (lane == 0 && row < tokens) {
-        const float lse = (m + log2f(s)) * HD_LN2;
-        p.stats[row] = at < 0 ? 0.0f : lse;
-        head_leave_nll(p.sum, row, at < 0 ? 0.0f : known ? lse - d : __uint_as_float(0x7fc00000u));
+        p.stats[row] = at < 0 ? 0.0f : (m + log2f(s)) * HD_LN2;
+        head_leave_nll(p.sum, row, at < 0 ? 0.0f : known ? head_nll(fmaf(-picked, HD_LOG2E, m), s) : __uint_as_float(0x7fc00000u));
     }
     head_sum<1024>(p.sum);
 }
@@ -764,7 +775,7 @@ template <typename E> __global__ __launch_bounds__(256) void head_dx_kernel(E *_
 struct HeadRows {
     float *logits;         // [tokens][n], n classes from v0 on
     float *g;              // G, there or somewhere else
-    float2 *state;         // [tokens]: maximum (times log2 e) and sum of the pieces so far
+    float2 *state;         // [tokens]: maximum and sum of the pieces so far
     float *picked;         // [tokens]: the target's logit
     float *stats;
     int64_t classes;
@@ -795,23 +806,26 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void head_rows_stat
             s = s * __expf(m - ref) + __expf(v - ref);
             m = top;
         }
-    m *= HD_LOG2E;
+    auto join = [&](float m2, float s2) {
+        const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+        s = s * __expf(m - ref) + s2 * __expf(m2 - ref);
+        m = top;
+    };
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    for (int o = 32; o > 0; o >>= 1) join(__shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
     if ((t & 63) == 0) {
         ms_[t >> 6] = m;
         ss_[t >> 6] = s;
     }
     __syncthreads();
     if (t) return;
-    for (int w = 1; w < THREADS / 64; ++w) head_join(m, s, ms_[w], ss_[w]);
-    if (!p.first && counts) head_join(m, s, p.state[row].x, p.state[row].y);
+    for (int w = 1; w < THREADS / 64; ++w) join(ms_[w], ss_[w]);
+    if (!p.first && counts) join(p.state[row].x, p.state[row].y);
     float picked = p.first || !known || !counts ? 0.0f : p.picked[row];
     if (counts && known && c >= p.v0 && c < p.v0 + p.n) picked = l[c - p.v0];
     if (p.last) {
-        const float lse = (m + log2f(s)) * HD_LN2;
-        p.stats[row] = counts ? lse : 0.0f;
-        head_leave_nll(p.sum, row, !counts ? 0.0f : known ? lse - picked : __uint_as_float(0x7fc00000u));
+        p.stats[row] = counts ? m + log2f(s) * HD_LN2 : 0.0f;
+        head_leave_nll(p.sum, row, !counts ? 0.0f : known ? head_nll((m - picked) * HD_LOG2E, s) : __uint_as_float(0x7fc00000u));
     } else {
         p.state[row] = float2{m, s};
         p.picked[row] = picked;
@@ -1080,6 +1094,8 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
             h.picked = room(tokens * 4);
             h.g = room(tokens * h.vp * 4);
         } else {
+            if (!h.direct) h.label = room(tokens * 4);
+            h.picked = room(tokens * 4);
             h.parts = h.few ? head_few_blocks(classes) : (int)(2 * cdiv(classes, HD_TILE));
             h.part = room(h.parts * tokens * 8);
         }
@@ -1146,10 +1162,10 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
         p.target = c.target;
         p.pos = c.at<int>(h.pos);
         p.count = c.at<int>(h.count);
+        p.label = c.at<int>(h.label);
         if (h.backward) {
             p.lse2 = c.at<float>(h.lse2);
             p.factor = c.at<float>(h.factor);
-            p.label = c.at<int>(h.label);
             p.stats = stats;
             p.dloss = dloss_rows;
         }
@@ -1214,21 +1230,15 @@ static int head_fwd_tiles(const HeadCall &c, float *loss, float *stats, int redu
     p.dim = (int)h.dp;
     p.classes = (int)h.classes;
     p.part = c.at<float2>(h.part);
+    p.picked = c.at<float>(h.picked);
+    p.label = h.direct ? nullptr : c.at<int>(h.label);
+    p.target = h.direct ? c.target : nullptr;
     p.tokens = h.tokens;
     if (int rc = head_logits<false>(p, h.classes, h.few, c.s)) return rc;
-    const int *pos = h.direct ? nullptr : c.at<int>(h.pos);
+    const HeadMerge m = {stats, p.part, p.picked, h.direct ? nullptr : c.at<int>(h.pos), h.classes, h.parts, head_sum_of(c, loss, stats, reduction)};
     // 16 lanes a token from as many tokens on as give every other compute unit a block of 64
-    const bool many = h.tokens >= 8192;
-    const unsigned blocks = (unsigned)cdiv(h.tokens, many ? 64 : 16);
-    if (h.planes > 1) {
-        const HeadMerge m = {stats, p.part, pos, c.x, c.w, c.ldx, c.ldw, h.classes, h.parts, (int)h.dim, head_sum_of(c, loss, stats, reduction)};
-        if (many) head_merge_kernel<16, true><<<blocks, 1024, 0, c.s>>>(m);
-        else head_merge_kernel<64, true><<<blocks, 1024, 0, c.s>>>(m);
-    } else {
-        const HeadMerge m = {stats, p.part, pos, p.x, w, p.ldx, ldw, h.classes, h.parts, (int)h.dp, head_sum_of(c, loss, stats, reduction)};
-        if (many) head_merge_kernel<16, false><<<blocks, 1024, 0, c.s>>>(m);
-        else head_merge_kernel<64, false><<<blocks, 1024, 0, c.s>>>(m);
-    }
+    if (h.tokens >= 8192) head_merge_kernel<16><<<(unsigned)cdiv(h.tokens, 64), 1024, 0, c.s>>>(m);
+    else head_merge_kernel<64><<<(unsigned)cdiv(h.tokens, 16), 1024, 0, c.s>>>(m);
     return check_launch("head_merge_kernel");
 }
 template <typename E> static int head_bwd_tiles(const HeadCall &c, E *dx, E *dw, const float *dloss, const float *stats, int reduction)
