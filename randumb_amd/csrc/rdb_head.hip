@@ -36,6 +36,7 @@ int f32_split_mode();
 constexpr int HD_TILE = 256, HD_TOK = DUO_B;
 constexpr uint32_t HD_OOB = 0xfffffff0u;   // outside a buffer of any size up to 2^32 - 16 bytes
 constexpr float HD_LOG2E = 1.44269504088896340736f, HD_LN2 = 0.69314718055994530942f;
+constexpr float HD_FAR = 1024.0f;   // logits from which on their product with log2 e is rounded by 2^-14 or more, up to anything: subtracted before they are multiplied
 enum HeadReduction { HD_NONE = 0, HD_MEAN = 1, HD_SUM = 2 };
 
 // ----------------------------------------------------------------------------------------------- the rows that count
@@ -47,7 +48,7 @@ struct HeadGather {
     int *pos;                // [tokens]: where a row went, -1: ignored
     int *count;              // rows that count; behind it the counter of head_merge_kernel's blocks, cleared
     int *label;              // by place: target (-1: none of the classes)
-    float *lse2, *factor;    // backward, by place, or NULL: log2 of the row's sum, its own factor of G
+    float *lse, *factor;     // backward, by place, or NULL: logarithm of the row's sum, its own factor of G
     const float *stats;      // lse by row
     const float *dloss;      // [tokens], or NULL: 1
     int64_t tokens, dim, classes, ignore;
@@ -132,8 +133,8 @@ template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const He
             if (counts) {
                 const bool known = c >= 0 && c < p.classes;
                 p.label[at] = known ? (int)c : -1;
-                if (p.lse2) {
-                    p.lse2[at] = p.stats[r0 + lane] * HD_LOG2E;
+                if (p.lse) {
+                    p.lse[at] = p.stats[r0 + lane];
                     p.factor[at] = !known ? __uint_as_float(0x7fc00000u) : p.dloss ? p.dloss[r0 + lane] : 1.0f;
                 }
             }
@@ -250,20 +251,30 @@ struct HeadLogits {
     unsigned int *cleared;   // NULL, or a word that block 0 sets to zero for a later launch
     int dim, classes, v0;     // classes v0 .. v0 + tiles_v * 256 of this launch
     int tiles_v;
-    float2 *part;         // stats: [2 * tiles_v][tokens]: maximum (times log2 e) and sum
+    float2 *part;         // stats: [2 * tiles_v][tokens]: maximum and sum
     float *picked;        // stats, by place: the target's logit, from the tile that has it
     int64_t tokens;
     bf16_t *g;            // gradient: [tokens][ldg], class v0 first
     int64_t ldg;
     int plane, plane_g;   // fp32: values from plane to plane of x and w, of g
-    const float *lse2, *factor;
+    const float *lse, *factor;
     const int *label;
     const int64_t *target;   // few tokens as they are (count NULL): their targets, instead of labels
 };
 __device__ __forceinline__ int head_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
 
 // Tiles of MI * 64 classes x NI * 64 tokens, waves 2 x 2.
-// Maximum (times log2 e) and sum of exponentials over a wave's `left` classes, of its ni-th 32 tokens.
+// Where `ref` is far (classes masked by a type's lowest value, for one), it is taken from v at once: what is returned, or 0 (the other lanes' values keep their bits).
+template <int N> __device__ __forceinline__ float head_far(float ref, float (&v)[N])
+{
+    const float far = fabsf(ref) > HD_FAR ? ref : 0.0f;
+    if (__any(far != 0.0f)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] -= far;
+    }
+    return far;
+}
+// Maximum and sum of exponentials relative to it over a wave's `left` classes, of its ni-th 32 tokens.
 template <int MI, int NI> __device__ __forceinline__ void head_stats(const f32x16 (&acc)[MI][NI], int ni, int left, int g, float &m, float &s)
 {
     constexpr int N = MI * 16;
@@ -279,16 +290,17 @@ template <int MI, int NI> __device__ __forceinline__ void head_stats(const f32x1
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
-    m = fmaxf(m, __shfl_xor(m, 32, 64)) * HD_LOG2E;
-    const float ref = m == -INFINITY ? 0.0f : m;
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float ref = m == -INFINITY ? 0.0f : m, far = head_far(ref, v), scaled = far != 0.0f ? 0.0f : ref * HD_LOG2E;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], HD_LOG2E, -ref));
+    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f(fmaf(v[i], HD_LOG2E, -scaled));
     s += __shfl_xor(s, 32, 64);
+    s *= __builtin_amdgcn_exp2f(-fmaf(ref - far, HD_LOG2E, -scaled));   // what `scaled` was rounded by
 }
 __device__ __forceinline__ void head_join(float &m, float &s, float m2, float s2)
 {
     const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
+    s = s * __builtin_amdgcn_exp2f((m - ref) * HD_LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * HD_LOG2E);
     m = top;
 }
 // The logit of class `rel` of a wave's, where it has it, of its ni-th 32 tokens.  It has to be the one that is in the sum: from a sum of products in another order nll of a token
@@ -302,13 +314,13 @@ template <int MI, int NI> __device__ __forceinline__ void head_pick(const f32x16
         if ((i >> 4) * 32 + head_row(i & 15, g) == rel) v = acc[i >> 4][ni][i & 15];
     if ((unsigned)rel < (unsigned)(MI * 32) && ((rel >> 2) & 1) == g) *to = v;
 }
-// nll from what the maximum is above the target's logit (times log2 e) and the sum: what rounding a maximum that is held times log2 e has put into the sum, the same rounding in
-// `above` takes out again.  A sum has its target's own part, so that what is below zero is rounding.
-__device__ __forceinline__ float head_nll(float above, float s)
+// A sum has its target's own part, so that what is below zero is rounding.
+__device__ __forceinline__ float head_nll(float m, float s, float picked)
 {
-    const float v = above + log2f(s);
-    return v < 0.0f ? 0.0f : v * HD_LN2;
+    const float v = (m - picked) + log2f(s) * HD_LN2;
+    return v < 0.0f ? 0.0f : v;
 }
+__device__ __forceinline__ float head_lse(float m, float s) { return m + log2f(s) * HD_LN2; }
 // ... for each of the wave's tokens; each wave leaves its half of the classes' own
 template <int MI, int NI>
 __device__ __forceinline__ void head_leave_stats(const f32x16 (&acc)[MI][NI], const HeadLogits &p, int tv, int tok0, int count, int t)
@@ -336,7 +348,16 @@ __device__ __forceinline__ void head_leave_grad(f32x16 (&acc)[MI][NI], bf16_t *_
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
         const int b = wn * NI * 32 + ni * 32 + r, tok = min(tok0 + b, count - 1);
-        const float l = p.lse2[tok], f = p.factor[tok];
+        const float lse = p.lse[tok], f = p.factor[tok];
+        const bool far = fabsf(lse) > HD_FAR;
+        const float l = far ? 0.0f : lse * HD_LOG2E;
+        if (__any(far)) {   // as head_far; no value above 1, whatever the logits' own rounding, which the forward pass may have had to the other side
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float v = acc[i >> 4][ni][i & 15], d = v - lse;
+                acc[i >> 4][ni][i & 15] = !far ? v : d > 0.0f ? 0.0f : d;
+            }
+        }
         const int rel = p.label[tok] - first;
         if constexpr (PLANES) {   // in place
 #pragma unroll
@@ -599,8 +620,8 @@ template <int LANES> __global__ __launch_bounds__(1024) void head_merge_kernel(H
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
     if (lane == 0 && row < tokens) {
-        p.stats[row] = at < 0 ? 0.0f : (m + log2f(s)) * HD_LN2;
-        head_leave_nll(p.sum, row, at < 0 ? 0.0f : known ? head_nll(fmaf(-picked, HD_LOG2E, m), s) : __uint_as_float(0x7fc00000u));
+        p.stats[row] = at < 0 ? 0.0f : head_lse(m, s);
+        head_leave_nll(p.sum, row, at < 0 ? 0.0f : known ? head_nll(m, s, picked) : __uint_as_float(0x7fc00000u));
     }
     head_sum<1024>(p.sum);
 }
@@ -806,26 +827,21 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void head_rows_stat
             s = s * __expf(m - ref) + __expf(v - ref);
             m = top;
         }
-    auto join = [&](float m2, float s2) {
-        const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
-        s = s * __expf(m - ref) + s2 * __expf(m2 - ref);
-        m = top;
-    };
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) join(__shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    for (int o = 32; o > 0; o >>= 1) head_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
     if ((t & 63) == 0) {
         ms_[t >> 6] = m;
         ss_[t >> 6] = s;
     }
     __syncthreads();
     if (t) return;
-    for (int w = 1; w < THREADS / 64; ++w) join(ms_[w], ss_[w]);
-    if (!p.first && counts) join(p.state[row].x, p.state[row].y);
+    for (int w = 1; w < THREADS / 64; ++w) head_join(m, s, ms_[w], ss_[w]);
+    if (!p.first && counts) head_join(m, s, p.state[row].x, p.state[row].y);
     float picked = p.first || !known || !counts ? 0.0f : p.picked[row];
     if (counts && known && c >= p.v0 && c < p.v0 + p.n) picked = l[c - p.v0];
     if (p.last) {
-        p.stats[row] = counts ? m + log2f(s) * HD_LN2 : 0.0f;
-        head_leave_nll(p.sum, row, !counts ? 0.0f : known ? head_nll((m - picked) * HD_LOG2E, s) : __uint_as_float(0x7fc00000u));
+        p.stats[row] = counts ? head_lse(m, s) : 0.0f;
+        head_leave_nll(p.sum, row, !counts ? 0.0f : known ? head_nll(m, s, picked) : __uint_as_float(0x7fc00000u));
     } else {
         p.state[row] = float2{m, s};
         p.picked[row] = picked;
@@ -843,7 +859,8 @@ __global__ __launch_bounds__(256) void head_rows_grad_kernel(HeadRows p)
     if (counts)
 #pragma unroll 4
         for (int i = begin + (int)threadIdx.x; i < end; i += 256) {
-            float v = expf(l[i] - lse);
+            const float e = expf(l[i] - lse);
+            float v = e > 1.0f ? 1.0f : e;   // logits of another kernel's may be rounded to the other side
             if (i == label) v -= 1.0f;
             out[i] = v * f;
         }
@@ -1031,7 +1048,7 @@ struct HeadPlan {
     int parts;                 // of a token's sum
     int64_t split_v;
     // offsets in the workspace
-    int64_t xc, pos, count, lse2, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
+    int64_t xc, pos, count, lse, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
 };
 // Tokens up to which a copy of the rows that count costs more than leaving some out gains: one tile of tokens either way.
 constexpr int64_t HD_FEW = HF_T;
@@ -1101,7 +1118,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         }
     } else {
         if (!f32) {
-            h.lse2 = room(tokens * 4);
+            h.lse = room(tokens * 4);
             h.factor = room(tokens * 4);
             h.label = room(tokens * 4);
         }
@@ -1164,7 +1181,7 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
         p.count = c.at<int>(h.count);
         p.label = c.at<int>(h.label);
         if (h.backward) {
-            p.lse2 = c.at<float>(h.lse2);
+            p.lse = c.at<float>(h.lse);
             p.factor = c.at<float>(h.factor);
             p.stats = stats;
             p.dloss = dloss_rows;
@@ -1269,7 +1286,7 @@ template <typename E> static int head_bwd_tiles(const HeadCall &c, E *dx, E *dw,
         p.tokens = h.tokens;
         p.g = c.at<bf16_t>(h.g) + (i & 1) * h.tokens * h.vp * h.planes;
         p.ldg = h.planes * h.vp;
-        p.lse2 = c.at<float>(h.lse2);
+        p.lse = c.at<float>(h.lse);
         p.factor = c.at<float>(h.factor);
         p.label = c.at<int>(h.label);
         return p;
