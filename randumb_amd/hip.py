@@ -879,10 +879,22 @@ def _rows(t: torch.Tensor, near: bool = False) -> torch.Tensor:
     return t if fits else t.contiguous()
 
 
+def _check_head(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: int) -> None:
+    if x.dtype not in _DT or weight.dtype != x.dtype:
+        raise TypeError(f"linear_cross_entropy: x and weight both bfloat16 or both float32, got {x.dtype} and {weight.dtype}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"linear_cross_entropy: target int64, got {target.dtype}")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or target.shape != x.shape[:1] or weight.numel() == 0:
+        raise ValueError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)} do not go together")
+    if reduction not in (0, 1, 2):
+        raise ValueError(f"linear_cross_entropy: reduction must be 0, 1 or 2, got {reduction}")
+
+
 def linear_cross_entropy_fwd(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int, reduction: int):
     """``(loss, stats)`` of the rows ``x`` (tokens, dim) and the weight (classes, dim), both fp32 or both bf16, for int64 targets; reduction 0: a loss
     for each row, 1: their mean, 2: their sum.  ``stats`` (fp32, tokens + 1) is what the backward call needs."""
     _need_gpu("linear_cross_entropy", x, weight, target)
+    _check_head(x, weight, target, reduction)
     x, w, t = _rows(x, True), _rows(weight), target.contiguous()
     tokens, dim = x.shape
     dev, L = x.device, _lib.load()
@@ -903,6 +915,7 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
                              want_dx: bool = True, want_dw: bool = True):
     """``(dx, dweight)`` of :func:`linear_cross_entropy_fwd`, ``None`` where not wanted; ``dloss`` one value, or one for each row with reduction 0."""
     _need_gpu("linear_cross_entropy", dloss, stats, x, weight, target)
+    _check_head(x, weight, target, reduction)
     x, w, t, d, stats = _rows(x, True), _rows(weight), target.contiguous(), dloss.to(torch.float32).contiguous(), stats.contiguous()
     tokens, dim = x.shape
     if d.numel() != (tokens if reduction == 0 else 1) or stats.dtype != torch.float32 or stats.numel() != tokens + 1:
@@ -921,9 +934,21 @@ def linear_cross_entropy_bwd(dloss: torch.Tensor, stats: torch.Tensor, x: torch.
     return dx, dw
 
 
+def check_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, positions: Optional[torch.Tensor]) -> None:
+    if q.dtype not in (torch.float32, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
+        raise TypeError(f"rotary: queries and keys both bfloat16 or both float32, got {q.dtype}" + ("" if k is None else f" and {k.dtype}"))
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError(f"rotary: queries {tuple(q.shape)}" + ("" if k is None else f" and keys {tuple(k.shape)}") + " are not (batch, time, heads, head_dim)")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= q.shape[3] or inv_freq.numel() > 1024:
+        raise ValueError(f"rotary: float32 frequencies, one for each pair of a head's {q.shape[3]} values (1024 at most), got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if positions is not None and (positions.dtype not in (torch.int64, torch.int32) or positions.shape not in (q.shape[1:2], q.shape[:2], (1, q.shape[1]))):
+        raise ValueError(f"rotary: positions int64 or int32 of shape (time,) or (batch, time), got {positions.dtype} {tuple(positions.shape)}")
+
+
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, positions: Optional[torch.Tensor], interleaved: bool, scale: float, inverse: bool = False):
     """``(q, k)`` (batch, time, heads, head_dim) turned by their positions; ``inverse``: the other way round, which is the gradient."""
     _need_gpu("rotary", q, k, inv_freq, positions)
+    check_rotary(q, k, inv_freq, positions)
     q, k = (None if t is None else t if t.stride(-1) == 1 else t.contiguous() for t in (q, k))
     out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
     rows = [None if t is None else ctypes.byref(_lib.RotaryRows(o.data_ptr(), t.data_ptr(), t.shape[2], t.stride(0), t.stride(1), t.stride(2)))

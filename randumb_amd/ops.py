@@ -593,17 +593,6 @@ def _rotary_backward(ctx, grads):
 _rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup_context)
 
 
-def _check_rotary(q, k, inv_freq, positions) -> None:
-    if q.dtype not in (torch.float32, torch.bfloat16) or (k is not None and k.dtype != q.dtype):
-        raise TypeError(f"rotary: queries and keys both bfloat16 or both float32, got {q.dtype}" + ("" if k is None else f" and {k.dtype}"))
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-        raise ValueError(f"rotary: queries {tuple(q.shape)}" + ("" if k is None else f" and keys {tuple(k.shape)}") + " are not (batch, time, heads, head_dim)")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= q.shape[3] or inv_freq.numel() > 1024:
-        raise ValueError(f"rotary: float32 frequencies, one for each pair of a head's {q.shape[3]} values (1024 at most), got {inv_freq.dtype} {tuple(inv_freq.shape)}")
-    if positions is not None and (positions.dtype not in (torch.int64, torch.int32) or positions.shape not in (q.shape[1:2], q.shape[:2], (1, q.shape[1]))):
-        raise ValueError(f"rotary: positions int64 or int32 of shape (time,) or (batch, time), got {positions.dtype} {tuple(positions.shape)}")
-
-
 def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional[Tensor] = None, *, interleaved: bool = False, scale: float = 1.0):
     """Queries (batch, time, heads, head_dim) and keys (batch, time, kv_heads, head_dim), or queries alone (``k`` None), turned by their positions, in one
     launch; returns both.  Of every head the first ``2 * len(inv_freq)`` values are pairs, value i with the one half of them
@@ -617,10 +606,10 @@ def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional
         try:   # which checks the same: 2 of the 9 us of a call go to saying what is wrong with it
             both = (_lib._ext or _lib.extension()).rotary(q, k, inv_freq, positions, interleaved, scale)
         except (TypeError, ValueError, RuntimeError):
-            _check_rotary(q, k, inv_freq, positions)
+            hip.check_rotary(q, k, inv_freq, positions)
             raise
     if both is None:
-        _check_rotary(q, k, inv_freq, positions)
+        hip.check_rotary(q, k, inv_freq, positions)
         both = _rotary(q, k, inv_freq.detach(), positions, bool(interleaved), scale, False)
     return both[0], None if k is None else both[1]
 
