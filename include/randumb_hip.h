@@ -564,7 +564,7 @@ int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const vo
  * a time (bf16: rounded to bf16 without the factor that its rows share).  Sums in fixed orders: results are bitwise reproducible.
  * fp32 of many tokens runs on the bf16 matrix cores in three planes, which take 1.5 times the weight's bytes of the workspace.  Infinities in w are what they are in a product at every
  * size: a class whose logit is -infinity counts for nothing.
- * The workspace's size depends on where x and w begin.  RDB_E_UNSUPPORTED: x of 2^29 values or more, 2^21 rows or more, ldw of 2^20 or more,
+ * The workspace's size depends on where x and w begin; of its query `backward` is 1 for a backward call, 0 for a forward call and 2 for a forward call that is given a buffer of logits.  RDB_E_UNSUPPORTED: x of 2^29 values or more, 2^21 rows or more, ldw of 2^20 or more,
  * 2^38 logits or more in tiles of 128 x 256 (size query: 0). */
 int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
                                                  int backward, int want_dx, int want_dw);

@@ -1053,7 +1053,7 @@ struct HeadPlan {
 // Tokens up to which a copy of the rows that count costs more than leaving some out gains: one tile of tokens either way.
 constexpr int64_t HD_FEW = HF_T;
 
-static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw, bool backward, bool want_dx, bool want_dw, bool wide_x, bool pack_w)
+static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtype, int64_t ldw, bool backward, bool want_dx, bool want_dw, bool wide_x, bool pack_w, bool kept)
 {
     HeadPlan h = {};
     h.tokens = tokens;
@@ -1109,7 +1109,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
         if (f32) {
             h.part = room(tokens * 8);
             h.picked = room(tokens * 4);
-            h.g = room(tokens * h.vp * 4);
+            if (!kept) h.g = room(tokens * h.vp * 4);   // logits that are kept have a buffer of the caller's
         } else {
             if (!h.direct) h.label = room(tokens * 4);
             h.picked = room(tokens * 4);
@@ -1456,17 +1456,11 @@ static int check_head(const char *who, int64_t tokens, int64_t dim, int64_t clas
 
 using namespace rdb;
 
-static HeadPlan head_plan_of(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, bool backward, bool want_dx, bool want_dw)
+static HeadPlan head_plan_of(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, bool backward, bool want_dx, bool want_dw,
+                             bool kept)
 {
     const bool whole = dim % 8 == 0;
-    return head_plan(tokens, dim, classes, dtype, ldw, backward, want_dx, want_dw, whole && head_aligned(x, ldx, 2) && ldx < (1ll << 20), !whole || !head_aligned(w, ldw, 2));
-}
-
-extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
-                                                            int backward, int want_dx, int want_dw)
-{
-    if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, ldx, ldw, 0)) return 0;
-    return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward != 0, want_dx != 0, want_dw != 0).total;
+    return head_plan(tokens, dim, classes, dtype, ldw, backward, want_dx, want_dw, whole && head_aligned(x, ldx, 2) && ldx < (1ll << 20), !whole || !head_aligned(w, ldw, 2), kept);
 }
 
 // A product less in a backward pass that few tokens leave bound by the weight: us a step, computed again | kept: 12 tokens x 2048 -> 47643 407 | 306, 69 x 2723 -> 55040 1107 | 862,
@@ -1475,7 +1469,15 @@ extern "C" int64_t rdb_linear_cross_entropy_keeps(int64_t tokens, int64_t dim, i
 {
     if (check_head("rdb_linear_cross_entropy_keeps", tokens, dim, classes, dtype, dim, ldw, 0)) return 0;
     if (dtype != RDB_F32 || !head_keepable(tokens, dim, classes)) return 0;
-    return head_plan(tokens, dim, classes, dtype, ldw, true, true, true, false, false).pieces == 1 ? tokens * classes : 0;
+    return head_plan(tokens, dim, classes, dtype, ldw, true, true, true, false, false, false).pieces == 1 ? tokens * classes : 0;
+}
+
+extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t dim, int64_t classes, int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                                                            int backward, int want_dx, int want_dw)
+{
+    if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, ldx, ldw, 0)) return 0;
+    const bool kept = backward == 2 && rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw);
+    return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward == 1, want_dx != 0, want_dw != 0, kept).total;
 }
 
 extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
@@ -1485,9 +1487,9 @@ extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *lo
     constexpr const char *who = "rdb_linear_cross_entropy_fwd";
     if (int rc = check_head(who, tokens, dim, classes, dtype, ldx, ldw, reduction)) return rc;
     if (!loss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
-    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, false, false, false);
-    if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
+    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, false, false, false, logits != nullptr);
+    if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};
     return h.tiles ? head_fwd_tiles(c, loss, stats, reduction) : head_fwd_f32(c, loss, stats, logits, reduction);
 }
@@ -1501,7 +1503,7 @@ extern "C" int rdb_linear_cross_entropy_bwd(void *dx, void *dw, const float *dlo
     if (!dx && !dw) return RDB_OK;
     if (!dloss || !stats || !x || !w || !target) return set_error(RDB_E_NULL, "%s: an argument is NULL", who);
     if (((uintptr_t)dx & 15) || ((uintptr_t)dw & 15)) return set_error(RDB_E_ALIGN, "%s: dx and dw must be 16-byte aligned", who);
-    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, true, dx != nullptr, dw != nullptr);
+    const HeadPlan h = head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, true, dx != nullptr, dw != nullptr, logits != nullptr);
     if (!workspace || workspace_bytes < h.total || ((uintptr_t)workspace & 15)) return set_error(RDB_E_WORKSPACE, "%s: needs %lld bytes from a 16-byte boundary on", who, (long long)h.total);
     if (logits && !rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw)) return set_error(RDB_E_UNSUPPORTED, "%s: logits of this size are not kept", who);
     const HeadCall c = {h, static_cast<char *>(workspace), x, w, ldx, ldw, target, ignore_index, (hipStream_t)stream};

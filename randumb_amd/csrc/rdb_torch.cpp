@@ -1150,7 +1150,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
     {
         return t.stride(1) == 1 && ld(t) >= t.size(1) && ld(t) < (1 << 20) && !(near && t.size(0) * ld(t) >= (1ll << 29)) ? t : t.contiguous();
     }
-    static Tensor forward(AutogradContext *ctx, const Tensor &x0, const Tensor &w0, const Tensor &target0, int64_t ignore, int64_t reduction)
+    static Tensor forward(AutogradContext *ctx, const Tensor &x0, const Tensor &w0, const Tensor &target0, int64_t ignore, int64_t reduction, bool differentiated)
     {
         const Tensor x = rows(x0, true), w = rows(w0), target = target0.contiguous();
         const c10::OptionalDeviceGuard guard(x.device());
@@ -1158,10 +1158,10 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
         const auto f32 = x.options().dtype(at::kFloat);
         Tensor loss = reduction ? at::empty({}, f32) : at::empty({tokens}, f32), stats = at::empty({tokens + 1}, f32), logits;
         if (tokens) {
-            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), 0, 0, 0);
+            const int64_t kept = differentiated ? rdb_linear_cross_entropy_keeps(tokens, dim, classes, code(x.scalar_type()), ld(w)) : 0;
+            if (kept) logits = at::empty({kept}, f32);
+            const int64_t need = rdb_linear_cross_entropy_workspace_bytes(tokens, dim, classes, code(x.scalar_type()), x.data_ptr(), ld(x), w.data_ptr(), ld(w), kept ? 2 : 0, 0, 0);
             const Tensor ws = bytes(need, x);
-            if (const int64_t n = x0.requires_grad() || w0.requires_grad() ? rdb_linear_cross_entropy_keeps(tokens, dim, classes, code(x.scalar_type()), ld(w)) : 0)
-                logits = at::empty({n}, f32);
             check(rdb_linear_cross_entropy_fwd(loss.data_ptr<float>(), stats.data_ptr<float>(), static_cast<float *>(ptr(logits)), x.data_ptr(), ld(x), w.data_ptr(), ld(w), code(x.scalar_type()),
                                                target.data_ptr<int64_t>(), tokens, dim, classes, ignore, (int)reduction, ptr(ws), need, stream_of(x)),
                   "rdb_linear_cross_entropy_fwd");
@@ -1176,7 +1176,7 @@ class LinearCrossEntropy : public Function<LinearCrossEntropy> {
     {
         auto d = gradients(ctx, grads[0]);
         for (Tensor &t : d) t = once_differentiable("linear_cross_entropy", t, grads[0], {0, 1});
-        return {d[0], d[1], Tensor(), Tensor(), Tensor()};
+        return {d[0], d[1], Tensor(), Tensor(), Tensor(), Tensor()};
     }
     static variable_list gradients(AutogradContext *ctx, const Tensor &grad)
     {
@@ -1568,7 +1568,7 @@ PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (x.dim() != 2 || w.dim() != 2 || t.dim() != 1 || x.size(1) != w.size(1) || t.size(0) != x.size(0) || !w.numel() || t.scalar_type() != at::kLong ||
             !readable(x.scalar_type()) || w.scalar_type() != x.scalar_type() || reduction < 0 || reduction > 2)
             fail(PyExc_ValueError, "linear_cross_entropy needs x (tokens, dim) and a weight (classes, dim) of one type, int64 targets (tokens) and a reduction 0, 1 or 2");
-        return THPVariable_Wrap(LinearCrossEntropy::apply(x, w, t, int_arg(a[3]), reduction));
+        return THPVariable_Wrap(LinearCrossEntropy::apply(x, w, t, int_arg(a[3]), reduction, at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad())));
     });
 }
 
