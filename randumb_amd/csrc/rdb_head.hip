@@ -1,5 +1,5 @@
 // Softmax cross entropy of an output head, x . W^T over a large vocabulary, and its gradient, in pieces of the vocabulary: the logits are
-// never kept whole (but those of few tokens in fp32), and neither is their gradient.
+// never kept whole (but those of few tokens in fp32); of their gradient there are two pieces at a time.
 //
 //   lse[t] = log sum_v exp <x_t, w_v>,  nll[t] = lse[t] - <x_t, w_target[t]>,  loss = their mean, their sum, or nll itself
 //   G[t][v] = (exp(<x_t, w_v> - lse[t]) - [v == target[t]]) g_t,   dx = G . W,   dW = G^T . x

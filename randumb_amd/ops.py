@@ -539,9 +539,10 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
-    """``F.cross_entropy(F.linear(x, weight).float(), target, ignore_index=..., reduction=...)`` for a large vocabulary, with its gradients and without
-    the logits: neither they nor their gradient are ever in memory beyond a piece of the vocabulary (fp32 of up to dim / 4 tokens keeps up to 256 MB of them from
-    the forward to the backward pass).
+    """``F.cross_entropy(F.linear(x, weight).float(), target, ignore_index=..., reduction=...)`` for a large vocabulary, with its gradients, in pieces of the
+    vocabulary instead of whole logits.  Between the passes it keeps a value a token (fp32 of up to dim / 4 tokens: up to 256 MB of logits).  While it runs it needs, forward, 8 bytes for
+    every 128 logits, or a piece of 256 MB of them; backward two pieces of their gradient of 128 to 512 MB each, which is all of it where that is less (bf16: 2 bytes a value,
+    fp32 of many tokens: 6); and copies of weights that are not read as they are (bf16 rows of no multiple of 16 bytes, fp32 of many tokens: 6 bytes a value).
 
     ``x`` (..., dim) and ``weight`` (classes, dim): both bf16 or both fp32, on one GPU; ``target`` (...): int64 or int32.  The loss is fp32; logits are
     not rounded on the way.  Tokens whose target is ``ignore_index`` are left out (in bf16, and in fp32 of many tokens, before anything is multiplied): what their rows hold does not matter.  The mean over no tokens is
