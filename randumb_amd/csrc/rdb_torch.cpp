@@ -1119,7 +1119,7 @@ class CausalAttention : public Function<CausalAttention> {
 
 // ----------------------------------------------------------------------------------------------- ends of a language model
 // A leaf's gradient goes to its accumulator on the stream on which that was made, and a capture under way would take in that stream and could not end: the process would.  So
-// an accumulator that an older graph keeps alive, made on a stream outside of the capture, is refused.
+// an accumulator that an older graph keeps alive, made on a stream outside of the capture, is refused: a leaf's own, and one behind nodes of one input each (a reshaped, sliced or cast leaf).
 void no_leaves_outside_capture(const char *who, const Tensor &grad)
 {
     const auto here = c10::hip::getCurrentHIPStream(grad.get_device());
@@ -1130,9 +1130,19 @@ void no_leaves_outside_capture(const char *who, const Tensor &grad)
     if (!capturing(here.stream())) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
+    auto only = [](torch::autograd::Node &n) -> torch::autograd::Node * {   // the one node behind n, or none
+        torch::autograd::Node *one = nullptr;
+        for (const auto &edge : n.next_edges()) {
+            if (edge.function && one) return nullptr;
+            if (edge.function) one = edge.function.get();
+        }
+        return one;
+    };
     for (const auto &edge : node->next_edges()) {
-        if (!edge.function || edge.function->name() != "torch::autograd::AccumulateGrad") continue;
-        const auto there = edge.function->stream();   // its device is called by the other name that autograd has for it
+        torch::autograd::Node *leaf = edge.function.get();
+        while (leaf && leaf->name() != "torch::autograd::AccumulateGrad") leaf = only(*leaf);
+        if (!leaf) continue;
+        const auto there = leaf->stream();   // its device is called by the other name that autograd has for it
         if (!there || (there->id() == here.id() && there->device_index() == here.device_index())) continue;
         if (!capturing(c10::hip::HIPStream(c10::Stream(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, there->device_index()), there->id())).stream()))
             fail(PyExc_RuntimeError, std::string(who) + ": captured while an earlier graph of the same leaf, made on another stream, is alive: drop what holds it (a loss, an output), or "
