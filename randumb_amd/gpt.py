@@ -290,7 +290,7 @@ class RT_GPT(nn.Module):
             w = head._parameters.get("weight")
             if not _unhooked(head) or head.bias is not None or w is None or w.dtype != x.dtype:
                 return None
-            return ops.linear_cross_entropy(x, w, target)
+            return ops.linear_cross_entropy(x.reshape(-1, x.shape[-1]), w, target.reshape(-1))
         if type(head) is not RT_CastedLinear or RT_CastedLinear.forward is not _LINEAR_FORWARD or not _unhooked(head):
             return None
         w, coef = head.weight, head.weight_coef
