@@ -134,9 +134,11 @@ class RT_CausalSelfAttention(nn.Module):
         B, T, D = x.shape
         qkv = self.c_qkv(x)
         ext = _fused(qkv)
-        stock = getattr(self.rotary, "stock", True)   # somebody's own rotation is called with one side at a time
+        stock = getattr(self.rotary, "stock", True)
+        # somebody's own rotation, and one with hooks, is called with one side at a time
+        both = not stock and type(self.rotary) is Rotary and Rotary.forward is _ROTARY_FORWARD and _unhooked(self.rotary)
         # q and k that turn without becoming longer may do so before they are normalised as well as behind: the kernel that normalises them then has nothing to turn
-        turned = not stock and type(self.rotary) is Rotary and self.rotary.scale == 1.0
+        turned = both and self.rotary.scale == 1.0
         if ext is not None and (stock or turned) and D == 64 * self.n_head and 0 < T * 3 * D < 1 << 29 and B > 0:
             if turned:
                 q, k, v = qkv.split(D, 2)
@@ -148,7 +150,7 @@ class RT_CausalSelfAttention(nn.Module):
                 return self.c_proj(y)
         q, k, v = qkv.view(B, T, 3, self.n_head, D // self.n_head).unbind(2)
         q, k = RT_norm(q), RT_norm(k)
-        q, k = (self.rotary(q), self.rotary(k)) if stock else self.rotary.both(q, k)
+        q, k = self.rotary.both(q, k) if both else (self.rotary(q), self.rotary(k))
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
         return self.c_proj(y.transpose(1, 2).reshape(B, T, D))
 
@@ -246,7 +248,8 @@ class RT_Block(nn.Module):
 
 
 # as they stand here: replaced ones are called
-_BLOCK_FORWARD, _LINEAR_FORWARD, _EMBEDDING_FORWARD, _DENSE_FORWARD, _MODULE_CALL = RT_Block.forward, RT_CastedLinear.forward, nn.Embedding.forward, nn.Linear.forward, nn.Module.__call__
+_BLOCK_FORWARD, _LINEAR_FORWARD, _EMBEDDING_FORWARD, _DENSE_FORWARD = RT_Block.forward, RT_CastedLinear.forward, nn.Embedding.forward, nn.Linear.forward
+_ROTARY_FORWARD, _MODULE_CALL = Rotary.forward, nn.Module.__call__
 
 
 def _embed(wte: nn.Module, idx: torch.Tensor) -> torch.Tensor:
