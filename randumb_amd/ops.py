@@ -624,7 +624,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optio
     "linear"    positions divided by ``factor``
     "base"      a larger base, ``base * factor ** (rotary_dim / (rotary_dim - 2))``: the lowest frequency divided by ``factor``, the highest kept
     "parts"     by the number of turns that a pair makes in ``original_context`` positions: divided by ``factor`` up to ``low`` turns, kept from ``high`` turns
-                on, a linear mixture by the pair's index in between, with ``scale = 0.1 ln(factor) + 1``"""
+                on, a mixture linear in that number in between, with ``scale = 0.1 ln(factor) + 1``: the interpolation by parts and the temperature of "YaRN:
+                Efficient Context Window Extension of Large Language Models" (Peng et al., 2023)"""
     if rotary_dim < 2 or rotary_dim % 2 or not base > 0 or not factor > 0:
         raise ValueError(f"rotary_frequencies: an even number of values, a positive base and factor, got {rotary_dim}, {base}, {factor}")
     if scaling not in (None, "linear", "base", "parts") or (scaling is None and factor != 1.0):
@@ -639,13 +640,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optio
     if scaling == "linear":
         freq = freq / factor
     if scaling == "parts":
-        if original_context < 1 or not 0 < low < high or base == 1.0:
+        if original_context < 1 or not 0 < low < high:
             raise ValueError(f"rotary_frequencies: parts of an original context and 0 < low < high, got {original_context}, {low}, {high}")
-        # the pair that makes n turns: original_context * base ** (-2 i / rotary_dim) = 2 pi n
-        first, last = (rotary_dim * math.log(original_context / (2 * math.pi * n)) / (2 * math.log(base)) for n in (high, low))
-        first, last = max(math.floor(first), 0), min(math.ceil(last), rotary_dim - 1)
-        stretched = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
-        freq = freq * (1 - stretched) + freq / factor * stretched
+        kept = ((original_context / (2 * math.pi) * freq - low) / (high - low)).clamp(0, 1)
+        freq = freq * kept + freq / factor * (1 - kept)
         scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
     return freq.to(torch.float32).to(device), scale
 
