@@ -598,7 +598,8 @@ def rotary(q: Tensor, k: Optional[Tensor], inv_freq: Tensor, positions: Optional
     """Queries (batch, time, heads, head_dim) and keys (batch, time, kv_heads, head_dim), or queries alone (``k`` None), turned by their positions, in one
     launch; returns both.  Of every head the first ``2 * len(inv_freq)`` values are pairs, value i with the one half of them
     on, or neighbours (``interleaved``): ``(a, b) -> (a cos + b sin, b cos - a sin)``, the direction of :class:`randumb_amd.gpt.Rotary`, with the angle
-    ``position * inv_freq[i]`` formed in 64 bits and cosine and sine times ``scale``; the rest passes through.
+    ``position * inv_freq[i]`` formed in 64 bits and cosine and sine times ``scale``; the rest passes through.  That is a turn by the negative angle.  Negated frequencies give the
+    other direction, ``(a cos - b sin, b cos + a sin)``, in which many models were trained: their queries and keys need ``-inv_freq``.
 
     bf16 or fp32, any strides (unit inner ones are read in place), arithmetic in fp32, rounded once.  ``inv_freq``: fp32 (:func:`rotary_frequencies`).  ``positions``:
     int64 or int32, (time,) or (batch, time), any integers; None: 0, 1, ...  Gradients of any order for q and k, none for the frequencies."""
@@ -625,7 +626,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optio
     "base"      a larger base, ``base * factor ** (rotary_dim / (rotary_dim - 2))``: the lowest frequency divided by ``factor``, the highest kept
     "parts"     by the number of turns that a pair makes in ``original_context`` positions: divided by ``factor`` up to ``low`` turns, kept from ``high`` turns
                 on, a mixture linear in that number in between, with ``scale = 0.1 ln(factor) + 1``: the interpolation by parts and the temperature of "YaRN:
-                Efficient Context Window Extension of Large Language Models" (Peng et al., 2023)"""
+                Efficient Context Window Extension of Large Language Models" (Peng et al., 2023)
+
+    Negated frequencies turn the other way, as :func:`rotary` says."""
     if rotary_dim < 2 or rotary_dim % 2 or not base > 0 or not factor > 0:
         raise ValueError(f"rotary_frequencies: an even number of values, a positive base and factor, got {rotary_dim}, {base}, {factor}")
     if scaling not in (None, "linear", "base", "parts") or (scaling is None and factor != 1.0):
