@@ -46,6 +46,7 @@ struct HeadGather {
     int64_t ldx, ldc;
     const int64_t *target;
     int *pos;                // [tokens]: where a row went, -1: ignored
+    const int *counts;       // rows that count of every HD_COUNT, or NULL
     int *count;              // rows that count; behind it the counter of head_merge_kernel's blocks, cleared
     int *label;              // by place: target (-1: none of the classes)
     float *lse, *factor;     // backward, by place, or NULL: logarithm of the row's sum, its own factor of G
@@ -108,7 +109,25 @@ __device__ __forceinline__ void head_split8(bf16_t *to, int plane, const float *
 #pragma unroll
     for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4 *>(to + i * plane) = v[i];
 }
-// Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.
+// Blocks count the rows before theirs themselves: 64 KB of targets for the last one of 8192, out of L2.  Of more than HD_COUNTED tokens, where that would grow with their square (2^20: 3700 us
+// beside 400 of the logits' launch at 64 -> 1000; 131072: 75; 16384: 16), a launch has counted every HD_COUNT rows (62 and 15 us with it).
+constexpr int HD_COUNT = 1024, HD_COUNTED = 16384;
+__global__ __launch_bounds__(256) void head_count_kernel(int *__restrict__ counts, const int64_t *__restrict__ target, int64_t tokens, int64_t ignore)
+{
+    __shared__ int n_[4];
+    const int t = threadIdx.x;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < HD_COUNT / 256; ++e) {
+        const int64_t i = (int64_t)blockIdx.x * HD_COUNT + e * 256 + t;
+        n += i < tokens && target[i] != ignore ? 1 : 0;
+    }
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
+    if ((t & 63) == 0) n_[t >> 6] = n;
+    __syncthreads();
+    if (t == 0) counts[blockIdx.x] = n_[0] + n_[1] + n_[2] + n_[3];
+}
 template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const HeadGather &p, int block)
 {
     __shared__ int before_[4], place_[64];
@@ -117,8 +136,13 @@ template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const He
     const int mine = p.tokens - r0 < p.rows ? (int)(p.tokens - r0) : p.rows;
     const int64_t c = wave == 0 && lane < mine ? p.target[r0 + lane] : p.ignore;
     int n = 0;
+    int64_t counted = 0;
+    if (p.counts) {
+        counted = r0 / HD_COUNT * HD_COUNT;
+        for (int i = t; i < (int)(r0 / HD_COUNT); i += 256) n += p.counts[i];
+    }
 #pragma unroll 16
-    for (int64_t i = t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
+    for (int64_t i = counted + t; i < r0; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) n += __shfl_xor(n, m, 64);
     if (lane == 0) before_[wave] = n;
@@ -178,7 +202,7 @@ template <bool PLANES> __device__ __forceinline__ void head_gather_rows(const He
 }
 
 // Rows of `cols` bf16 values into rows of a multiple of 8 of them (PAD, zeros behind the last ones) or out of them into rows without gaps; a lane reads 8 values at any address
-// and writes them to a multiple of 16 bytes.  per_block: a multiple of 8, at most 8192 values; out of padded rows it reads up to 14 bytes behind the last of them.
+// and writes them to a multiple of 16 bytes.  per_block: a multiple of 8, of 8192 values or so, or 8 longer rows; out of padded rows it reads up to 14 bytes behind the last of them.
 struct HeadRepack {
     bf16_t *dst;
     const void *src;
@@ -1048,7 +1072,7 @@ struct HeadPlan {
     int parts;                 // of a token's sum
     int64_t split_v;
     // offsets in the workspace
-    int64_t xc, pos, count, lse, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
+    int64_t xc, pos, counts, count, lse, factor, label, wc, part, nll, picked, g, dx, dw, product, product_bytes, total;
 };
 // Tokens up to which a copy of the rows that count costs more than leaving some out gains: one tile of tokens either way.
 constexpr int64_t HD_FEW = HF_T;
@@ -1102,6 +1126,7 @@ static HeadPlan head_plan(int64_t tokens, int64_t dim, int64_t classes, int dtyp
     h.direct = dtype != RDB_F32 && !backward && tokens <= HD_FEW && wide_x;
     if (f32 ? want_dw : !h.direct) h.xc = room(tokens * h.dp * es);
     if (!f32 && !h.direct) h.pos = room(tokens * 4);
+    if (!f32 && tokens > HD_COUNTED) h.counts = room(cdiv(tokens, HD_COUNT) * 4);
     h.count = room(8);
     if (h.pack_w) h.wc = room(classes * h.dp * 2 * h.planes);
     if (!backward) {
@@ -1190,10 +1215,16 @@ static int head_gather(const HeadCall &c, const float *stats, const float *dloss
         p.dim = h.dim;
         p.classes = h.classes;
         p.ignore = c.ignore;
-        p.rows = h.tokens > 16384 ? 64 : h.tokens > 4096 ? 8 : 4;
+        p.rows = h.tokens > HD_COUNTED ? 64 : h.tokens > 4096 ? 8 : 4;
         gathering = cdiv(h.tokens, p.rows);
     }
     if (!gathering && !r.blocks) return RDB_OK;
+    if (gathering && h.tokens > HD_COUNTED) {
+        int *counts = c.at<int>(h.counts);
+        head_count_kernel<<<(unsigned)cdiv(h.tokens, HD_COUNT), 256, 0, c.s>>>(counts, c.target, h.tokens, c.ignore);
+        if (int rc = check_launch("head_count_kernel")) return rc;
+        p.counts = counts;
+    }
     if (h.planes > 1) head_gather_kernel<true><<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
     else head_gather_kernel<false><<<(unsigned)(gathering + r.blocks), 256, 0, c.s>>>(p, r, (int)gathering);
     return check_launch("head_gather_kernel");
