@@ -558,10 +558,12 @@ int rdb_causal_attention_bwd(void *dqkv, const void *dy, const void *y, const vo
  * sums; fp32: at the accuracy of rdb_product_f32).
  *   reduction  0: loss[tokens] (0 where target == ignore_index); 1: loss[0], the mean over the other rows (NaN of none); 2: loss[0], their sum
  *   stats      tokens + 1 floats, for the backward call: log of every row's sum of exponentials, and (reductions 1 and 2) the number of rows that count
- * A target outside the classes makes its row's loss and gradients NaN.  Rows with target == ignore_index are not read.
+ * A target outside the classes makes its row's loss and gradients NaN.  What rows with target == ignore_index hold reaches no
+ * result.
  * Backward: dloss[tokens] for reduction 0, dloss[0] otherwise; dx [tokens x dim] and dw [classes x dim] contiguous, of `dtype`, overwritten,
  * 16-byte aligned, NULL where not wanted.  G = (softmax - onehot) is formed from the logits computed again, a piece of the vocabulary at
- * a time, of which the workspace holds two, of up to 512 MB each (bf16: rounded to bf16 without the factor that its rows share).  Sums in fixed orders: results are bitwise reproducible.
+ * a time, of which the workspace holds two, of up to 512 MB each (bf16: rounded to bf16 without the factor that its rows share, which
+ * makes dx and dw 1.2 times as far from 64 bits as their own rounding does, 1.35 times with reduction 0).  Sums in fixed orders: results are bitwise reproducible.
  * fp32 of many tokens runs on the bf16 matrix cores in three planes, which take 1.5 times the weight's bytes of the workspace.  Infinities in w are what they are in a product at every
  * size: a class whose logit is -infinity counts for nothing.
  * The workspace's size depends on where x and w begin; of its query `backward` is 1 for a backward call, 0 for a forward call and 2 for a forward call that is given a buffer of logits.  RDB_E_UNSUPPORTED: x of 2^29 values or more, 2^21 rows or more, ldw of 2^20 or more,

@@ -4,8 +4,8 @@
 //   lse[t] = log sum_v exp <x_t, w_v>,  nll[t] = lse[t] - <x_t, w_target[t]>,  loss = their mean, their sum, or nll itself
 //   G[t][v] = (exp(<x_t, w_v> - lse[t]) - [v == target[t]]) g_t,   dx = G . W,   dW = G^T . x
 //
-// Rows whose target is the ignored label are left out before anything is multiplied (head_gather_kernel): they cost nothing, and what they hold, NaN
-// included, reaches no sum.  A target outside the classes makes its row NaN.
+// What rows hold whose target is the ignored label, NaN included, reaches no sum: they are read and left out before anything is multiplied (head_gather_kernel); up to 64 tokens of a
+// forward call, and in the products of fp32, they are multiplied with the others and left out behind that.  A target outside the classes makes its row NaN.
 //
 // On the tiles of rdb_duo.hpp (bf16; of few tokens on those of rdb_gemm.hpp; fp32 in three bf16 planes, where that is faster):
 //   head_gather_kernel      the rows that count, one after the other, in rows of a multiple of 8 values
@@ -16,14 +16,15 @@
 //   head_products_kernel    dx += G . W and dW = G^T . x of the piece, and the next piece's G, one list of tiles
 //   head_dx_kernel          dx from its sums, back in the rows' own places
 // G leaves without the factor that all its rows share (1 / count, the loss's gradient), which the products' results get in fp32: rounded with it, the targets' values,
-// which are nearly all of the gradient, would all be off by the same rounding.
+// which are nearly all of the gradient, would all be off by the same rounding.  G in 16 bits is a choice: two planes of it would double two of four products.  dx and dW are 1.9e-3 - 2.0e-3 of their norms
+// from 64 bits with it, 2.2e-3 where rows have factors of their own, which are in G; their own rounding alone is 1.7e-3.
 // fp32 otherwise: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between, which of few tokens stay for the
 // backward pass (rdb_linear_cross_entropy_keeps); ignored rows are rows of zeros of G there.
 //
-// Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 68 % of the time at
-// 1.7 GHz in the statistics and in the products alike (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
+// Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 67 % of the time at
+// 1.65 GHz in the statistics and 58 - 64 % at 1.7 - 1.8 GHz in the products (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
 // priority for the main loop all change nothing.  Measured there, us: statistics 540 - 640, by the card (1172 - 990 TFLOP/s; the library's product alone 656), backward 1700 (three
-// products, 1900 GFLOP), a step 2310; 8192 x 256 -> 50304 1030; 4096 x 4096 -> 65536 7080 (four products, 1240 TFLOP/s).
+// products, 1900 GFLOP), a step 2330; 8192 x 256 -> 50304 1060; 4096 x 4096 -> 65536 7080 (four products, 1240 TFLOP/s).
 #include "rdb_duo.hpp"
 #include "rdb_f32.hpp"
 #include <algorithm>
@@ -531,6 +532,7 @@ template <bool GRAD, bool SOLO, bool PLANES> __device__ __forceinline__ void hea
     if constexpr (GRAD) head_leave_grad<DUO_MI, DUO_NI, PLANES>(acc, lds, p, tv, tok0, count, (int)threadIdx.x);
     else head_leave_stats<DUO_MI, DUO_NI>(acc, p, tv, tok0, count, (int)threadIdx.x);
 }
+// Two blocks a compute unit have 256 registers a lane, accumulators among them: 208 and 222 (head_products_kernel) in bf16; G in planes, whose accumulators are taken apart in place, spills 12 and 13.
 template <bool GRAD, bool PLANES> __global__ __launch_bounds__(256, 2) void head_logits_duo_kernel(HeadLogits p)
 {
     __shared__ __align__(16) bf16_t lds[DUO_LDS];

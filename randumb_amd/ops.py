@@ -545,8 +545,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     fp32 of many tokens: 6); and copies of weights that are not read as they are (bf16 rows of no multiple of 16 bytes, fp32 of many tokens: 6 bytes a value).
 
     ``x`` (..., dim) and ``weight`` (classes, dim): both bf16 or both fp32, on one GPU; ``target`` (...): int64 or int32.  The loss is fp32; logits are
-    not rounded on the way.  Tokens whose target is ``ignore_index`` are left out (in bf16, and in fp32 of many tokens, before anything is multiplied): what their rows hold does not matter.  The mean over no tokens is
-    NaN, with gradients of zero; a target outside the classes makes its token's loss and gradients NaN.  First derivatives only."""
+    not rounded on the way; their gradient is, to bf16, for bf16 inputs.  Tokens whose target is ``ignore_index`` are left out (of more than 64 tokens in bf16, and of many in fp32, before
+    anything is multiplied): what their rows hold does not matter.  A class whose logits are -infinity, or far below the others, counts for nothing.  The mean over no tokens is
+    NaN, with gradients of zero; a target outside the classes makes its token's loss and gradients NaN.  First derivatives only.  Up to 2^21 tokens, x of less than 2^29 values,
+    rows of the weight of less than 2^20."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if hasattr(weight, "get_materialized") or hasattr(x, "get_materialized"):
