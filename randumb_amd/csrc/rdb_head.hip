@@ -21,9 +21,9 @@
 // fp32 otherwise: the products of rdb_f32.hip, or of few tokens head_few_*_kernel, logits of a piece in fp32 in between, which of few tokens stay for the
 // backward pass (rdb_linear_cross_entropy_keeps); ignored rows are rows of zeros of G there.
 //
-// Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 67 % of the time at
-// 1.65 GHz in the statistics and 58 - 64 % at 1.7 - 1.8 GHz in the products (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
-// priority for the main loop all change nothing.  Measured there, us: statistics 540 - 640, by the card (1172 - 990 TFLOP/s; the library's product alone 656), backward 1700 (three
+// Bound by the matrix cores, and these by their power: with 1 - 2 us of their own behind every tile hidden (two blocks a compute unit) the matrix cores are busy 66 % of the time at
+// 1.65 GHz in the statistics and 58 - 65 % at 1.75 - 1.8 GHz in the products (8192 tokens x 768 -> 50304).  Requesting a block's next tile before its epilogue, other orders of the tiles and a higher
+// priority for the main loop all change nothing.  Measured there, us: statistics 550 - 680, by the card (1150 - 930 TFLOP/s; the library's product alone 656), backward 1700 (three
 // products, 1900 GFLOP), a step 2330; 8192 x 256 -> 50304 1060; 4096 x 4096 -> 65536 7080 (four products, 1240 TFLOP/s).
 #include "rdb_duo.hpp"
 #include "rdb_f32.hpp"
