@@ -1510,7 +1510,7 @@ extern "C" int64_t rdb_linear_cross_entropy_workspace_bytes(int64_t tokens, int6
 {
     if (check_head("rdb_linear_cross_entropy_workspace_bytes", tokens, dim, classes, dtype, ldx, ldw, 0)) return 0;
     const bool kept = backward == 2 && rdb_linear_cross_entropy_keeps(tokens, dim, classes, dtype, ldw);
-    return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward == 1, want_dx != 0, want_dw != 0, kept).total;
+    return head_plan_of(tokens, dim, classes, dtype, x, ldx, w, ldw, backward != 0 && backward != 2, want_dx != 0, want_dw != 0, kept).total;
 }
 
 extern "C" int rdb_linear_cross_entropy_fwd(float *loss, float *stats, float *logits, const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, const int64_t *target,
